@@ -124,6 +124,9 @@ _SIGNATURES = {
     "gi_argmax": [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_long, c_void_p],
     "gi_sample_temperature": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_long, c_void_p],
     "gi_sample_filtered": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_long, c_void_p],
+    "gi_verify_drafts": [c_void_p, c_int, c_long, c_void_p, c_long, c_long, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p],
+    "gi_adapters_add": [c_void_p, c_int, c_long, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_long, c_void_p, c_int, c_long, c_void_p, c_int, c_int, c_int, c_int,
+                        c_int, c_void_p, c_int, c_void_p],
 }
 
 _lib = None
@@ -141,6 +144,10 @@ def lib():
         l.gi_argmax_chunks.restype = c_int
         l.gi_sample_filtered_histogram_bytes.argtypes = []
         l.gi_sample_filtered_histogram_bytes.restype = c_int
+        l.gi_verify_drafts_scratch_bytes.argtypes = [c_int, c_int, c_int]
+        l.gi_verify_drafts_scratch_bytes.restype = c_long
+        l.gi_adapters_scratch_floats.argtypes = [c_int, c_int, c_int]
+        l.gi_adapters_scratch_floats.restype = c_long
         l.gi_attention_exact_spans.argtypes = [c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int]
         l.gi_attention_exact_spans.restype = c_int
         l.gi_attention_exact_part_floats.argtypes = [c_int, c_int, c_int, c_int, c_int, c_int, c_int]
@@ -337,6 +344,15 @@ def _i32(t, what, n=None):
 
 def _ptr(t):
     return None if t is None else t.data_ptr()
+
+
+def _here(what, *tensors):
+    """The operands lie on the device whose stream the kernels are launched on."""
+    _dev(*tensors)
+    current = torch.cuda.current_device()
+    for t in tensors:
+        if t is not None and t.device.index != current:
+            raise KernelError(f"{what}: an operand lies on {t.device}, the current device is cuda:{current}")
 
 
 def device_arch() -> str:
@@ -2145,6 +2161,104 @@ def sample_filtered(logits, temperature, top_k, top_p, uniform, out):
     tops = torch.empty(n * lib().gi_sample_filtered_histogram_bytes() // 8, dtype=torch.int64, device=logits.device)
     _call("gi_sample_filtered", logits.data_ptr(), temperature.data_ptr(), top_k.data_ptr(), top_p.data_ptr(), uniform.data_ptr(),
           out.data_ptr(), part_m.data_ptr(), part_s.data_ptr(), kept.data_ptr(), tops.data_ptr(), n, vocab, logits.stride(0), _stream())
+    return out
+
+
+# ------------------------------------------------------------------------------------------------ drafted tokens
+VERIFY_MAX_DRAFTS = 64
+
+
+def verify_drafts(logits, drafts, temperature, uniform, tokens, counts, draft_logits=None, n_drafts=None, first_row=None):
+    """Judges the drafted tokens of many requests against the target's probabilities.  Request r brings drafts[r, :n_drafts[r]] (int32 [requests, K];
+    n_drafts None: K each) and n_drafts[r] + 1 rows of `logits` (float32 [rows, vocab]) from row first_row[r] on (None: r (K + 1)), row j the target's
+    before draft j.  draft_logits: float32 [requests, K, vocab], what draft j was drawn from at the same temperature; None: drafts that
+    no probabilities belong to (a lookup), of which each stays with the target's own probability of it.  temperature: float32 [requests], 0 (and what is not
+    greater) for the arg max.  uniform: float32 [requests, K + 1] in [0, 1): u[r, j] decides over draft j, u[r, K] draws the token behind those that stay.
+
+    tokens, int32 [requests, K + 1], receives the drafts that stay, the token behind them and then -1; counts, int32 [requests], how many tokens those are.
+    A draft x stays if those before it do and u q(x) < p(x) (arg max: if it is the row's lowest arg max); the token behind is drawn in index order
+    from max(p - q, 0) where a draft fell and from p where none did.  Logits of -infinity or NaN are no tokens (a row of nothing else lets no draft stay and gives token
+    0), a draft outside the vocabulary falls.  A request whose rows do not lie among those given gets count 0."""
+    what = "verify_drafts"
+    if not (logits.dtype == torch.float32 and logits.dim() == 2 and logits.shape[1] > 0 and (logits.stride(1) == 1 or logits.shape[1] == 1)):
+        raise KernelError(f"{what}: logits must be float32 [rows, vocab] with unit inner stride")
+    if not (drafts.dtype == torch.int32 and drafts.dim() == 2 and drafts.is_contiguous()):
+        raise KernelError(f"{what}: drafts must be a contiguous int32 [requests, K] tensor")
+    (n_rows, vocab), (n, k) = logits.shape, drafts.shape
+    if k > VERIFY_MAX_DRAFTS:
+        raise KernelError(f"{what}: {k} drafts a request, at most {VERIFY_MAX_DRAFTS} are taken")
+    for t, name, shape in ((temperature, "temperature", (n,)), (uniform, "uniform", (n, k + 1))):
+        if not (t.dtype == torch.float32 and t.is_contiguous() and t.shape == shape):
+            raise KernelError(f"{what}: {name} must be a contiguous float32 tensor of shape {shape}")
+    for t, name, shape in ((tokens, "tokens", (n, k + 1)), (counts, "counts", (n,)), (n_drafts, "n_drafts", (n,)), (first_row, "first_row", (n,))):
+        if t is not None and not (t.dtype == torch.int32 and t.is_contiguous() and t.shape == shape):
+            raise KernelError(f"{what}: {name} must be a contiguous int32 tensor of shape {shape}")
+    if draft_logits is not None and not (draft_logits.dtype == torch.float32 and draft_logits.shape == (n, k, vocab) and (draft_logits.stride(2) == 1 or vocab == 1)):
+        raise KernelError(f"{what}: draft_logits must be float32 {(n, k, vocab)} with unit inner stride")
+    if first_row is None and n_drafts is None and n_rows < n * (k + 1):
+        raise KernelError(f"{what}: {n} requests of {k} drafts need {n * (k + 1)} rows of logits, there are {n_rows}")
+    if n == 0:
+        return tokens, counts
+    if n_rows == 0:
+        raise KernelError(f"{what}: there are no rows of logits")
+    _here(what, logits, drafts, temperature, uniform, tokens, counts, draft_logits, n_drafts, first_row)
+    scratch = torch.empty(lib().gi_verify_drafts_scratch_bytes(n, k, vocab), dtype=torch.uint8, device=logits.device)
+    drafter = draft_logits if k > 0 else None
+    _call("gi_verify_drafts", logits.data_ptr(), n_rows, logits.stride(0) if n_rows > 1 else max(logits.stride(0), vocab), _ptr(drafter), drafter.stride(0) if drafter is not None else 0,
+          drafter.stride(1) if drafter is not None else 0, drafts.data_ptr(), _ptr(n_drafts), _ptr(first_row), temperature.data_ptr(), uniform.data_ptr(), tokens.data_ptr(),
+          counts.data_ptr(), scratch.data_ptr(), n, k, vocab, _stream())
+    return tokens, counts
+
+
+# ------------------------------------------------------------------------------------------------ adapters
+ADAPTER_MAX_SLICES = 4
+
+
+def adapters_check(x, a, b, ids, out, scales, base, slices):
+    """The columns of the packed projections, once `adapters_add` can take the operands; KernelError if not."""
+    what = "adapters_add"
+    if not (x.dim() == 2 and a.dim() == 3 and b.dim() == 3 and out.dim() == 2):
+        raise KernelError(f"{what}: x [rows, width], a [adapters, ranks, width], b [adapters, columns, rank] and out [rows, columns] are needed")
+    (n, width), (n_adapters, columns, rank) = x.shape, b.shape
+    slices = (columns,) if slices is None else tuple(int(c) for c in slices)
+    if not (1 <= len(slices) <= ADAPTER_MAX_SLICES and min(slices) > 0 and sum(slices) == columns):
+        raise KernelError(f"{what}: slices {slices} are not 1 to {ADAPTER_MAX_SLICES} positive numbers that add up to the {columns} columns")
+    if not (a.shape == (n_adapters, len(slices) * rank, width) and out.shape == (n, columns) and base.shape == (n, columns)):
+        raise KernelError(f"{what}: x {tuple(x.shape)}, a {tuple(a.shape)}, b {tuple(b.shape)}, base {tuple(base.shape)} and out {tuple(out.shape)} do not fit ({len(slices)} projections)")
+    if 0 in (width, rank, n_adapters):
+        raise KernelError(f"{what}: {n_adapters} adapters of rank {rank} beside a width of {width} have no entries")
+    if not (a.dtype == b.dtype and a.is_contiguous() and b.is_contiguous()):
+        raise KernelError(f"{what}: a and b must be contiguous and of one dtype")
+    if not (ids.dtype == torch.int32 and ids.is_contiguous() and ids.shape == (n,)):
+        raise KernelError(f"{what}: ids must be a contiguous int32 [rows] tensor")
+    if scales is not None and not (scales.dtype == torch.float32 and scales.is_contiguous() and scales.shape == (n_adapters,)):
+        raise KernelError(f"{what}: scales must be a contiguous float32 [adapters] tensor")
+    for t, name in ((x, "x"), (a, "a"), (base, "base"), (out, "out")):
+        _code(t, f"{what}: {name}")
+    for t, name in ((x, "x"), (base, "base"), (out, "out")):
+        if not ((t.stride(1) == 1 or t.shape[1] == 1) and (n <= 1 or t.stride(0) >= t.shape[1])):
+            raise KernelError(f"{what}: {name} must have unit inner stride and rows that do not overlap")
+    if n:
+        _here(what, x, a, b, ids, out, scales, base)
+    return slices
+
+
+def adapters_add(x, a, b, ids, out, scales=None, base=None, slices=None):
+    """out[t] = base[t] + scales[e] * (b[e] @ (a[e] @ x[t])) with e = ids[t], the low-rank adapter of row t's request; out[t] = base[t] where ids[t] is
+    none of 0 .. adapters-1.  x float32 or bfloat16 [rows, width], a [adapters, rank, width] and b [adapters, columns, rank] of one dtype
+    (either), contiguous; ids int32 [rows] in any order; scales float32 [adapters], None for 1; base float32 or bfloat16 [rows, columns], None: out itself (it may
+    also be given as both, but otherwise out shares no memory with an operand); out likewise.  slices: the columns of the projections that out packs, in their order
+    (at most ADAPTER_MAX_SLICES); a then holds a block of `rank` rows for each, [adapters, len(slices) * rank, width].  Adapters of smaller rank are filled up with zeros.
+    Sums are in 32 bits; a row's result does not depend on what the other rows hold, and with float32 x not on how many there are either."""
+    base = out if base is None else base
+    slices = adapters_check(x, a, b, ids, out, scales, base, slices)
+    (n, width), (n_adapters, columns, rank) = x.shape, b.shape
+    if n == 0:
+        return out
+    t = torch.empty(lib().gi_adapters_scratch_floats(n, width, len(slices) * rank), dtype=torch.float32, device=x.device)
+    _call("gi_adapters_add", x.data_ptr(), _CODE[x.dtype], max(x.stride(0), width), a.data_ptr(), b.data_ptr(), _CODE[a.dtype], ids.data_ptr(), _ptr(scales), base.data_ptr(),
+          _CODE[base.dtype], max(base.stride(0), columns), out.data_ptr(), _CODE[out.dtype], max(out.stride(0), columns), t.data_ptr(), n, width, columns, rank, len(slices),
+          (c_int * len(slices))(*slices), n_adapters, _stream())
     return out
 
 

@@ -11,17 +11,33 @@ times the norm's weights in bfloat16 and the pieces of their sums of squares, th
 multiplies its results by the rows' rsqrt(mean square + eps)."""
 from __future__ import annotations
 
+from dataclasses import dataclass
+from typing import Optional, Sequence
+
 import torch
 
 from ..kernels import ops
 from .norm import HandedRows, NormedRows, NormToMake, ReadyRows
 
 
+@dataclass
+class RowAdapters:
+    """Low-rank adapters beside one projection and which of them each row of a batch takes (`ops.adapters_add`)."""
+    down: torch.Tensor                              # [adapters, len(slices) * rank, in_features]
+    up: torch.Tensor                                # [adapters, out_features, rank]
+    ids: torch.Tensor                               # int32 [rows]: each row's adapter, -1 for none
+    scales: Optional[torch.Tensor] = None           # float32 [adapters]
+    slices: Optional[Sequence[int]] = None          # output features of the projections that the weight packs
+
+
 def linear(a, weight: torch.Tensor, out: torch.Tensor, accumulate: bool = False, gated: bool = False, gate_limit: float = 0.0,
-           ctx=None) -> torch.Tensor:
+           ctx=None, adapters: Optional[RowAdapters] = None) -> torch.Tensor:
     """gated: weight is [gate; up] interleaved by `ops.interleave_gate_up` and out = act(gate) * up (bfloat16 only); True or "silu"
     for SiLU, "gelu_tanh" for the tanh form of GELU, "swish_clamped" (with `gate_limit`) for the clamped form.  ctx: the step the product is one
-    of, whose counters (`ops.step_counters`) save it a launch where it has a use for them."""
+    of, whose counters (`ops.step_counters`) save it a launch where it has a use for them.  adapters: every row's own adapter beside the weight; the sum
+    of both products is rounded once, to out's dtype."""
+    if adapters is not None:
+        return _linear_adapted(a, weight, out, accumulate, gated, ctx, adapters)
     if isinstance(a, HandedRows):
         if (weight.dtype == torch.bfloat16 and ops.gemm_bf16_supports(a.scaled, weight, out)
                 and ops.gemm_bf16_takes_norm(a.scaled.shape[0], weight.shape[0], weight.shape[1], gated)):
@@ -33,6 +49,21 @@ def linear(a, weight: torch.Tensor, out: torch.Tensor, accumulate: bool = False,
     if gated:
         raise ops.KernelError("the gated product exists for bfloat16 operands only")
     return ops.gemm_exact(a, weight, out, accumulate)
+
+
+def _linear_adapted(a, weight, out, accumulate, gated, ctx, adapters):
+    if gated:
+        raise ops.KernelError("a gated product takes no adapters: they belong before its activation")
+    if isinstance(a, NormedRows):
+        a = a.materialize()
+    if accumulate and out.dtype != torch.float32:
+        raise ops.KernelError("a product with adapters adds onto float32 rows only")
+    ops.adapters_check(a, adapters.down, adapters.up, adapters.ids, out, adapters.scales, out, adapters.slices)      # (before the shared product changes out)
+    if out.dtype == torch.float32:
+        shared = linear(a, weight, out, accumulate, ctx=ctx)
+    else:                                           # in 32 bits until the adapters' share is in
+        shared = linear(a, weight, torch.empty(out.shape, dtype=torch.float32, device=out.device), ctx=ctx)
+    return ops.adapters_add(a, adapters.down, adapters.up, adapters.ids, out, scales=adapters.scales, base=shared, slices=adapters.slices)
 
 
 def linear_xielu(a, weight: torch.Tensor, params: torch.Tensor, columns: int, dtype: torch.dtype, out: torch.Tensor = None, into: torch.Tensor = None):
