@@ -40,7 +40,8 @@ def adapter_args(n=5, width=16, columns=12, rank=4, adapters=3, slices=1):
     (dict(a=torch.zeros(3, 16, 4).transpose(1, 2)), "contiguous"), (dict(a=torch.zeros(3, 4, 16, dtype=torch.bfloat16)), "one dtype"), (dict(b=torch.zeros(2, 12, 4)), "do not fit"),
     (dict(ids=torch.zeros(5, dtype=torch.int64)), "ids"), (dict(ids=torch.zeros(4, dtype=torch.int32)), "ids"), (dict(scales=torch.ones(2)), "scales"),
     (dict(scales=torch.ones(3, dtype=torch.bfloat16)), "scales"), (dict(slices=(6, 5)), "slices"), (dict(slices=(12, 0)), "slices"), (dict(slices=()), "slices"),
-    (dict(slices=(3, 3, 2, 2, 2)), "slices"), (dict(slices=(6, 6)), "do not fit"), (dict(a=torch.zeros(3, 0, 16), b=torch.zeros(3, 12, 0)), "no entries"), ({}, "device memory"),
+    (dict(slices=(3, 3, 2, 2, 2)), "slices"), (dict(slices=(6, 6)), "do not fit"), (dict(a=torch.zeros(3, 0, 16), b=torch.zeros(3, 12, 0)), "no entries"),
+    (dict(a=torch.zeros(3, 257, 16), b=torch.zeros(3, 12, 257)), "at most 256"), ({}, "device memory"),
 ])
 def test_adapters_refuse(change, message):
     with pytest.raises(ops.KernelError, match=message):
