@@ -5,24 +5,25 @@
 // each and the columns of projection s read block s.  A number outside 0 .. adapters-1 is no adapter: out[t] = base[t].
 //
 // Both ways are matrix products of few ranks (8 to 64 as a rule), far below the matrix cores' rate: what bounds them is the traffic, x once on the way
-// down, base and out once on the way up, and, for a few rows with an adapter each, the adapters themselves.  Two launches.  Down: a
-// workgroup takes a tile of rows, up to 64 ranks and a segment of the width, which its four waves share out, so that none loads what another does;
-// the segments' sums go to scratch.  Up: a workgroup adds the segments' sums of its tile of rows, keeps them in LDS and walks a strip of columns.
-//
-// Rows of one tile may take different adapters.  In a product D = M N with the rows as N's columns a lane of the matrix core's result holds values of one row only, so a
-// tile is multiplied by an adapter as it is and the lanes of other rows drop what comes out: no operand is masked, and what one request's rows or matrices hold,
-// numbers or not, cannot reach another's.  The tile's different adapters are counted off: workgroup z of `slots` takes every slots-th of them.
+// down, base and out once on the way up, and, for a few rows with an adapter each, the adapters themselves.  Two launches, which leave the sums A x of every
+// row in scratch between them.  A few rows are taken one by one (the last kernels below).  More are cut into tiles: runs of neighbours with one adapter, ended at every 64th row too, as a
+// request's rows lie together.  How many tiles there are only the device knows: every workgroup of the way down counts them for itself and takes every so manieth piece of work, and they leave the way up a list.
 #include "common.h"
+
+#include <type_traits>
 
 namespace {
 
 constexpr int MAX_SLICES = 4;
 constexpr int MAX_RANK = 256;
-constexpr int WAVES = 4;
-constexpr int SEGMENT = 512;                // of the width: what a workgroup of the way down takes at least, and always in 32 bits, where the order of a sum must not depend on the batch
+constexpr int DOWN_WAVES = 2, DOWN_NT = 64 * DOWN_WAVES, UP_WAVES = 4, UP_NT = 64 * UP_WAVES;
+constexpr int SEGMENT = 256;                // of the width: the least that a workgroup of the way down takes
+constexpr int EXACT_SEGMENT = 256;          // what it always takes in 32 bits, where the order of a sum must not depend on the batch
+constexpr int TILE = 64;                    // rows
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float floatx4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) void* lds_ptr_t;
 
 struct Slices {                             // of the columns: slice s begins at begin[s] and reads block s of the ranks; its strips begin at strip[s]
     int n;
@@ -35,11 +36,15 @@ struct Slices {                             // of the columns: slice s begins at
 template <bool LOW> struct Piece;
 template <> struct Piece<true> {            // bfloat16: 128 bytes of a row a block, two instructions
     static constexpr int BLOCK = 64, RUN = 8;
-    uint4 v[2];
+    typedef bf16_t T;
+    typedef uint4 V;
+    V v[2];
 };
 template <> struct Piece<false> {           // 32 bits: 128 bytes a block, eight instructions
     static constexpr int BLOCK = 32, RUN = 4;
-    float4 v[2];
+    typedef float T;
+    typedef float4 V;
+    V v[2];
 };
 
 __device__ __forceinline__ floatx4 times(const Piece<true>& m, const Piece<true>& n, floatx4 sum) {
@@ -47,21 +52,23 @@ __device__ __forceinline__ floatx4 times(const Piece<true>& m, const Piece<true>
     for (int h = 0; h < 2; ++h) sum = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, m.v[h]), __builtin_bit_cast(bf16x8, n.v[h]), sum, 0, 0, 0);
     return sum;
 }
-__device__ __forceinline__ floatx4 times(const Piece<false>& m, const Piece<false>& n, floatx4 sum) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        sum = __builtin_amdgcn_mfma_f32_16x16x4f32(m.v[h].x, n.v[h].x, sum, 0, 0, 0);
-        sum = __builtin_amdgcn_mfma_f32_16x16x4f32(m.v[h].y, n.v[h].y, sum, 0, 0, 0);
-        sum = __builtin_amdgcn_mfma_f32_16x16x4f32(m.v[h].z, n.v[h].z, sum, 0, 0, 0);
-        sum = __builtin_amdgcn_mfma_f32_16x16x4f32(m.v[h].w, n.v[h].w, sum, 0, 0, 0);
-    }
-    return sum;
+__device__ __forceinline__ floatx4 times(const float4& m, const float4& n, floatx4 sum) {
+    sum = __builtin_amdgcn_mfma_f32_16x16x4f32(m.x, n.x, sum, 0, 0, 0);
+    sum = __builtin_amdgcn_mfma_f32_16x16x4f32(m.y, n.y, sum, 0, 0, 0);
+    sum = __builtin_amdgcn_mfma_f32_16x16x4f32(m.z, n.z, sum, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_16x16x4f32(m.w, n.w, sum, 0, 0, 0);
 }
+__device__ __forceinline__ floatx4 times(const Piece<false>& m, const Piece<false>& n, floatx4 sum) { return times(m.v[1], n.v[1], times(m.v[0], n.v[0], sum)); }
 
-// Numbers k .. k + RUN of a row, 0 from `end` on.  ALIGNED: `end` is a multiple of RUN and the row begins at a whole run of loads.
+// Numbers k .. k + RUN of a row, 0 from `end` on.  ALIGNED: `end` is a multiple of RUN, not 0, and the row begins at a whole run of loads.  What lies beyond is asked for at the last
+// run's place and dropped: a branch around a load would make the wave wait for all its loads where the first is used.
 template <bool ALIGNED>
 __device__ __forceinline__ uint4 load_run(const bf16_t* __restrict__ row, int k, int end) {
-    if (ALIGNED) return k < end ? *reinterpret_cast<const uint4*>(row + k) : uint4{0u, 0u, 0u, 0u};
+    if (ALIGNED) {
+        const uint4 v = *reinterpret_cast<const uint4*>(row + min(k, end - 8));
+        const bool in = k < end;
+        return uint4{in ? v.x : 0u, in ? v.y : 0u, in ? v.z : 0u, in ? v.w : 0u};
+    }
     uint32_t v[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = k + i < end ? row[k + i] : 0u;
@@ -69,7 +76,11 @@ __device__ __forceinline__ uint4 load_run(const bf16_t* __restrict__ row, int k,
 }
 template <bool ALIGNED>
 __device__ __forceinline__ float4 load_run_f32(const float* __restrict__ row, int k, int end) {
-    if (ALIGNED) return k < end ? *reinterpret_cast<const float4*>(row + k) : float4{0.f, 0.f, 0.f, 0.f};
+    if (ALIGNED) {
+        const float4 v = *reinterpret_cast<const float4*>(row + min(k, end - 4));
+        const bool in = k < end;
+        return float4{in ? v.x : 0.f, in ? v.y : 0.f, in ? v.z : 0.f, in ? v.w : 0.f};
+    }
     float v[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[i] = k + i < end ? row[k + i] : 0.f;
@@ -78,9 +89,9 @@ __device__ __forceinline__ float4 load_run_f32(const float* __restrict__ row, in
 template <bool ALIGNED>
 __device__ __forceinline__ float4 load_run_f32(const bf16_t* __restrict__ row, int k, int end) {
     if (ALIGNED) {
-        if (k >= end) return float4{0.f, 0.f, 0.f, 0.f};
-        const uint2 v = *reinterpret_cast<const uint2*>(row + k);
-        return float4{__uint_as_float(v.x << 16), __uint_as_float(v.x & 0xffff0000u), __uint_as_float(v.y << 16), __uint_as_float(v.y & 0xffff0000u)};
+        const uint2 v = *reinterpret_cast<const uint2*>(row + min(k, end - 4));
+        const bool in = k < end;
+        return float4{in ? __uint_as_float(v.x << 16) : 0.f, in ? __uint_as_float(v.x & 0xffff0000u) : 0.f, in ? __uint_as_float(v.y << 16) : 0.f, in ? __uint_as_float(v.y & 0xffff0000u) : 0.f};
     }
     float v[4];
 #pragma unroll
@@ -98,348 +109,740 @@ __device__ __forceinline__ void load_piece(Piece<false>& p, const T* __restrict_
     for (int h = 0; h < 2; ++h) p.v[h] = load_run_f32<ALIGNED>(row, k + 16 * h + 4 * group, end);
 }
 
-// The different adapters of a tile of at most 64 rows, one after the other: `next` gives the next one and the rows that take it, as bits.  Every
-// wave of a workgroup counts them off for itself.
-struct Tile {
-    int id;                                 // this lane's row's adapter, -1 for none
-    unsigned long long left;                // rows whose adapter has not come yet
+// The tiles of a batch, counted by every workgroup: a tile begins at every 64th row and where a row's adapter is not its neighbour's.
+constexpr int COUNTS = 1024;
+struct Tiles {
+    const int* ids;
+    int n_rows, each, entries;              // rows; blocks of 64 rows that one count is of; counts
 
-    __device__ Tile(const int* __restrict__ ids, int first, int rows, int n_rows, int n_adapters) {
-        const int lane = threadIdx.x & 63;
-        id = -1;
-        if (lane < rows && first + lane < n_rows) id = ids[first + lane];
-        if (id >= n_adapters) id = -1;
-        left = __ballot(id >= 0);
+    __device__ unsigned long long begins(int block) const {            // the rows of a block at which tiles begin
+        const int lane = threadIdx.x & 63, i = block * TILE + lane, mine = ids[min(i, n_rows - 1)], neighbour = __shfl_up(mine, 1, 64);
+        return __ballot(i < n_rows && (lane == 0 || mine != neighbour));
     }
-    __device__ int next(unsigned long long& rows) {
-        const int e = __shfl(id, __ffsll((long long)left) - 1, 64);
-        rows = __ballot(id == e);
-        left &= ~rows;
-        return e;
+    // before[c]: tiles before the rows of count c; the number of all tiles comes back.
+    __device__ int count(int* before) {
+        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, blocks = (n_rows + TILE - 1) / TILE;
+        each = (blocks + COUNTS - 1) / COUNTS;
+        entries = (blocks + each - 1) / each;
+        constexpr int AT_ONCE = 8;                                     // counts of a wave whose rows' numbers are asked for together
+        for (int c = wave; c < entries; c += AT_ONCE * DOWN_WAVES) {
+            int sum[AT_ONCE] = {};
+            for (int b = 0; b < each; ++b) {
+#pragma unroll
+                for (int u = 0; u < AT_ONCE; ++u) sum[u] += __popcll(begins((c + u * DOWN_WAVES) * each + b));       // (a block beyond the rows has none)
+            }
+#pragma unroll
+            for (int u = 0; u < AT_ONCE; ++u)
+                if (lane == 0 && c + u * DOWN_WAVES < entries) before[c + u * DOWN_WAVES] = sum[u];
+        }
+        __syncthreads();
+        // every wave adds the counts up for itself and wave 0 lays the sums down
+        int total = 0;
+        int mine[COUNTS / 64];
+#pragma unroll
+        for (int u = 0; u < COUNTS / 64; ++u) {
+            if (u * 64 >= entries) break;
+            const int c = u * 64 + lane, v = c < entries ? before[c] : 0;
+            int upto = v;
+#pragma unroll
+            for (int off = 1; off < 64; off <<= 1) {
+                const int below = __shfl_up(upto, off, 64);
+                if (lane >= off) upto += below;
+            }
+            mine[u] = total + upto - v;
+            total += __shfl(upto, 63, 64);
+        }
+        __syncthreads();
+        if (wave == 0)
+#pragma unroll
+            for (int u = 0; u < COUNTS / 64; ++u) {
+                if (u * 64 >= entries) break;
+                if (u * 64 + lane < entries) before[u * 64 + lane] = mine[u];
+            }
+        __syncthreads();
+        return total;
+    }
+    // Tile `which`: its first row, how many, and their adapter.  The same in every lane.
+    __device__ void find(const int* before, int which, int& first, int& rows, int& id) const {
+        const int lane = threadIdx.x & 63;
+        int c = -1;
+        for (int u = 0; u < entries; u += 64) c += __popcll(__ballot(u + lane < entries && before[u + lane] <= which));      // the last count that begins at or before it
+        int left = which - before[c], block = c * each;
+        unsigned long long at = begins(block);
+        while (left >= __popcll(at)) {
+            left -= __popcll(at);
+            at = begins(++block);
+        }
+        const int place = __ffsll((long long)__ballot((at >> lane & 1) && __popcll(at & ((1ull << lane) - 1)) == left)) - 1;
+        const unsigned long long behind = place < 63 ? at >> (place + 1) : 0;
+        first = __builtin_amdgcn_readfirstlane(block * TILE + place);
+        rows = __builtin_amdgcn_readfirstlane(min(behind != 0 ? __ffsll((long long)behind) : TILE - place, n_rows - block * TILE - place));
+        id = __builtin_amdgcn_readfirstlane(ids[block * TILE + place]);
     }
 };
 
-// Down: sums[segment][row][rank] over a segment of the width.  NT tiles of 16 rows, MT tiles of 16 ranks.  blockIdx: (tile of rows, segment, group of ranks * slots + slot).
-template <bool LOW, typename X, typename W, int NT, int MT, bool ALIGNED>
-__global__ __launch_bounds__(64 * WAVES) void adapters_down_kernel(const X* __restrict__ x, long ldx, const W* __restrict__ a, const int* __restrict__ ids, float* __restrict__ sums,
-                                                                   int n_rows, int width, int ranks, int n_adapters, int segment, int slots) {
+struct Tile {                               // of the list that the way down leaves
+    int first, rows, id, unused;
+};
+
+// ------------------------------------------------------------------ down, in tiles
+// sums[segment][row][rank] of a tile, a segment of the width and a group of 16 MT ranks.  The two waves of a workgroup share out the segment, every second block of 128 bytes a row, so that none
+// loads what the other does.  In the product D = M N the ranks are M's rows and the tile's rows N's columns: a lane of the result has values of one row only, and rows behind the tile's
+// last are loaded as that one and dropped.
+struct Down {
+    Tile* list;
+    int* n_listed;
+    int n_rows, width, ranks, n_adapters, segment, n_segments, n_parts;       // parts: segments times groups of ranks
+    long ldx;
+};
+
+template <int MT>
+__device__ __forceinline__ void store_sums(floatx4 (&sum)[4][MT], unsigned char* meet, float* __restrict__ sums, const Down& d, int segment, int first_row, int rows, int first_rank) {
+    // wave 0's and wave 1's, through `meet`: 8 KB * MT, which no wave reads as anything else any more
+    floatx4* at = (floatx4*)meet;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+            if (16 * j < rows) at[(wave * 4 * MT + j * MT + i) * 64 + lane] = sum[j][i];
+    __syncthreads();
+    for (int item = threadIdx.x; item < 4 * MT * 64; item += DOWN_NT) {
+        const int l = item & 63, j = item / 64 / MT, i = item / 64 % MT;
+        const int row = 16 * j + (l & 15), rank = first_rank + 16 * i + 4 * (l >> 4);
+        if (row >= rows || rank >= d.ranks) continue;
+        const floatx4 s = at[item] + at[item + 4 * MT * 64];
+        float* to = sums + ((size_t)segment * d.n_rows + first_row + row) * d.ranks + rank;
+        if ((d.ranks & 3) == 0) {
+            *reinterpret_cast<floatx4*>(to) = s;
+        } else {
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+                if (rank + c < d.ranks) to[c] = s[c];
+        }
+    }
+    __syncthreads();
+}
+
+// Rows of one type, 16-byte loads.  Global memory goes straight into LDS (a lane's 16 bytes land behind the lane's before it), every wave through a ring of its own, so that no barrier stands in the loop: in registers the
+// operands' layout, neighbouring lanes in different rows, would take a load through the first-level cache in 64 pieces of 16 bytes instead of 16 whole sectors.  A stage is 64 rows of x and 16 MT of A,
+// 128 bytes each, its 16-byte chunk c of a row at place c ^ (row / 2 % 8), so that 16 rows' chunks lie in different banks.
+template <int MT> constexpr int stages_of() { return MT <= 2 ? 3 : 2; }
+template <int MT> constexpr int stage_bytes() { return (TILE + 16 * MT) * 128; }
+
+template <bool LOW, int MT>
+__global__ __launch_bounds__(DOWN_NT) void adapters_down_kernel(const typename Piece<LOW>::T* __restrict__ x, const typename Piece<LOW>::T* __restrict__ a, const int* __restrict__ ids,
+                                                           float* __restrict__ sums, Down d) {
     typedef Piece<LOW> P;
-    __shared__ floatx4 meet[2][NT * MT * 64];
+    typedef typename P::T T;
+    constexpr int STAGES = stages_of<MT>(), BYTES = stage_bytes<MT>(), LOADS = BYTES / 1024, STEP = P::BLOCK * DOWN_WAVES;
+    extern __shared__ __align__(16) unsigned char ring[];
+    __shared__ int before[COUNTS];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, at = lane & 15, group = lane >> 4;
-    const int first_row = blockIdx.x * 16 * NT, slot = blockIdx.z % slots, first_rank = blockIdx.z / slots * 16 * MT;
-    const int begin = blockIdx.y * segment, end = min(width, begin + segment);
-    Tile tile(ids, first_row, 16 * NT, n_rows, n_adapters);
-    const X* xr[NT];
+    Tiles tiles{ids, d.n_rows, 0, 0};
+    const int n_tiles = tiles.count(before);
+    const long n_items = (long)n_tiles * d.n_parts;
+    unsigned char* mine = ring + wave * STAGES * BYTES;
+    const unsigned mine_at = (unsigned)(size_t)(lds_ptr_t)mine;
+    for (long item = blockIdx.x; item < n_items; item += gridDim.x) {
+        int first_row, rows, e;
+        const int part = (int)(item % d.n_parts), which = (int)(item / d.n_parts);
+        tiles.find(before, which, first_row, rows, e);
+        if (part == 0 && threadIdx.x == 0) {
+            d.list[which] = Tile{first_row, rows, e, 0};
+            *d.n_listed = n_tiles;
+        }
+        if (e < 0 || e >= d.n_adapters) continue;
+        const int segment = part % d.n_segments, first_rank = part / d.n_segments * 16 * MT;
+        const int begin = segment * d.segment, end = min(d.width, begin + d.segment), k0 = begin + wave * P::BLOCK;
+        const int whole = max(0, (end - k0 + (DOWN_WAVES - 1) * P::BLOCK) / STEP);          // this wave's blocks
+        const T* ae = a + (size_t)e * d.ranks * d.width;
+        const T* from[LOADS];
 #pragma unroll
-    for (int j = 0; j < NT; ++j) xr[j] = x + (size_t)min(first_row + 16 * j + at, n_rows - 1) * ldx;
-    for (int count = 0; tile.left != 0; ++count) {
-        unsigned long long rows;
-        const int e = tile.next(rows);
-        if (count % slots != slot) continue;
-        const W* ar[MT];
+        for (int i = 0; i < LOADS; ++i) {
+            const int row = 8 * i + (lane >> 3), c = (lane & 7) ^ (row >> 1 & 7);
+            from[i] = (row < TILE ? x + (size_t)(first_row + min(row, rows - 1)) * d.ldx : ae + (size_t)min(first_rank + row - TILE, d.ranks - 1) * d.width) + k0 + P::RUN * c;
+        }
+        auto ask = [&](int block) {
 #pragma unroll
-        for (int i = 0; i < MT; ++i) ar[i] = a + ((size_t)e * ranks + min(first_rank + 16 * i + at, ranks - 1)) * width;
-        floatx4 sum[NT][MT];
+            for (int i = 0; i < LOADS; ++i) {
+                const unsigned to = __builtin_amdgcn_readfirstlane(mine_at + block % STAGES * BYTES + i * 1024);
+                asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(from[i] + (size_t)block * STEP) : "memory", "m0");
+            }
+        };
+        floatx4 sum[4][MT];
 #pragma unroll
-        for (int j = 0; j < NT; ++j)
+        for (int j = 0; j < 4; ++j)
 #pragma unroll
             for (int i = 0; i < MT; ++i) sum[j][i] = floatx4{0.f, 0.f, 0.f, 0.f};
-        constexpr int STEP = P::BLOCK * WAVES;
-        P xp[NT], ap[MT];
-        int k = begin + wave * P::BLOCK;
 #pragma unroll
-        for (int j = 0; j < NT; ++j) load_piece<ALIGNED>(xp[j], xr[j], k, end, group);
+        for (int s = 0; s < STAGES - 1; ++s)
+            if (s < whole) ask(s);
+        for (int block = 0; block < whole; ++block) {
+            // the block before has been read into registers; the next goes where it was
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            if (block + STAGES - 1 < whole) ask(block + STAGES - 1);
+            const int ahead = min(whole - 1 - block, STAGES - 1);                      // blocks that may still be on their way
+            if (ahead >= 2) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * LOADS) : "memory");
+            else if (ahead == 1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LOADS) : "memory");
+            else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            const unsigned char* stage = mine + block % STAGES * BYTES;
+            P ap[MT];
+            const int swizzle = at >> 1;                                               // (16 rows further it is the same)
 #pragma unroll
-        for (int i = 0; i < MT; ++i) load_piece<ALIGNED>(ap[i], ar[i], k, end, group);
-        for (; k < end; k += STEP) {                      // the next block is on its way while this one is multiplied
-            P xn[NT], an[MT];
+            for (int i = 0; i < MT; ++i)
 #pragma unroll
-            for (int j = 0; j < NT; ++j) load_piece<ALIGNED>(xn[j], xr[j], k + STEP, end, group);
+                for (int h = 0; h < 2; ++h)
+                    ap[i].v[h] = *reinterpret_cast<const typename P::V*>(stage + (TILE + 16 * i + at) * 128 + ((4 * h + group) ^ swizzle) * 16);
 #pragma unroll
-            for (int i = 0; i < MT; ++i) load_piece<ALIGNED>(an[i], ar[i], k + STEP, end, group);
+            for (int j = 0; j < 4; ++j) {
+                if (16 * j >= rows) break;
+                P xp;
 #pragma unroll
-            for (int j = 0; j < NT; ++j)
+                for (int h = 0; h < 2; ++h) xp.v[h] = *reinterpret_cast<const typename P::V*>(stage + (16 * j + at) * 128 + ((4 * h + group) ^ swizzle) * 16);
 #pragma unroll
-                for (int i = 0; i < MT; ++i) sum[j][i] = times(ap[i], xp[j], sum[j][i]);
-#pragma unroll
-            for (int j = 0; j < NT; ++j) xp[j] = xn[j];
-#pragma unroll
-            for (int i = 0; i < MT; ++i) ap[i] = an[i];
-        }
-        // (wave 0 + wave 2) + (wave 1 + wave 3)
-        if (wave >= 2) {
-#pragma unroll
-            for (int j = 0; j < NT; ++j)
-#pragma unroll
-                for (int i = 0; i < MT; ++i) meet[wave - 2][(j * MT + i) * 64 + lane] = sum[j][i];
-        }
-        __syncthreads();
-        if (wave < 2) {
-#pragma unroll
-            for (int j = 0; j < NT; ++j)
-#pragma unroll
-                for (int i = 0; i < MT; ++i) sum[j][i] += meet[wave][(j * MT + i) * 64 + lane];
-        }
-        __syncthreads();
-        if (wave == 1) {
-#pragma unroll
-            for (int j = 0; j < NT; ++j)
-#pragma unroll
-                for (int i = 0; i < MT; ++i) meet[0][(j * MT + i) * 64 + lane] = sum[j][i];
-        }
-        __syncthreads();
-        if (wave == 0) {
-#pragma unroll
-            for (int j = 0; j < NT; ++j) {
-                if (!(rows >> (16 * j + at) & 1)) continue;
-                float* to = sums + ((size_t)blockIdx.y * n_rows + first_row + 16 * j + at) * ranks;
-#pragma unroll
-                for (int i = 0; i < MT; ++i) {
-                    const floatx4 s = sum[j][i] + meet[0][(j * MT + i) * 64 + lane];
-                    const int rank = first_rank + 16 * i + 4 * group;
-                    if ((ranks & 3) == 0) {
-                        if (rank < ranks) *reinterpret_cast<floatx4*>(to + rank) = s;
-                    } else {
-#pragma unroll
-                        for (int c = 0; c < 4; ++c)
-                            if (rank + c < ranks) to[rank + c] = s[c];
-                    }
-                }
+                for (int i = 0; i < MT; ++i) sum[j][i] = times(ap[i], xp, sum[j][i]);
             }
         }
-        __syncthreads();                                   // (the next adapter's sums meet in the same place)
+        if (k0 + whole * STEP < end) {                     // what is left of the segment behind the last block
+            const int k = k0 + whole * STEP;
+            P ap[MT];
+#pragma unroll
+            for (int i = 0; i < MT; ++i) load_piece<true>(ap[i], ae + (size_t)min(first_rank + 16 * i + at, d.ranks - 1) * d.width, k, end, group);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if (16 * j >= rows) break;
+                P xp;
+                load_piece<true>(xp, x + (size_t)(first_row + min(16 * j + at, rows - 1)) * d.ldx, k, end, group);
+#pragma unroll
+                for (int i = 0; i < MT; ++i) sum[j][i] = times(ap[i], xp, sum[j][i]);
+            }
+        }
+        store_sums<MT>(sum, ring, sums, d, segment, first_row, rows, first_rank);
     }
 }
 
-// 4 numbers of base or out at once.
-__device__ __forceinline__ floatx4 load4(const float* p) { return *reinterpret_cast<const floatx4*>(p); }
-__device__ __forceinline__ floatx4 load4(const bf16_t* p) {
-    const uint2 v = *reinterpret_cast<const uint2*>(p);
+// Operands of two types, or rows that do not begin at 16 bytes: through registers, in the same order.
+template <bool LOW, typename X, typename W, bool ALIGNED>
+__global__ __launch_bounds__(DOWN_NT) void adapters_down_any_kernel(const X* __restrict__ x, const W* __restrict__ a, const int* __restrict__ ids, float* __restrict__ sums, Down d) {
+    typedef Piece<LOW> P;
+    constexpr int MT = 2;
+    __shared__ __align__(16) unsigned char meet[DOWN_WAVES * 4 * MT * 1024];
+    __shared__ int before[COUNTS];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, at = lane & 15, group = lane >> 4;
+    Tiles tiles{ids, d.n_rows, 0, 0};
+    const int n_tiles = tiles.count(before);
+    const long n_items = (long)n_tiles * d.n_parts;
+    for (long item = blockIdx.x; item < n_items; item += gridDim.x) {
+        int first_row, rows, e;
+        const int part = (int)(item % d.n_parts), which = (int)(item / d.n_parts);
+        tiles.find(before, which, first_row, rows, e);
+        if (part == 0 && threadIdx.x == 0) {
+            d.list[which] = Tile{first_row, rows, e, 0};
+            *d.n_listed = n_tiles;
+        }
+        if (e < 0 || e >= d.n_adapters) continue;
+        const int segment = part % d.n_segments, first_rank = part / d.n_segments * 16 * MT;
+        const int begin = segment * d.segment, end = min(d.width, begin + d.segment);
+        const W* ar[MT];
+        const X* xr[4];
+#pragma unroll
+        for (int i = 0; i < MT; ++i) ar[i] = a + ((size_t)e * d.ranks + min(first_rank + 16 * i + at, d.ranks - 1)) * d.width;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) xr[j] = x + (size_t)(first_row + min(16 * j + at, rows - 1)) * d.ldx;
+        floatx4 sum[4][MT];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int i = 0; i < MT; ++i) sum[j][i] = floatx4{0.f, 0.f, 0.f, 0.f};
+        for (int k = begin + wave * P::BLOCK; k < end; k += P::BLOCK * DOWN_WAVES) {
+            P ap[MT];
+#pragma unroll
+            for (int i = 0; i < MT; ++i) load_piece<ALIGNED>(ap[i], ar[i], k, end, group);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if (16 * j >= rows) break;
+                P xp;
+                load_piece<ALIGNED>(xp, xr[j], k, end, group);
+#pragma unroll
+                for (int i = 0; i < MT; ++i) sum[j][i] = times(ap[i], xp, sum[j][i]);
+            }
+        }
+        store_sums<MT>(sum, meet, sums, d, segment, first_row, rows, first_rank);
+    }
+}
+
+// ------------------------------------------------------------------ up, in tiles
+// 4 numbers of base, as they lie in memory and as numbers, and of out.
+__device__ __forceinline__ uint4 raw4(const unsigned char* base, uint32_t i, bool low) {
+    if (!low) return *reinterpret_cast<const uint4*>(base + 4 * i);
+    const uint2 v = *reinterpret_cast<const uint2*>(base + 2 * i);
+    return uint4{v.x, v.y, 0u, 0u};
+}
+__device__ __forceinline__ floatx4 numbers4(uint4 v, bool low) {
+    if (!low) return __builtin_bit_cast(floatx4, v);
     return floatx4{__uint_as_float(v.x << 16), __uint_as_float(v.x & 0xffff0000u), __uint_as_float(v.y << 16), __uint_as_float(v.y & 0xffff0000u)};
 }
-__device__ __forceinline__ void store4(float* p, floatx4 v) { *reinterpret_cast<floatx4*>(p) = v; }
-__device__ __forceinline__ void store4(bf16_t* p, floatx4 v) { *reinterpret_cast<uint2*>(p) = uint2{f32x2_to_bf16x2(v[0], v[1]), f32x2_to_bf16x2(v[2], v[3])}; }
+__device__ __forceinline__ void store4(unsigned char* out, uint32_t i, floatx4 v, bool low) {
+    if (low) *reinterpret_cast<uint2*>(out + 2 * i) = uint2{f32x2_to_bf16x2(v[0], v[1]), f32x2_to_bf16x2(v[2], v[3])};
+    else *reinterpret_cast<floatx4*>(out + 4 * i) = v;
+}
+__device__ __forceinline__ float number1(const void* base, size_t i, bool low) { return low ? load_f32((const bf16_t*)base, i) : load_f32((const float*)base, i); }
+__device__ __forceinline__ void store1(void* out, size_t i, float v, bool low) { low ? store_f32((bf16_t*)out, i, v) : store_f32((float*)out, i, v); }
 
-// Up: NT tiles of 16 rows, a strip of columns, 32 at a time and wave: of each such step the lane of row r and group g has columns 8 g .. 8 g + 7, so that a row's four lanes
-// write whole lines.  The sums of A x are bfloat16 in two pieces where B is multiplied as bfloat16 (a half step of 2^-8 is left of a half step of 2^-8: one piece alone would lose more than
-// the 32-bit result keeps), 32-bit otherwise.  blockIdx: (strip, tile of rows, slot).
-template <bool LOW, typename W, typename S, typename O, int NT, bool ALIGNED>
-__global__ __launch_bounds__(64 * WAVES) void adapters_up_kernel(const float* __restrict__ sums, const W* __restrict__ b, const float* __restrict__ scales, const int* __restrict__ ids,
-                                                                 const S* base, long ldb, O* out, long ldo, int n_rows, int rank, int n_segments, Slices slices,
-                                                                 int strip_columns, int n_adapters, int slots, int vectors) {
+struct Rows {                               // base and out
+    const void* base;
+    void* out;
+    long ldb, ldo;
+    bool low_base, low_out, vectors;        // bfloat16; columns come in fours that may be loaded and stored at once
+};
+
+constexpr int PIECES = 3;                   // bfloat16 numbers that hold a 32-bit one: each the rounding of what the ones before leave, 8 bits of the 24 each
+
+// One run along the ranks of 16 columns of B.
+template <bool LOW> struct Run { uint4 v; };
+template <> struct Run<false> { float4 v; };
+template <bool ALIGNED, typename W> __device__ __forceinline__ void load_b(Run<true>& m, const W* row, int k, int rank) { m.v = load_run<ALIGNED>((const bf16_t*)row, k, rank); }
+template <bool ALIGNED, typename W> __device__ __forceinline__ void load_b(Run<false>& m, const W* row, int k, int rank) { m.v = load_run_f32<ALIGNED>(row, k, rank); }
+
+// One run of a row's sums, in pieces; they lie `apart` numbers behind one another.
+template <bool LOW> struct Held { bf16x8 v[PIECES]; };
+template <> struct Held<false> { float4 v; };
+__device__ __forceinline__ void load_row(Held<true>& t, const bf16_t* row, int apart) {
+#pragma unroll
+    for (int p = 0; p < PIECES; ++p) t.v[p] = *reinterpret_cast<const bf16x8*>(row + p * apart);
+}
+__device__ __forceinline__ floatx4 times(const Held<true>& t, const Run<true>& n, floatx4 sum) {
+#pragma unroll
+    for (int p = PIECES - 1; p >= 0; --p) sum = __builtin_amdgcn_mfma_f32_16x16x32_bf16(t.v[p], __builtin_bit_cast(bf16x8, n.v), sum, 0, 0, 0);
+    return sum;
+}
+__device__ __forceinline__ void load_row(Held<false>& t, const float* row, int) { t.v = *reinterpret_cast<const float4*>(row); }
+__device__ __forceinline__ floatx4 times(const Held<false>& t, const Run<false>& n, floatx4 sum) { return times(t.v, n.v, sum); }
+
+// A tile and a strip of columns.  The workgroup first adds up its rows' sums over the segments and keeps them in LDS: where B is bfloat16 and so multiplied, in PIECES, which lose nothing of their 24 bits.
+// Then a wave takes 64 columns at a time and of them 16 rows after 16 rows, with the columns' runs of B in registers throughout (loaded, they lie as the matrix cores want them, every lane in another
+// row of B: 64 accesses to the first-level cache a load); where the strip is no wider than 64 columns the waves share out the rows.  In the product D = M N the rows are M's and the columns
+// N's: number n of the four products of a step has columns 4 l + n, l = 0 .. 15, so that a lane ends with four neighbours and sixteen lanes with whole lines of base and out.  As on the way down no
+// row's values meet another's.  ALIGNED: runs of B, and fours of columns of base and out, may be loaded at once, and columns come in fours.  KS: runs of ranks that a wave keeps; 0 for any number,
+// loaded again for every 16 rows.  LOW_BASE, LOW_OUT: of aligned ones whether they are bfloat16 (a branch on it where they are loaded would have every load waited for); `io` says it of others.
+template <bool LOW, typename W, bool ALIGNED, int KS, bool LOW_BASE, bool LOW_OUT>
+__global__ __launch_bounds__(UP_NT) void adapters_up_kernel(const float* __restrict__ sums, const W* __restrict__ b, const float* __restrict__ scales, const Tile* __restrict__ list,
+                                                            const int* __restrict__ n_listed, Rows io, int n_rows, int rank, int n_segments, Slices slices, int strip_columns, int n_adapters) {
     typedef Piece<LOW> P;
+    typedef typename P::T T;
     extern __shared__ __align__(16) unsigned char room[];
-    const int padded = (rank + P::BLOCK / 2 - 1) / (P::BLOCK / 2) * (P::BLOCK / 2), pitch = padded + P::RUN;      // (rows of LDS a run further apart than a multiple of all banks)
-    bf16_t* high = (bf16_t*)room;                          // [16 NT][pitch], and the second pieces behind
-    bf16_t* low = high + 16 * NT * pitch;
-    float* whole = (float*)room;
+    constexpr int DEPTH = P::BLOCK / 2;                    // ranks of a matrix instruction (of four, in 32 bits)
+    const int padded = (rank + DEPTH - 1) / DEPTH * DEPTH, pitch = padded + P::RUN, apart = TILE * pitch;       // (rows of LDS a run further apart than a multiple of all banks)
+    T* held = (T*)room;                                    // [pieces][TILE][pitch], the largest piece first
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, at = lane & 15, group = lane >> 4;
-    const int first_row = blockIdx.y * 16 * NT, slot = blockIdx.z;
-    int s = 0;
-    while (s + 1 < slices.n && (int)blockIdx.x >= slices.strip[s + 1]) ++s;
-    const int begin = slices.begin[s] + ((int)blockIdx.x - slices.strip[s]) * strip_columns, end = min(slices.begin[s + 1], begin + strip_columns);
-    const int columns = slices.begin[slices.n], ranks = rank * slices.n;
-    Tile tile(ids, first_row, 16 * NT, n_rows, n_adapters);
-
-    // Base with the adapter's share, or without (`e` < 0), for the rows in `rows`.
-    if (slot == 0) {                                       // rows without an adapter
-        unsigned long long none = ~tile.left;
-        const int there = min(16 * NT, n_rows - first_row);
-        none &= there < 64 ? (1ull << there) - 1 : ~0ull;
-        if ((const void*)base != (const void*)out) {
-            while (none != 0) {
-                const int row = first_row + __ffsll((long long)none) - 1;
-                none &= none - 1;
-                for (int c = begin + threadIdx.x; c < end; c += 64 * WAVES) store_f32(out, (size_t)row * ldo + c, load_f32(base, (size_t)row * ldb + c));
-            }
+    const int columns = slices.begin[slices.n], ranks = rank * slices.n, n_strips = slices.strip[slices.n];
+    const long n_items = (long)*n_listed * n_strips;
+    for (long item = blockIdx.x; item < n_items; item += gridDim.x) {
+        const int strip = (int)(item % n_strips);
+        int s = 0;
+        while (s + 1 < slices.n && strip >= slices.strip[s + 1]) ++s;
+        const int begin = slices.begin[s] + (strip - slices.strip[s]) * strip_columns, end = min(slices.begin[s + 1], begin + strip_columns);
+        const Tile tile = list[item / n_strips];
+        const int first_row = tile.first, rows = tile.rows, e = tile.id;
+        if (e < 0 || e >= n_adapters) {                    // rows without an adapter
+            if (io.base != io.out)
+                for (int r = first_row; r < first_row + rows; ++r)
+                    for (int c = begin + threadIdx.x; c < end; c += UP_NT) store1(io.out, (size_t)r * io.ldo + c, number1(io.base, (size_t)r * io.ldb + c, io.low_base), io.low_out);
+            continue;
         }
-    }
-    for (int count = 0; tile.left != 0; ++count) {
-        unsigned long long rows;
-        const int e = tile.next(rows);
-        if (count % slots != slot) continue;
+        const W* be = b + (size_t)e * columns * rank;
+        const bool by_rows = strip_columns == 64;
+        const int j_step = by_rows ? UP_WAVES : 1, last_j = (rows - 1) / 16;
+        const unsigned char* base_at = (const unsigned char*)io.base + (size_t)first_row * io.ldb * (io.low_base ? 2 : 4);
+        unsigned char* out_at = (unsigned char*)io.out + (size_t)first_row * io.ldo * (io.low_out ? 2 : 4);
+        Run<LOW> br[KS == 0 ? 1 : KS][4];
+        uint4 next[4];
+        auto ask_b = [&](int c0) {                         // for a step's columns of B
+#pragma unroll
+            for (int k = 0; k < KS; ++k)
+#pragma unroll
+                for (int n = 0; n < 4; ++n) load_b<ALIGNED>(br[k][n], be + (size_t)(min(c0 + 4 * at, end - 4) + n) * rank, DEPTH * k + P::RUN * group, rank);
+        };
+        // Rows behind the last are taken as that one throughout, and columns behind the end as the last four: their lanes load and store what the lanes that own them do, at the same time.  Without a branch
+        // around any store the wait for a load counts what was asked for behind it, and no load waits for a store's end.
+        auto ask_base = [&](int c0, int j) {
+            if constexpr (ALIGNED)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) next[i] = raw4(base_at, (uint32_t)(min(16 * j + 4 * group + i, rows - 1) * (int)io.ldb + min(c0 + 4 * at, end - 4)), LOW_BASE);
+        };
+        int c0 = begin + (by_rows ? 0 : 64 * wave);
+        const int j0 = by_rows ? wave : 0;
+        const bool idle = c0 >= end || j0 > last_j;
+        if (!idle) {                                       // the first step's come while the rows' sums are made
+            ask_b(c0);
+            ask_base(c0, j0);
+        }
         const float scale = scales != nullptr ? scales[e] : 1.f;
-        __syncthreads();                                   // (the adapter before has been read)
-        for (int item = threadIdx.x; item < 16 * NT * padded; item += 64 * WAVES) {
-            const int r = item / padded, k = item % padded;
-            float v = 0.f;
-            if (k < rank && (rows >> r & 1)) {
-                const float* from = sums + (size_t)(first_row + r) * ranks + s * rank + k;
-                for (int seg = 0; seg < n_segments; ++seg) v += from[(size_t)seg * n_rows * ranks];
-                v *= scale;
+        const int n_fours = ((rows + 15) & ~15) * (padded / 4);
+        const size_t further = (size_t)n_rows * ranks;
+        __syncthreads();                                   // (the item before has been read)
+        for (int i0 = threadIdx.x; i0 < n_fours; i0 += 2 * UP_NT) {            // four ranks of a row at a time, and twice that, of four segments
+            floatx4 v[2];
+            const float* from[2];
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                const int i = min(i0 + q * UP_NT, n_fours - 1);
+                from[q] = sums + (size_t)(first_row + min(i / (padded / 4), rows - 1)) * ranks + s * rank;
+                v[q] = floatx4{0.f, 0.f, 0.f, 0.f};
             }
-            if (LOW) {
-                const bf16_t h = f32_to_bf16(v);
-                high[r * pitch + k] = h;
-                low[r * pitch + k] = f32_to_bf16(v - bf16_to_f32(h));
-            } else {
-                whole[r * pitch + k] = v;
+            for (int seg = 0; seg < n_segments; seg += 4) {
+                floatx4 part[4][2];
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+#pragma unroll
+                    for (int q = 0; q < 2; ++q) {
+                        const int k = min(i0 + q * UP_NT, n_fours - 1) % (padded / 4) * 4;
+                        const float* p = from[q] + min(seg + u, n_segments - 1) * further;
+                        if ((rank & 3) == 0) part[u][q] = *reinterpret_cast<const floatx4*>(p + min(k, rank - 4));
+                        else
+#pragma unroll
+                            for (int c = 0; c < 4; ++c) part[u][q][c] = p[min(k + c, rank - 1)];
+                    }
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+#pragma unroll
+                    for (int q = 0; q < 2; ++q)
+                        if (seg + u < n_segments) v[q] += part[u][q];
+            }
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                const int i = i0 + q * UP_NT, r = i / (padded / 4), k = i % (padded / 4) * 4;
+                if (i >= n_fours) break;
+                v[q] *= scale;
+#pragma unroll
+                for (int c = 0; c < 4; ++c) v[q][c] = k + c < rank ? v[q][c] : 0.f;
+                if constexpr (LOW) {
+#pragma unroll
+                    for (int p = 0; p < PIECES; ++p) {
+                        const uint2 two = uint2{f32x2_to_bf16x2(v[q][0], v[q][1]), f32x2_to_bf16x2(v[q][2], v[q][3])};
+                        *reinterpret_cast<uint2*>(held + p * apart + r * pitch + k) = two;
+                        v[q] -= numbers4(uint4{two.x, two.y, 0u, 0u}, true);
+                    }
+                } else {
+                    *reinterpret_cast<floatx4*>(held + r * pitch + k) = v[q];
+                }
             }
         }
         __syncthreads();
-        const W* be = b + (size_t)e * columns * rank;
-        for (int c0 = begin + 32 * wave; c0 < end; c0 += 32 * WAVES) {
-            floatx4 sum[NT][2];
+        if (idle) continue;
+        while (true) {
+            const int col = ALIGNED ? min(c0 + 4 * at, end - 4) : c0 + 4 * at;
+#pragma unroll 1
+            for (int j = j0; j <= last_j; j += j_step) {
+                uint4 was[4];
 #pragma unroll
-            for (int j = 0; j < NT; ++j)
+                for (int i = 0; i < 4; ++i) was[i] = next[i];
+                ask_base(c0, min(j + j_step, last_j));
+                floatx4 sum[4];
 #pragma unroll
-                for (int h = 0; h < 2; ++h) sum[j][h] = floatx4{0.f, 0.f, 0.f, 0.f};
-            const W* br[2];
+                for (int n = 0; n < 4; ++n) sum[n] = floatx4{0.f, 0.f, 0.f, 0.f};
+                const T* row = held + (16 * j + at) * pitch + P::RUN * group;
+                Held<LOW> t;
+                if constexpr (KS > 0) {
 #pragma unroll
-            for (int h = 0; h < 2; ++h) br[h] = be + (size_t)min(c0 + 8 * (at >> 2) + 4 * h + (at & 3), end - 1) * rank;
-            const int c = c0 + 8 * group;
-            for (int k = 0; k < padded; k += P::BLOCK / 2) {
-                const int mine = k + P::RUN * group;
-                if constexpr (LOW) {
-                    uint4 m[2];
+                    for (int k = 0; k < KS; ++k) {
+                        load_row(t, row + DEPTH * k, apart);
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) m[h] = load_run<ALIGNED>((const bf16_t*)br[h], mine, rank);
-#pragma unroll
-                    for (int j = 0; j < NT; ++j) {
-                        const bf16x8 th = *reinterpret_cast<const bf16x8*>(high + (16 * j + at) * pitch + mine), tl = *reinterpret_cast<const bf16x8*>(low + (16 * j + at) * pitch + mine);
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            sum[j][h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, m[h]), tl, sum[j][h], 0, 0, 0);
-                            sum[j][h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, m[h]), th, sum[j][h], 0, 0, 0);
-                        }
+                        for (int n = 0; n < 4; ++n) sum[n] = times(t, br[k][n], sum[n]);
                     }
                 } else {
-                    float4 m[2];
+                    for (int k = 0; k < padded; k += DEPTH) {
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) m[h] = load_run_f32<ALIGNED>(br[h], mine, rank);
+                        for (int n = 0; n < 4; ++n) load_b<ALIGNED>(br[0][n], be + (size_t)(ALIGNED ? col + n : min(col + n, end - 1)) * rank, k + P::RUN * group, rank);
+                        load_row(t, row + k, apart);
 #pragma unroll
-                    for (int j = 0; j < NT; ++j) {
-                        const float4 t = *reinterpret_cast<const float4*>(whole + (16 * j + at) * pitch + mine);
+                        for (int n = 0; n < 4; ++n) sum[n] = times(t, br[0][n], sum[n]);
+                    }
+                }
 #pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            sum[j][h] = __builtin_amdgcn_mfma_f32_16x16x4f32(m[h].x, t.x, sum[j][h], 0, 0, 0);
-                            sum[j][h] = __builtin_amdgcn_mfma_f32_16x16x4f32(m[h].y, t.y, sum[j][h], 0, 0, 0);
-                            sum[j][h] = __builtin_amdgcn_mfma_f32_16x16x4f32(m[h].z, t.z, sum[j][h], 0, 0, 0);
-                            sum[j][h] = __builtin_amdgcn_mfma_f32_16x16x4f32(m[h].w, t.w, sum[j][h], 0, 0, 0);
-                        }
+                for (int i = 0; i < 4; ++i) {
+                    const int r = 16 * j + 4 * group + i;
+                    if constexpr (ALIGNED) {
+                        const uint32_t to = (uint32_t)(min(r, rows - 1) * (int)io.ldo + col);
+                        store4(out_at, to, numbers4(was[i], LOW_BASE) + floatx4{sum[0][i], sum[1][i], sum[2][i], sum[3][i]}, LOW_OUT);
+                    } else if (r < rows) {
+                        const uint32_t to = (uint32_t)(r * (int)io.ldo + col);
+#pragma unroll
+                        for (int n = 0; n < 4; ++n)
+                            if (col + n < end) store1(out_at, to + n, number1(base_at, (size_t)(uint32_t)(r * (int)io.ldb + col + n), io.low_base) + sum[n][i], io.low_out);
                     }
                 }
             }
+            c0 += by_rows ? 64 : 64 * UP_WAVES;
+            if (c0 >= end) break;
+            ask_b(c0);
+            ask_base(c0, j0);
+        }
+    }
+}
+
+// ------------------------------------------------------------------ a few rows
+// Decoded rows, as a rule each with an adapter of its own: nothing is shared, the adapters' bytes bound it, and what counts is that all of them are asked for at once and few waits
+// follow one another.  Every row is taken alone, without tiles.  Down: a workgroup has a row and RG ranks, its threads share out the width.
+template <int RG>
+__global__ __launch_bounds__(256) void adapters_down_few_kernel(const bf16_t* __restrict__ x, long ldx, const bf16_t* __restrict__ a, const int* __restrict__ ids, float* __restrict__ sums,
+                                                                int width, int ranks, int n_adapters) {
+    __shared__ float red[4][RG];
+    const int row = blockIdx.y, first = blockIdx.x * RG, tid = threadIdx.x;
+    const int e = ids[row];
+    if (e < 0 || e >= n_adapters) return;
+    const bf16_t* xr = x + (size_t)row * ldx;
+    const bf16_t* ar[RG];
 #pragma unroll
-            for (int j = 0; j < NT; ++j) {
-                if (!(rows >> (16 * j + at) & 1)) continue;
-                const size_t row = first_row + 16 * j + at;
+    for (int i = 0; i < RG; ++i) ar[i] = a + ((size_t)e * ranks + min(first + i, ranks - 1)) * width;
+    float sum[RG];
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const int col = c + 4 * h;
-                    if (vectors && col + 4 <= end) {
-                        store4(out + row * ldo + col, load4(base + row * ldb + col) + sum[j][h]);
-                    } else {
+    for (int i = 0; i < RG; ++i) sum[i] = 0.f;
+#pragma unroll 2
+    for (int k = 8 * tid; k < width; k += 2048) {
+        const uint4 xv = *reinterpret_cast<const uint4*>(xr + k);
+        uint4 av[RG];
 #pragma unroll
-                        for (int u = 0; u < 4; ++u)
-                            if (col + u < end) store_f32(out, row * ldo + col + u, load_f32(base, row * ldb + col + u) + sum[j][h][u]);
-                    }
-                }
+        for (int i = 0; i < RG; ++i) av[i] = *reinterpret_cast<const uint4*>(ar[i] + k);
+        const uint32_t xw[4] = {xv.x, xv.y, xv.z, xv.w};
+#pragma unroll
+        for (int i = 0; i < RG; ++i) {
+            const uint32_t aw[4] = {av[i].x, av[i].y, av[i].z, av[i].w};
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                sum[i] = fmaf(__uint_as_float(xw[u] << 16), __uint_as_float(aw[u] << 16), sum[i]);
+                sum[i] = fmaf(__uint_as_float(xw[u] & 0xffff0000u), __uint_as_float(aw[u] & 0xffff0000u), sum[i]);
             }
         }
     }
+#pragma unroll
+    for (int i = 0; i < RG; ++i) {
+        sum[i] = wave_sum(sum[i]);
+        if ((tid & 63) == 0) red[tid >> 6][i] = sum[i];
+    }
+    __syncthreads();
+    if (tid < RG && first + tid < ranks) sums[(size_t)row * ranks + first + tid] = (red[0][tid] + red[1][tid]) + (red[2][tid] + red[3][tid]);
+}
+
+// Up: a thread has FEW_COLUMNS columns, 256 apart, of a row; the row's sums come as scalars.
+constexpr int FEW_COLUMNS = 2;
+__global__ __launch_bounds__(256) void adapters_up_few_kernel(const float* __restrict__ sums, const bf16_t* __restrict__ b, const float* __restrict__ scales, const int* __restrict__ ids,
+                                                              Rows io, int rank, Slices slices, int n_adapters) {
+    const int row = blockIdx.y;
+    int s = 0;
+    while (s + 1 < slices.n && (int)blockIdx.x >= slices.strip[s + 1]) ++s;
+    const int begin = slices.begin[s] + ((int)blockIdx.x - slices.strip[s]) * 256 * FEW_COLUMNS + threadIdx.x, end = slices.begin[s + 1];
+    const int e = ids[row];
+    const bool some = e >= 0 && e < n_adapters;
+    if (!some && io.base == io.out) return;
+    float was[FEW_COLUMNS], sum[FEW_COLUMNS];
+#pragma unroll
+    for (int c = 0; c < FEW_COLUMNS; ++c) {
+        was[c] = number1(io.base, (size_t)row * io.ldb + min(begin + 256 * c, end - 1), io.low_base);
+        sum[c] = 0.f;
+    }
+    if (some) {
+        const float* t = sums + (size_t)row * rank * slices.n + s * rank;
+        const bf16_t* br[FEW_COLUMNS];
+#pragma unroll
+        for (int c = 0; c < FEW_COLUMNS; ++c) br[c] = b + ((size_t)e * slices.begin[slices.n] + min(begin + 256 * c, end - 1)) * rank;
+        const float scale = scales != nullptr ? scales[e] : 1.f;
+        for (int k = 0; k < rank; k += 8) {
+            uint4 v[FEW_COLUMNS];
+#pragma unroll
+            for (int c = 0; c < FEW_COLUMNS; ++c) v[c] = *reinterpret_cast<const uint4*>(br[c] + k);
+#pragma unroll
+            for (int c = 0; c < FEW_COLUMNS; ++c) {
+                const uint32_t w[4] = {v[c].x, v[c].y, v[c].z, v[c].w};
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    sum[c] = fmaf(t[k + 2 * u], __uint_as_float(w[u] << 16), sum[c]);
+                    sum[c] = fmaf(t[k + 2 * u + 1], __uint_as_float(w[u] & 0xffff0000u), sum[c]);
+                }
+            }
+        }
+#pragma unroll
+        for (int c = 0; c < FEW_COLUMNS; ++c) was[c] = fmaf(scale, sum[c], was[c]);
+    }
+#pragma unroll
+    for (int c = 0; c < FEW_COLUMNS; ++c)
+        if (begin + 256 * c < end) store1(io.out, (size_t)row * io.ldo + begin + 256 * c, was[c], io.low_out);
 }
 
 bool aligned(const void* p, int bytes) { return (size_t)p % bytes == 0; }
 
 struct Call {
-    const void* x; long ldx; const void* a; const void* b; const int* ids; const float* scales; const void* base; long ldb; void* out; long ldo; float* sums;
-    int n_rows, width, columns, rank, n_adapters, n_segments, segment;
+    const void* x; long ldx; const void* a; const void* b; const int* ids; const float* scales; Rows io; float* sums; Tile* list; int* n_listed;
+    int n_rows, width, columns, rank, n_adapters, segment, n_segments;
     Slices slices;
     hipStream_t stream;
 };
 
-template <bool LOW, typename X, typename W, int NT, int MT>
-void down_sized(const Call& c, int slots) {
-    const int ranks = c.rank * c.slices.n, run = Piece<LOW>::RUN;
-    const dim3 grid((c.n_rows + 16 * NT - 1) / (16 * NT), c.n_segments, (ranks + 16 * MT - 1) / (16 * MT) * slots);
-    const bool even = c.width % run == 0 && c.ldx % run == 0 && aligned(c.x, run * sizeof(X)) && aligned(c.a, run * sizeof(W));
-    if (even) adapters_down_kernel<LOW, X, W, NT, MT, true><<<grid, 64 * WAVES, 0, c.stream>>>((const X*)c.x, c.ldx, (const W*)c.a, c.ids, c.sums, c.n_rows, c.width, ranks, c.n_adapters, c.segment, slots);
-    else adapters_down_kernel<LOW, X, W, NT, MT, false><<<grid, 64 * WAVES, 0, c.stream>>>((const X*)c.x, c.ldx, (const W*)c.a, c.ids, c.sums, c.n_rows, c.width, ranks, c.n_adapters, c.segment, slots);
+// At most so many tiles: every 64th row begins one, and every row may.  Workgroups beyond the work there is leave at once, ones short of it come again.
+long most_tiles(int n_rows) { return n_rows; }
+// ... and about so many where the rows are a few requests'.
+long usual_tiles(int n_rows) { return (n_rows + TILE - 1) / TILE + 4; }
+
+// Lets a kernel have `bytes` of LDS, asked for once per device.
+constexpr int MAX_DEVICES = 64;
+int raise_lds(const void* kernel, int bytes, bool (&raised)[MAX_DEVICES]) {
+    int device = -1;
+    if (hipGetDevice(&device) != hipSuccess || device < 0 || device >= MAX_DEVICES) return gi_fail("adapters_add: no current device");
+    if (!raised[device]) {
+        if (hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes) != hipSuccess) return gi_fail("adapters_add: cannot reserve %d bytes of LDS", bytes);
+        raised[device] = true;
+    }
+    return 0;
 }
 
-// Bytes of LDS that the way up keeps `rows` rows' sums in.
-template <bool LOW> int up_lds(int rows, int rank) {
-    typedef Piece<LOW> P;
-    return rows * ((rank + P::BLOCK / 2 - 1) / (P::BLOCK / 2) * (P::BLOCK / 2) + P::RUN) * 4;
-}
-int tiles_of_rows(const Call& c) { return c.n_rows <= 128 || up_lds<true>(64, c.rank) > 65536 ? 1 : 4; }
-int slots_of(const Call& c, int tile_rows) {
-    const int most = min(min(tile_rows, c.n_rows), c.n_adapters);
-    return tile_rows == 16 ? most : min(most, 4);
+template <bool LOW, int MT>
+int down_sized(const Call& c, Down d) {
+    constexpr int lds = DOWN_WAVES * stages_of<MT>() * stage_bytes<MT>();
+    static_assert(lds >= DOWN_WAVES * 4 * MT * 1024, "the waves' sums meet in the ring");
+    d.n_parts = d.n_segments * ((d.ranks + 16 * MT - 1) / (16 * MT));
+    const long items = most_tiles(c.n_rows) * d.n_parts;
+    const int grid = (int)min(items, (long)gi_compute_units() * (163840 / (lds + 4 * COUNTS)));
+    typedef typename Piece<LOW>::T T;
+    static bool raised[MAX_DEVICES] = {};
+    if (raise_lds((const void*)adapters_down_kernel<LOW, MT>, lds, raised) != 0) return -1;
+    adapters_down_kernel<LOW, MT><<<grid, DOWN_NT, lds, c.stream>>>((const T*)c.x, (const T*)c.a, c.ids, c.sums, d);
+    return 0;
 }
 
 template <bool LOW, typename X, typename W>
-void down(const Call& c) {
-    const int ranks = c.rank * c.slices.n, groups = (ranks + 63) / 64, mt = ((ranks + groups - 1) / groups + 15) / 16;
-    const int nt = tiles_of_rows(c), slots = slots_of(c, 16 * nt);
-#define GI_DOWN(NT) (mt == 1 ? down_sized<LOW, X, W, NT, 1>(c, slots) : mt == 2 ? down_sized<LOW, X, W, NT, 2>(c, slots) : mt == 3 ? down_sized<LOW, X, W, NT, 3>(c, slots) : down_sized<LOW, X, W, NT, 4>(c, slots))
-    if (nt == 1) GI_DOWN(1);
-    else GI_DOWN(4);
-#undef GI_DOWN
+int down(const Call& c) {
+    const int ranks = c.rank * c.slices.n, run = Piece<LOW>::RUN;
+    Down d{c.list, c.n_listed, c.n_rows, c.width, ranks, c.n_adapters, c.segment, c.n_segments, 0, c.ldx};
+    const bool even = c.width % run == 0 && c.ldx % run == 0 && aligned(c.x, run * sizeof(X)) && aligned(c.a, run * sizeof(W));
+    if constexpr (std::is_same<X, W>::value) {
+        if (even) {
+            const int groups = (ranks + 63) / 64, mt = ((ranks + groups - 1) / groups + 15) / 16;
+            return mt == 1 ? down_sized<LOW, 1>(c, d) : mt == 2 ? down_sized<LOW, 2>(c, d) : mt == 3 ? down_sized<LOW, 3>(c, d) : down_sized<LOW, 4>(c, d);
+        }
+    }
+    d.n_parts = d.n_segments * ((ranks + 31) / 32);
+    const int grid = (int)min(most_tiles(c.n_rows) * d.n_parts, (long)gi_compute_units() * 8);
+    if constexpr (!std::is_same<X, W>::value) {
+        if (even) {
+            adapters_down_any_kernel<LOW, X, W, true><<<grid, DOWN_NT, 0, c.stream>>>((const X*)c.x, (const W*)c.a, c.ids, c.sums, d);
+            return 0;
+        }
+    }
+    adapters_down_any_kernel<LOW, X, W, false><<<grid, DOWN_NT, 0, c.stream>>>((const X*)c.x, (const W*)c.a, c.ids, c.sums, d);
+    return 0;
 }
 
-template <bool LOW, typename W, typename S, typename O, int NT>
-void up_sized(const Call& c) {
-    typedef Piece<LOW> P;
-    const int slots = slots_of(c, 16 * NT), tiles = (c.n_rows + 16 * NT - 1) / (16 * NT), lds = up_lds<LOW>(16 * NT, c.rank);
-    // A strip's workgroup first makes its rows' sums, so strips are as long as leaves every compute unit a few workgroups.
-    int strip = 128;
-    while (strip < 1024 && (long)tiles * ((c.columns + strip - 1) / strip) > 2048) strip *= 2;
-    Slices slices = c.slices;
-    for (int s = 0; s < slices.n; ++s) slices.strip[s + 1] = slices.strip[s] + (slices.begin[s + 1] - slices.begin[s] + strip - 1) / strip;
-    bool vectors = c.ldb % 4 == 0 && c.ldo % 4 == 0 && aligned(c.base, 4 * sizeof(S)) && aligned(c.out, 4 * sizeof(O));
-    for (int s = 0; s < slices.n; ++s) vectors = vectors && slices.begin[s] % 4 == 0;
-    const bool even = c.rank % P::RUN == 0 && aligned(c.b, P::RUN * sizeof(W));
-    const dim3 grid(slices.strip[slices.n], tiles, slots);
-    if (even) adapters_up_kernel<LOW, W, S, O, NT, true><<<grid, 64 * WAVES, lds, c.stream>>>(c.sums, (const W*)c.b, c.scales, c.ids, (const S*)c.base, c.ldb, (O*)c.out, c.ldo, c.n_rows, c.rank,
-                                                                                              c.n_segments, slices, strip, c.n_adapters, slots, vectors);
-    else adapters_up_kernel<LOW, W, S, O, NT, false><<<grid, 64 * WAVES, lds, c.stream>>>(c.sums, (const W*)c.b, c.scales, c.ids, (const S*)c.base, c.ldb, (O*)c.out, c.ldo, c.n_rows, c.rank,
-                                                                                          c.n_segments, slices, strip, c.n_adapters, slots, vectors);
+// Bytes of LDS that the way up keeps a tile's sums in.
+template <bool LOW> constexpr int up_lds(int rank) {
+    constexpr int DEPTH = Piece<LOW>::BLOCK / 2;
+    return TILE * ((rank + DEPTH - 1) / DEPTH * DEPTH + Piece<LOW>::RUN) * (LOW ? 2 * PIECES : 4);
 }
 
-template <bool LOW, typename W, typename S, typename O>
-void up(const Call& c) {
-    if (tiles_of_rows(c) == 1) up_sized<LOW, W, S, O, 1>(c);
-    else up_sized<LOW, W, S, O, 4>(c);
+template <bool LOW, typename W, bool ALIGNED, int KS, bool LOW_BASE, bool LOW_OUT>
+int up_launch(const Call& c, const Slices& slices, int strip) {
+    static bool raised[MAX_DEVICES] = {};
+    constexpr int most = up_lds<LOW>(MAX_RANK);
+    if (raise_lds((const void*)adapters_up_kernel<LOW, W, ALIGNED, KS, LOW_BASE, LOW_OUT>, most, raised) != 0) return -1;
+    const int grid = (int)min(most_tiles(c.n_rows) * slices.strip[slices.n], 4l * gi_compute_units());
+    adapters_up_kernel<LOW, W, ALIGNED, KS, LOW_BASE, LOW_OUT><<<grid, UP_NT, up_lds<LOW>(c.rank), c.stream>>>(c.sums, (const W*)c.b, c.scales, c.list, c.n_listed, c.io, c.n_rows, c.rank,
+                                                                                                               c.n_segments, slices, strip, c.n_adapters);
+    return 0;
+}
+
+template <bool LOW, typename W, bool ALIGNED, int KS>
+int up_sized(const Call& c, const Slices& slices, int strip) {
+    if constexpr (!ALIGNED) return up_launch<LOW, W, ALIGNED, KS, false, false>(c, slices, strip);
+    else if (c.io.low_base) return c.io.low_out ? up_launch<LOW, W, ALIGNED, KS, true, true>(c, slices, strip) : up_launch<LOW, W, ALIGNED, KS, true, false>(c, slices, strip);
+    else return c.io.low_out ? up_launch<LOW, W, ALIGNED, KS, false, true>(c, slices, strip) : up_launch<LOW, W, ALIGNED, KS, false, false>(c, slices, strip);
 }
 
 template <bool LOW, typename W>
-void up_typed(const Call& c, int base_type, int out_type) {
-    if (base_type == GI_BF16) out_type == GI_BF16 ? up<LOW, W, bf16_t, bf16_t>(c) : up<LOW, W, bf16_t, float>(c);
-    else out_type == GI_BF16 ? up<LOW, W, float, bf16_t>(c) : up<LOW, W, float, float>(c);
+int up(const Call& c) {
+    // A strip's workgroup first makes its rows' sums, so strips are as long as leaves every compute unit (of 256) two or three workgroups: aimed at 200, 350, 700 and 1,400 of them, 4,096 rows of 4,096 columns
+    // and rank 64 take 52, 52, 46 and 45 us, 2,048 rows of 2,048 columns and rank 32 12.3, 10.4, 10.4 and 14.6.
+    const long even = usual_tiles(c.n_rows) * c.columns / 700;
+    const int steps = (c.rank + Piece<LOW>::BLOCK / 2 - 1) / (Piece<LOW>::BLOCK / 2);
+    const int strip = even <= 64 ? 64 : (int)min((even + 255) / 256 * 256, 1024l);
+    Slices slices = c.slices;
+    for (int s = 0; s < slices.n; ++s) slices.strip[s + 1] = slices.strip[s] + (slices.begin[s + 1] - slices.begin[s] + strip - 1) / strip;
+    if (c.io.vectors && c.rank % Piece<LOW>::RUN == 0 && aligned(c.b, Piece<LOW>::RUN * sizeof(W)))
+        return steps == 1 ? up_sized<LOW, W, true, 1>(c, slices, strip) : steps == 2 ? up_sized<LOW, W, true, 2>(c, slices, strip) : up_sized<LOW, W, true, 0>(c, slices, strip);
+    return up_sized<LOW, W, false, 0>(c, slices, strip);
+}
+
+// bfloat16 rows that may be loaded 8 numbers at a time, few enough that loading an adapter once for every row that takes it costs less than tiles that share it.
+bool few_rows(const Call& c) {
+    return c.n_rows <= 64 && c.rank % 8 == 0 && c.width % 8 == 0 && c.ldx % 8 == 0 && aligned(c.x, 16) && aligned(c.a, 16) && aligned(c.b, 16);
+}
+
+void add_few(const Call& c) {
+    const int ranks = c.rank * c.slices.n;
+    const long items = (long)c.n_rows * ranks;
+    const int rg = items >= 4096 ? 4 : 1;
+    const dim3 grid((ranks + rg - 1) / rg, c.n_rows);
+#define GI_FEW(RG) adapters_down_few_kernel<RG><<<grid, 256, 0, c.stream>>>((const bf16_t*)c.x, c.ldx, (const bf16_t*)c.a, c.ids, c.sums, c.width, ranks, c.n_adapters)
+    if (rg == 1) GI_FEW(1);
+    else GI_FEW(4);
+#undef GI_FEW
+    Slices slices = c.slices;
+    for (int s = 0; s < slices.n; ++s) slices.strip[s + 1] = slices.strip[s] + (slices.begin[s + 1] - slices.begin[s] + 256 * FEW_COLUMNS - 1) / (256 * FEW_COLUMNS);
+    adapters_up_few_kernel<<<dim3(slices.strip[slices.n], c.n_rows), 256, 0, c.stream>>>(c.sums, (const bf16_t*)c.b, c.scales, c.ids, c.io, c.rank, slices, c.n_adapters);
+}
+
+// In 32 bits a segment is always the same.  Otherwise there are as many as give every compute unit (of 256) a workgroup: the sums of every segment are written and read again, and with two workgroups a unit
+// the way down gains less than the way up loses (4,096 rows of 14,336, rank 64: 39 + 46 us with seven segments, 41 + 42 with three; 531 rows of 4,096, rank 3 * 24: 12.0 + 12.7, 10.0 + 10.3).
+int segment_of(int n_rows, int width, int ranks, bool low) {
+    if (!low) return EXACT_SEGMENT;
+    const long segments = max(250 / (usual_tiles(n_rows) * ((ranks + 63) / 64)), 1l);
+    return (int)(((width + segments - 1) / segments + SEGMENT - 1) / SEGMENT * SEGMENT);
 }
 
 }  // namespace
 
-// The segments of the width on the way down.
-GI_API int gi_adapters_segments(int n_rows, int width) { return (width + SEGMENT - 1) / SEGMENT; }
+// Floats of scratch that gi_adapters_add needs, 16-byte aligned: the sums of every segment of the width, the list of tiles and its length.
+static long segments_for(int x_type, int w_type, int n_rows, int width, int ranks) {
+    const int segment = segment_of(n_rows, width, ranks, x_type == GI_BF16 && w_type == GI_BF16);
+    return (width + segment - 1) / segment;
+}
+static long sums_for(int x_type, int w_type, int n_rows, int width, int ranks) { return (segments_for(x_type, w_type, n_rows, width, ranks) * n_rows * ranks + 3) / 4 * 4; }
+GI_API long gi_adapters_scratch_floats(int x_type, int w_type, int n_rows, int width, int rank, int n_slices) {
+    return sums_for(x_type, w_type, n_rows, width, rank * n_slices) + 4 * (long)n_rows + 4;
+}
 
-// sums: gi_adapters_segments(n_rows, width) * n_rows * rank * n_slices floats, 16-byte aligned.
 GI_API int gi_adapters_add(const void* x, int x_type, long ldx, const void* a, const void* b, int w_type, const int* ids, const float* scales, const void* base, int base_type, long ldb,
-                           void* out, int out_type, long ldo, float* sums, int n_rows, int width, int columns, int rank, int n_slices, const int* slice_columns, int n_adapters,
+                           void* out, int out_type, long ldo, float* scratch, int n_rows, int width, int columns, int rank, int n_slices, const int* slice_columns, int n_adapters,
                            hipStream_t stream) {
     GI_REQUIRE(n_rows > 0 && width > 0 && columns > 0 && rank > 0 && n_adapters > 0 && ldx >= width && ldb >= columns && ldo >= columns,
                "adapters_add: bad sizes (rows %d, width %d, columns %d, rank %d, adapters %d, strides %ld %ld %ld)", n_rows, width, columns, rank, n_adapters, ldx, ldb, ldo);
     GI_REQUIRE(rank <= MAX_RANK, "adapters_add: rank %d, at most %d is taken", rank, MAX_RANK);
     GI_REQUIRE(n_slices >= 1 && n_slices <= MAX_SLICES, "adapters_add: %d packed projections, 1 to %d are taken", n_slices, MAX_SLICES);
-    GI_REQUIRE(sums != nullptr && aligned(sums, 16), "adapters_add: scratch is missing");
-    Call c{x, ldx, a, b, ids, scales, base, ldb, out, ldo, sums, n_rows, width, columns, rank, n_adapters, gi_adapters_segments(n_rows, width), SEGMENT, Slices{n_slices, {0}, {0}}, stream};
+    GI_REQUIRE(ldb <= 1 << 23 && ldo <= 1 << 23, "adapters_add: rows of base and out %ld and %ld numbers apart, at most %d are taken", ldb, ldo, 1 << 23);
+    GI_REQUIRE(n_rows <= 1 << 20 && width <= 1 << 24 && columns <= 1 << 22, "adapters_add: %d rows of %d numbers onto %d columns are too many for one launch", n_rows, width, columns);
+    GI_REQUIRE(scratch != nullptr && aligned(scratch, 16), "adapters_add: scratch is missing");
+    const bool low = x_type == GI_BF16 && w_type == GI_BF16;
+    Tile* list = (Tile*)(scratch + sums_for(x_type, w_type, n_rows, width, rank * n_slices));
+    Call c{x, ldx, a, b, ids, scales, Rows{base, out, ldb, ldo, base_type == GI_BF16, out_type == GI_BF16, false}, scratch, list, (int*)(list + n_rows), n_rows, width, columns, rank, n_adapters,
+           segment_of(n_rows, width, rank * n_slices, low), (int)segments_for(x_type, w_type, n_rows, width, rank * n_slices), Slices{n_slices, {0}, {0}}, stream};
+    bool fours = ldb % 4 == 0 && ldo % 4 == 0 && aligned(base, base_type == GI_BF16 ? 8 : 16) && aligned(out, out_type == GI_BF16 ? 8 : 16);
     for (int s = 0; s < n_slices; ++s) {
         GI_REQUIRE(slice_columns[s] > 0, "adapters_add: a packed projection of %d columns", slice_columns[s]);
+        fours = fours && slice_columns[s] % 4 == 0;
         c.slices.begin[s + 1] = c.slices.begin[s] + slice_columns[s];
     }
     GI_REQUIRE(c.slices.begin[n_slices] == columns, "adapters_add: the packed projections have %d columns, out has %d", c.slices.begin[n_slices], columns);
-    GI_REQUIRE(c.n_segments <= 65535 && (n_rows + 15) / 16 <= 65535, "adapters_add: %d rows of %d numbers are too many for one launch", n_rows, width);
-    const bool low = x_type == GI_BF16 && w_type == GI_BF16;
-    if (low) down<true, bf16_t, bf16_t>(c);
-    else if (x_type == GI_BF16) down<false, bf16_t, float>(c);
-    else if (w_type == GI_BF16) down<false, float, bf16_t>(c);
-    else down<false, float, float>(c);
+    c.io.vectors = fours;
+    if (low && few_rows(c)) {
+        add_few(c);
+        GI_CHECK_LAUNCH("adapters_add (few rows)");
+        return 0;
+    }
+    const int went = low ? down<true, bf16_t, bf16_t>(c) : x_type == GI_BF16 ? down<false, bf16_t, float>(c) : w_type == GI_BF16 ? down<false, float, bf16_t>(c) : down<false, float, float>(c);
+    if (went != 0) return went;
     GI_CHECK_LAUNCH("adapters_add (down)");
-    if (low) up_typed<true, bf16_t>(c, base_type, out_type);
-    else if (w_type == GI_BF16) up_typed<false, bf16_t>(c, base_type, out_type);
-    else up_typed<false, float>(c, base_type, out_type);
+    const int came = low ? up<true, bf16_t>(c) : w_type == GI_BF16 ? up<false, bf16_t>(c) : up<false, float>(c);
+    if (came != 0) return came;
     GI_CHECK_LAUNCH("adapters_add (up)");
     return 0;
 }

@@ -146,8 +146,8 @@ def lib():
         l.gi_sample_filtered_histogram_bytes.restype = c_int
         l.gi_verify_drafts_scratch_bytes.argtypes = [c_int, c_int, c_int]
         l.gi_verify_drafts_scratch_bytes.restype = c_long
-        l.gi_adapters_segments.argtypes = [c_int, c_int]
-        l.gi_adapters_segments.restype = c_int
+        l.gi_adapters_scratch_floats.argtypes = [c_int, c_int, c_int, c_int, c_int, c_int]
+        l.gi_adapters_scratch_floats.restype = c_long
         l.gi_attention_exact_spans.argtypes = [c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int]
         l.gi_attention_exact_spans.restype = c_int
         l.gi_attention_exact_part_floats.argtypes = [c_int, c_int, c_int, c_int, c_int, c_int, c_int]
@@ -2257,7 +2257,7 @@ def adapters_add(x, a, b, ids, out, scales=None, base=None, slices=None):
     (n, width), (n_adapters, columns, rank) = x.shape, b.shape
     if n == 0:
         return out
-    t = torch.empty(lib().gi_adapters_segments(n, width) * n * len(slices) * rank, dtype=torch.float32, device=x.device)
+    t = torch.empty(lib().gi_adapters_scratch_floats(_CODE[x.dtype], _CODE[a.dtype], n, width, rank, len(slices)), dtype=torch.float32, device=x.device)
     _call("gi_adapters_add", x.data_ptr(), _CODE[x.dtype], max(x.stride(0), width), a.data_ptr(), b.data_ptr(), _CODE[a.dtype], ids.data_ptr(), _ptr(scales), base.data_ptr(),
           _CODE[base.dtype], max(base.stride(0), columns), out.data_ptr(), _CODE[out.dtype], max(out.stride(0), columns), t.data_ptr(), n, width, columns, rank, len(slices),
           (c_int * len(slices))(*slices), n_adapters, _stream())

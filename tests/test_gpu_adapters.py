@@ -2,7 +2,7 @@
 
 How far a result may be off, with s the sum of the absolute values that its formula adds up (|base| + scale |B| |A| |x|):
   32-bit sums of at most width + rank + 4 terms, in whatever order, are off by at most that many steps of 2^-24 relative to s;
-  rows of A x that the matrix cores take as two bfloat16 pieces are off by 2^-16 relative (a half step of a half step, 2^-8 each);
+  sums A x that the matrix cores take as two bfloat16 pieces, where the result is bfloat16, are off by 2^-16 relative (a half step of a half step, 2^-8 each);
   a result stored as bfloat16 is off by 2^-8 of itself.
 """
 import pytest
@@ -48,10 +48,10 @@ def formula(x, a, b, ids, scales, base, slices, absolute=False):
     return out
 
 
-def assert_right(got, c, pieces=True):
+def assert_right(got, c):
     args = {k: c[k] for k in ("x", "a", "b", "ids", "scales", "base", "slices")}
     want, size = formula(**args), formula(**args, absolute=True)
-    steps = (c["x"].shape[1] + c["b"].shape[2] + 4) * 2.0 ** -24 + (2.0 ** -16 if c["x"].dtype == c["a"].dtype == BF16 else 0.0)
+    steps = (c["x"].shape[1] + c["b"].shape[2] + 4) * 2.0 ** -24 + (2.0 ** -16 if c["x"].dtype == c["a"].dtype == got.dtype == BF16 else 0.0)
     bound = size * steps
     if got.dtype == BF16:
         bound = bound + (want.abs() + bound) * 2.0 ** -8
@@ -246,7 +246,7 @@ def test_beside_the_shared_projection(n, dtype, result):
     c["base"] = c["x"].double() @ weight.double().t()
     size = formula(*(c[k] for k in ("x", "a", "b", "ids", "scales")), c["x"].double().abs() @ weight.double().abs().t(), None, absolute=True)
     want = formula(**c)
-    bound = size * ((2 * 512 + 16 + 8) * 2.0 ** -24 + (2.0 ** -16 if dtype == BF16 else 0.0))
+    bound = size * ((2 * 512 + 16 + 8) * 2.0 ** -24 + (2.0 ** -16 if dtype == result == BF16 else 0.0))
     if result == BF16:
         bound = bound + (want.abs() + bound) * 2.0 ** -8
     assert bool(((got.double() - want).abs() <= bound).all())
