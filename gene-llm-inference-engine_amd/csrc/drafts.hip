@@ -9,6 +9,9 @@
 //
 // A running sum over a hundred thousand tokens is compared with a number that falls anywhere between: in 32 bits one draw in some thousands
 // comes out a token off.  So weights exp((l - max) / T) and all sums are held in 64 bits, which this chip computes at the rate of 32.
+//
+// Three launches.  All rows once, in runs of 4,096 logits: the runs' maxima and sums.  Then, per request and run, the verdict (every workgroup of a request comes to it by itself, from the runs' numbers) and,
+// where a draft fell, the run's share of what is drawn from.  Then a request's draw.
 #include "common.h"
 
 namespace {
@@ -19,6 +22,8 @@ constexpr int PER = CHUNK / NT;             // ... and a thread: in the pick as 
 constexpr int MAX_CHUNKS = 1024;            // runs of a row that the pick holds in LDS (a vocabulary of 4 M tokens)
 constexpr int MAX_DRAFTS = 64;
 constexpr int MAX_ROWS = 2 * MAX_DRAFTS + 1;
+
+constexpr double NOTHING_LEFT = 1e-12;      // of p beside q
 
 enum { DONE = 0, PLAIN = 1, LESS_ROW = 2, LESS_TOKEN = 3 };       // what a request's last token is drawn from: nothing, p, max(p - q, 0), p without x
 
@@ -51,12 +56,40 @@ __device__ __forceinline__ int drafts_of(const Inputs& in, int r, long& first) {
 
 __device__ __forceinline__ float number(float v) { return v == v ? v : -INFINITY; }        // (what is no number is no token)
 
-// exp((l - top) / T): 1 for the largest, also where that is infinite; 0 for -infinity.
-__device__ __forceinline__ double weight(float l, float top, double inv_t) {
-    if (l == top) return top == -INFINITY ? 0.0 : 1.0;
-    const double d = (double)l - (double)top;
-    return d > -1e300 ? exp(d * inv_t) : 0.0;
+// 2^m for -1100 <= m <= 0: with n the nearest integer and |f| <= 1/2, 2^n (1 + f q(f)), q the polynomial through (2^f - 1) / f at nine Chebyshev points of [-1/2, 1/2]; off by less than
+// 4e-14 relative, less than a draw over a million tokens can notice.
+__device__ __forceinline__ double exp2_below(double m) {
+    const double n = rint(m), f = m - n;
+    double q = 1.0203114674825208e-07;
+    q = fma(f, q, 1.3255227922924584e-06);
+    q = fma(f, q, 1.5252686963534207e-05);
+    q = fma(f, q, 0.00015403455840537416);
+    q = fma(f, q, 0.001333355817880503);
+    q = fma(f, q, 0.009618129159412746);
+    q = fma(f, q, 0.05550410866476055);
+    q = fma(f, q, 0.24022650695812997);
+    q = fma(f, q, 0.6931471805599455);
+    return ldexp(fma(f, q, 1.0), (int)n);
 }
+
+// Weights exp((l - top) / T) of a row whose largest logit is `top`: 1 for the largest, 0 for what is no token (-infinity, NaN).
+struct Weigher {
+    double top, per;                        // log2(e) / T
+    bool plain;                             // what is no token may be taken as the lowest number: it weighs nothing either
+    float top_f;
+
+    __device__ Weigher(float largest, float t) : top((double)largest), per(1.4426950408889634 / (double)t), top_f(largest) {
+        plain = largest < INFINITY && (3.4028234663852886e38 + top) * per > 1100.0;
+    }
+    __device__ double fast(float l) const { return exp2_below(fmax(((double)fmaxf(l, -3.4028234663852886e38f) - top) * per, -1100.0)); }
+    __device__ double any(float l) const {
+        if (plain) return fast(l);
+        l = number(l);
+        if (l == top_f) return l == -INFINITY ? 0.0 : 1.0;
+        const double d = (double)l - top;
+        return d > -1e300 ? exp2_below(fmax(d * per, -1100.0)) : 0.0;
+    }
+};
 
 __device__ __forceinline__ double wave_sum_f64(double v) {
 #pragma unroll
@@ -64,12 +97,27 @@ __device__ __forceinline__ double wave_sum_f64(double v) {
     return v;
 }
 
-__device__ __forceinline__ void better(float& bv, int& bi, float ov, int oi) {
-    if (ov > bv || (ov == bv && oi < bi)) { bv = ov; bi = oi; }
-}
+// A thread's logits of a run: numbers i, of which `v[4 u + c]` is number begin + 4 (tid + NT u) + c where four may be loaded at once, begin + tid + NT (4 u + c) otherwise; behind `end` the last one again.
+struct RunOf {
+    int begin, end;
+    bool fours;
+    __device__ RunOf(const float* row, int run, int vocab) : begin(run * CHUNK), end(min(vocab, run * CHUNK + CHUNK)), fours((vocab & 3) == 0 && ((size_t)row & 15) == 0) {}
+    __device__ int at(int j) const { return fours ? begin + 4 * ((int)threadIdx.x + NT * (j >> 2)) + (j & 3) : begin + (int)threadIdx.x + NT * j; }
+    __device__ void load(const float* __restrict__ row, float (&v)[PER]) const {
+        if (fours) {
+#pragma unroll
+            for (int u = 0; u < PER / 4; ++u) {
+                const float4 w = *reinterpret_cast<const float4*>(row + min(at(4 * u), end - 4));
+                v[4 * u] = w.x; v[4 * u + 1] = w.y; v[4 * u + 2] = w.z; v[4 * u + 3] = w.w;
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < PER; ++j) v[j] = row[min(at(j), end - 1)];
+        }
+    }
+};
 
-// Largest logit (with its lowest index) and sum of exp((l - that) / T) of every run of CHUNK logits: workgroup (run, request, row), rows 0 .. K
-// the target's, K + 1 .. 2 K the drafter's.
+// Largest logit (with its lowest index) and sum of exp((l - that) / T) of every run: workgroup (run, request, row), rows 0 .. K the target's, K + 1 .. 2 K the drafter's.
 __global__ __launch_bounds__(NT) void parts_kernel(Inputs in, float* __restrict__ part_m, int* __restrict__ part_i, double* __restrict__ part_s) {
     __shared__ float sv[4];
     __shared__ int si[4];
@@ -81,154 +129,216 @@ __global__ __launch_bounds__(NT) void parts_kernel(Inputs in, float* __restrict_
     const bool greedy = arg_max_asked(t);
     if (n < 0 || (z <= in.K ? z > n : (z - in.K - 1 >= n || greedy))) return;
     const float* row = z <= in.K ? in.logits + (first + z) * in.stride : in.drafter + r * in.drafter_request + (z - in.K - 1) * in.drafter_row;
-    const int begin = blockIdx.x * CHUNK, end = min(in.vocab, begin + CHUNK);
+    const RunOf run(row, blockIdx.x, in.vocab);
     float v[PER];
-#pragma unroll
-    for (int u = 0; u < PER; ++u) v[u] = row[min(begin + tid + NT * u, end - 1)];
+    run.load(row, v);
     float bv = -INFINITY;
-    int bi = 0x7fffffff;
 #pragma unroll
-    for (int u = 0; u < PER; ++u) {
-        const int i = begin + tid + NT * u;
-        v[u] = i < end ? number(v[u]) : -INFINITY;
-        if (i < end && (v[u] > bv || bi == 0x7fffffff)) { bv = v[u]; bi = i; }
-    }
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) better(bv, bi, __shfl_xor(bv, off, 64), __shfl_xor(bi, off, 64));
-    if (lane == 0) { sv[wave] = bv; si[wave] = bi; }
+    for (int j = 0; j < PER; ++j) bv = fmaxf(bv, v[j]);                // (a number again behind the end is no larger; NaN is passed over)
+    bv = wave_max(bv);
+    if (lane == 0) sv[wave] = bv;
     __syncthreads();
-    bv = sv[0]; bi = si[0];
-    for (int w = 1; w < 4; ++w) better(bv, bi, sv[w], si[w]);
-    double sum = 0.0;
-    if (!greedy) {
-        const double inv_t = 1.0 / (double)t;
-#pragma unroll
-        for (int u = 0; u < PER; ++u) sum += weight(v[u], bv, inv_t);
-        sum = wave_sum_f64(sum);
-        if (lane == 0) red[wave] = sum;
-        __syncthreads();
-    }
-    if (tid == 0) {
-        const size_t at = ((size_t)r * (2 * in.K + 1) + z) * in.n_chunks + blockIdx.x;
-        part_m[at] = bv;
-        part_i[at] = bi;
-        part_s[at] = greedy ? 0.0 : ((red[0] + red[1]) + red[2]) + red[3];
-    }
-}
-
-// Which drafts stay: one workgroup a request, a wave a row.
-__global__ __launch_bounds__(NT) void judge_kernel(Inputs in, const float* __restrict__ part_m, const int* __restrict__ part_i,
-                                                   const double* __restrict__ part_s, Verdict* __restrict__ verdicts, int* __restrict__ tokens,
-                                                   int* __restrict__ counts) {
-    __shared__ float top[MAX_ROWS];
-    __shared__ int arg[MAX_ROWS];
-    __shared__ double whole[MAX_ROWS];
-    __shared__ int stays[MAX_DRAFTS];
-    const int r = blockIdx.x, tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, K = in.K;
-    long first;
-    const int n = drafts_of(in, r, first);
-    const float t = in.temperature[r];
-    const bool greedy = arg_max_asked(t);
-    const double inv_t = greedy ? 0.0 : 1.0 / (double)t;
-    for (int z = wave; z < 2 * K + 1; z += 4) {
-        if (n < 0 || (z <= K ? z > n : (in.drafter == nullptr || z - K - 1 >= n || greedy))) continue;
-        const size_t at = ((size_t)r * (2 * K + 1) + z) * in.n_chunks;
-        float bv = -INFINITY;
+    bv = fmaxf(fmaxf(sv[0], sv[1]), fmaxf(sv[2], sv[3]));
+    const size_t at = ((size_t)r * (2 * in.K + 1) + z) * in.n_chunks + blockIdx.x;
+    if (greedy) {                                                       // the lowest place of the largest (of -infinity where there are only such and NaN)
         int bi = 0x7fffffff;
-        for (int c = lane; c < in.n_chunks; c += 64) better(bv, bi, part_m[at + c], part_i[at + c]);
 #pragma unroll
-        for (int off = 32; off > 0; off >>= 1) better(bv, bi, __shfl_xor(bv, off, 64), __shfl_xor(bi, off, 64));
-        double sum = 0.0;
-        if (!greedy)
-            for (int c = lane; c < in.n_chunks; c += 64) sum += part_s[at + c] * weight(part_m[at + c], bv, inv_t);
-        sum = wave_sum_f64(sum);
-        if (lane == 0) { top[z] = bv; arg[z] = bi; whole[z] = sum; }
-    }
-    __syncthreads();
-    if (tid < MAX_DRAFTS) {
-        bool stay = false;
-        if (tid < n) {
-            const int x = in.drafts[(size_t)r * K + tid];
-            if (x >= 0 && x < in.vocab) {
-                if (greedy) {
-                    stay = x == arg[tid];
-                } else {
-                    const double p = weight(number(in.logits[(first + tid) * in.stride + x]), top[tid], inv_t);
-                    double q = 1.0, whole_q = 1.0;
-                    if (in.drafter != nullptr) {
-                        q = weight(number(in.drafter[r * in.drafter_request + tid * in.drafter_row + x]), top[K + 1 + tid], inv_t);
-                        whole_q = whole[K + 1 + tid];
-                    }
-                    // u q / whole_q < p / whole_p; a row without a token has no probabilities (its sum and all its weights are 0)
-                    const double u = (double)in.uniform[(size_t)r * (K + 1) + tid];
-                    stay = u * (whole_q > 0.0 ? q / whole_q : 0.0) < (whole[tid] > 0.0 ? p / whole[tid] : 0.0);
-                }
-            }
+        for (int j = 0; j < PER; ++j)
+            if (number(v[j]) == bv && run.at(j) < run.end) bi = min(bi, run.at(j));
+#pragma unroll
+        for (int off = 32; off > 0; off >>= 1) bi = min(bi, __shfl_xor(bi, off, 64));
+        if (lane == 0) si[wave] = bi;
+        __syncthreads();
+        if (tid == 0) {
+            part_m[at] = bv;
+            part_i[at] = min(min(si[0], si[1]), min(si[2], si[3]));
         }
-        stays[tid] = stay;
+        return;
     }
+    const Weigher weigh(bv, t);
+    double sum = 0.0;
+    if (weigh.plain) {
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+            const double w = weigh.fast(v[j]);
+            sum += run.at(j) < run.end ? w : 0.0;
+        }
+    } else {
+        for (int j = 0; j < PER; ++j)
+            if (run.at(j) < run.end) sum += weigh.any(v[j]);
+    }
+    sum = wave_sum_f64(sum);
+    if (lane == 0) red[wave] = sum;
     __syncthreads();
-    int kept = 0;
-    while (kept < n && stays[kept]) ++kept;
-    if (tid <= K) {
-        const int x = tid < kept ? in.drafts[(size_t)r * K + tid] : -1;
-        tokens[(size_t)r * (K + 1) + tid] = greedy && n >= 0 && tid == kept ? arg[kept] : x;
-    }
     if (tid == 0) {
-        counts[r] = n < 0 ? 0 : kept + 1;
-        Verdict v{kept, DONE, kept, -1, 0.f, 0.f, 0.0, 0.0};
-        if (n >= 0 && !greedy) {
-            v.top_p = top[kept];
-            v.sum_p = whole[kept];
-            v.kind = PLAIN;
-            if (kept < n) {
-                v.x = in.drafts[(size_t)r * K + kept];
-                if (in.drafter != nullptr) {
-                    v.kind = LESS_ROW;
-                    v.top_q = top[K + 1 + kept];
-                    v.sum_q = whole[K + 1 + kept];
-                } else if (v.x >= 0 && v.x < in.vocab) {
-                    v.kind = LESS_TOKEN;
-                }
-            }
-        }
-        verdicts[r] = v;
+        part_m[at] = bv;
+        part_s[at] = ((red[0] + red[1]) + red[2]) + red[3];
     }
 }
 
 // The weight token i is drawn with, up to a factor that all of a request's tokens share.
-__device__ __forceinline__ double drawn_weight(const Verdict& v, const float* __restrict__ row, const float* __restrict__ drafter, int i, double inv_t) {
-    const double p = weight(number(row[i]), v.top_p, inv_t);
-    if (v.kind == LESS_ROW) {
-        const double q = v.sum_q > 0.0 ? weight(number(drafter[i]), v.top_q, inv_t) / v.sum_q : 0.0;
-        return fmax((v.sum_p > 0.0 ? p / v.sum_p : 0.0) - q, 0.0);
+struct Drawn {
+    Weigher p, q;
+    double over_p, over_q;
+    int kind, x;
+    __device__ Drawn(const Verdict& v, float t) : p(v.top_p, t), q(v.top_q, t), over_p(v.sum_p > 0.0 ? 1.0 / v.sum_p : 0.0), over_q(v.sum_q > 0.0 ? 1.0 / v.sum_q : 0.0), kind(v.kind), x(v.x) {}
+    __device__ bool plain() const { return p.plain && (kind != LESS_ROW || q.plain); }
+    template <bool PLAIN_ROWS>
+    __device__ double operator()(float target, float drafter, int i) const {
+        const double w = PLAIN_ROWS ? p.fast(target) : p.any(target);
+        if (kind == LESS_ROW) return fmax(w * over_p - (PLAIN_ROWS ? q.fast(drafter) : q.any(drafter)) * over_q, 0.0);
+        return kind == LESS_TOKEN && i == x ? 0.0 : w;
     }
-    return v.kind == LESS_TOKEN && i == v.x ? 0.0 : p;
-}
+};
 
-// Sums of those weights over runs, where the parts do not hold them already: every run of a request whose drafter's row is taken off, and the run
-// that a draft is left out of.
-__global__ __launch_bounds__(NT) void rest_kernel(Inputs in, const Verdict* __restrict__ verdicts, double* __restrict__ rest) {
+// Which drafts stay, and the sums over runs of what is drawn from, where the parts do not hold them already: every run of a request whose drafter's row is taken off, and the run that a draft is
+// left out of.  Workgroup (run, request); run 0's writes what the request has so far.
+__global__ __launch_bounds__(NT) void judge_kernel(Inputs in, const float* __restrict__ part_m, const int* __restrict__ part_i, const double* __restrict__ part_s, Verdict* __restrict__ verdicts,
+                                                   double* __restrict__ rest, int* __restrict__ tokens, int* __restrict__ counts) {
+    __shared__ float top[MAX_ROWS];
+    __shared__ int arg[MAX_ROWS];
+    __shared__ double whole[MAX_ROWS];
+    __shared__ int stays;                                   // drafts before the first that falls
     __shared__ double red[4];
-    const int r = blockIdx.y, tid = threadIdx.x;
-    const Verdict v = verdicts[r];
-    if (v.kind != LESS_ROW && !(v.kind == LESS_TOKEN && v.x / CHUNK == (int)blockIdx.x)) return;
+    const int r = blockIdx.y, tid = threadIdx.x, K = in.K, member = tid & 15;
     long first;
-    drafts_of(in, r, first);
+    const int n = drafts_of(in, r, first);
+    const float t = in.temperature[r];
+    const bool greedy = arg_max_asked(t);
+    if (greedy && blockIdx.x != 0) return;
+    int x = -1;                                             // this thread's draft, its logits, its number
+    float target_x = -INFINITY, drafter_x = -INFINITY, u = 0.f;
+    if (tid < n) {
+        x = in.drafts[(size_t)r * K + tid];
+        if (x < 0 || x >= in.vocab) x = -1;
+        if (x >= 0 && !greedy) {
+            target_x = in.logits[(first + tid) * in.stride + x];
+            if (in.drafter != nullptr) drafter_x = in.drafter[r * in.drafter_request + tid * in.drafter_row + x];
+            u = in.uniform[(size_t)r * (K + 1) + tid];
+        }
+    }
+    for (int z = tid >> 4; z < 2 * K + 1; z += NT / 16) {   // sixteen lanes a row
+        if (n < 0 || (z <= K ? z > n : (in.drafter == nullptr || z - K - 1 >= n || greedy))) continue;
+        const size_t at = ((size_t)r * (2 * K + 1) + z) * in.n_chunks;
+        float largest = -INFINITY;
+        int place = 0x7fffffff;
+        double sum = 0.0;
+        for (int c0 = 0; c0 < in.n_chunks; c0 += 64) {      // (once, for up to 262,144 tokens)
+            float m[4];
+            int i[4] = {};
+            double s[4] = {};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int c = c0 + member + 16 * j;
+                m[j] = -INFINITY;
+                if (c < in.n_chunks) {
+                    m[j] = part_m[at + c];
+                    if (greedy) i[j] = part_i[at + c];
+                    else s[j] = part_s[at + c];
+                }
+            }
+            float bv = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+#pragma unroll
+            for (int off = 8; off > 0; off >>= 1) bv = fmaxf(bv, __shfl_xor(bv, off, 64));
+            const float now = fmaxf(largest, bv);
+            if (greedy) {
+                if (now > largest) place = 0x7fffffff;      // (a place of an earlier run that holds as much is lower)
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (c0 + member + 16 * j < in.n_chunks && m[j] == now) place = min(place, i[j]);
+            } else {
+                const Weigher weigh(now, t);
+                double more = 0.0;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) more += s[j] * weigh.any(m[j]);
+#pragma unroll
+                for (int off = 8; off > 0; off >>= 1) more += __shfl_xor(more, off, 64);
+                sum = sum * weigh.any(largest) + more;
+            }
+            largest = now;
+        }
+#pragma unroll
+        for (int off = 8; off > 0; off >>= 1) place = min(place, __shfl_xor(place, off, 64));
+        if (member == 0) { top[z] = largest; arg[z] = place; whole[z] = sum; }
+    }
+    __syncthreads();
+    static_assert(MAX_DRAFTS == 64, "one wave judges the drafts");
+    if (tid < MAX_DRAFTS) {
+        bool stay = false;
+        if (tid < n && x >= 0) {
+            if (greedy) {
+                stay = x == arg[tid];
+            } else {
+                // u q / whole_q < p / whole_p; a row without a token has no probabilities (its sum and all its weights are 0)
+                const double p = whole[tid] > 0.0 ? Weigher(top[tid], t).any(target_x) / whole[tid] : 0.0;
+                double q = 1.0;
+                if (in.drafter != nullptr) q = whole[K + 1 + tid] > 0.0 ? Weigher(top[K + 1 + tid], t).any(drafter_x) / whole[K + 1 + tid] : 0.0;
+                stay = (double)u * q < p;
+            }
+        }
+        const unsigned long long fell = __ballot(!stay);    // (the places behind the request's drafts among them)
+        if (tid == 0) stays = fell != 0 ? __ffsll((long long)fell) - 1 : MAX_DRAFTS;
+    }
+    __syncthreads();
+    const int kept = min(max(n, 0), stays);
+    Verdict v{kept, DONE, kept, -1, 0.f, 0.f, 0.0, 0.0};
+    if (n >= 0 && !greedy) {
+        v.top_p = top[kept];
+        v.sum_p = whole[kept];
+        v.kind = PLAIN;
+        if (kept < n) {
+            v.x = in.drafts[(size_t)r * K + kept];
+            if (in.drafter != nullptr) {
+                v.kind = LESS_ROW;
+                v.top_q = top[K + 1 + kept];
+                v.sum_q = whole[K + 1 + kept];
+            } else if (v.x >= 0 && v.x < in.vocab) {
+                v.kind = LESS_TOKEN;
+            }
+        }
+    }
+    if (blockIdx.x == 0) {
+        if (tid <= K) tokens[(size_t)r * (K + 1) + tid] = tid < kept ? in.drafts[(size_t)r * K + tid] : greedy && n >= 0 && tid == kept ? arg[kept] : -1;
+        if (tid == 0) {
+            counts[r] = n < 0 ? 0 : kept + 1;
+            verdicts[r] = v;
+        }
+    }
+    if (v.kind != LESS_ROW && !(v.kind == LESS_TOKEN && v.x / CHUNK == (int)blockIdx.x)) return;
     const float* row = in.logits + (first + v.row) * in.stride;
-    const float* drafter = in.drafter == nullptr ? nullptr : in.drafter + r * in.drafter_request + v.row * in.drafter_row;
-    const double inv_t = 1.0 / (double)in.temperature[r];
-    const int begin = blockIdx.x * CHUNK, end = min(in.vocab, begin + CHUNK);
+    const float* drafter = v.kind == LESS_ROW ? in.drafter + r * in.drafter_request + v.row * in.drafter_row : row;
+    const RunOf run(row, blockIdx.x, in.vocab), other(drafter, blockIdx.x, in.vocab);
+    float a[PER], b[PER];
     double sum = 0.0;
-    for (int i = begin + tid; i < end; i += NT) sum += drawn_weight(v, row, drafter, i, inv_t);
+    const Drawn drawn(v, t);
+    if (run.fours == other.fours && drawn.plain()) {
+        run.load(row, a);
+        if (v.kind == LESS_ROW) other.load(drafter, b);
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+            const double w = drawn.operator()<true>(a[j], b[j], run.at(j));
+            sum += run.at(j) < run.end ? w : 0.0;
+        }
+    } else {
+        for (int i = run.begin + tid; i < run.end; i += NT) sum += drawn.operator()<false>(row[i], drafter[i], i);
+    }
     sum = wave_sum_f64(sum);
     if ((tid & 63) == 0) red[tid >> 6] = sum;
     __syncthreads();
     if (tid == 0) rest[(size_t)r * in.n_chunks + blockIdx.x] = ((red[0] + red[1]) + red[2]) + red[3];
 }
 
-// The draw: one workgroup a request.  The run is found among the runs' sums, then the token in the run: a thread owns PER consecutive tokens,
-// a prefix sum over the threads finds the thread, which walks its tokens.
+__device__ __forceinline__ double scan_f64(double v, int lane) {               // inclusive, over a wave
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+        const double below = __shfl_up(v, off, 64);
+        if (lane >= off) v += below;
+    }
+    return v;
+}
+
+// The draw: one workgroup a request.  The run is found among the runs' sums (by a prefix sum over a wave's lanes, which share the runs out, and a walk over one lane's), then the token in the run: a
+// thread owns PER consecutive tokens, a prefix sum over the threads finds the thread, which walks its tokens.
 __global__ __launch_bounds__(NT) void pick_kernel(Inputs in, const Verdict* __restrict__ verdicts, const float* __restrict__ part_m, const double* __restrict__ part_s,
                                                   const double* __restrict__ rest, int* __restrict__ tokens) {
     __shared__ double sums[MAX_CHUNKS];
@@ -240,32 +350,40 @@ __global__ __launch_bounds__(NT) void pick_kernel(Inputs in, const Verdict* __re
     if (v.kind == DONE) return;
     long first;
     drafts_of(in, r, first);
+    const float t = in.temperature[r];
     const float* row = in.logits + (first + v.row) * in.stride;
-    const float* drafter = in.drafter == nullptr ? nullptr : in.drafter + r * in.drafter_request + v.row * in.drafter_row;
-    const double inv_t = 1.0 / (double)in.temperature[r];
+    const float* drafter = v.kind == LESS_ROW ? in.drafter + r * in.drafter_request + v.row * in.drafter_row : row;
     const size_t parts = ((size_t)r * (2 * in.K + 1) + v.row) * in.n_chunks;
+    const Weigher weigh(v.top_p, t);
     for (int attempt = 0; attempt < 2; ++attempt) {
         for (int c = tid; c < in.n_chunks; c += NT) {
             const bool own = v.kind == LESS_ROW || (v.kind == LESS_TOKEN && v.x / CHUNK == c);
-            sums[c] = own ? rest[(size_t)r * in.n_chunks + c] : part_s[parts + c] * weight(part_m[parts + c], v.top_p, inv_t);
+            sums[c] = own ? rest[(size_t)r * in.n_chunks + c] : part_s[parts + c] * weigh.any(part_m[parts + c]);
         }
         __syncthreads();
-        if (tid == 0) {
-            double total = 0.0;
-            for (int c = 0; c < in.n_chunks; ++c) total += sums[c];
+        if (wave == 0) {
+            const int each = (in.n_chunks + 63) / 64, from = lane * each, to = min(in.n_chunks, from + each);
+            double mine = 0.0;
+            for (int c = from; c < to; ++c) mine += sums[c];
+            const double upto = scan_f64(mine, lane), below = __shfl_up(upto, 1, 64), total = __shfl(upto, 63, 64);
             const double goal = (double)in.uniform[(size_t)r * (in.K + 1) + in.K] * total;
-            double before = 0.0, before_last = 0.0;
-            int run = -1, last = -1;
-            for (int c = 0; c < in.n_chunks && run < 0; ++c) {
-                if (goal < before + sums[c]) run = c;
-                else {
+            const unsigned long long beyond = __ballot(goal < upto && mine > 0.0), some = __ballot(mine > 0.0);
+            // the first lane whose runs end beyond the goal; by rounding, or for u = 1, the last that weighs anything
+            // (what rounding leaves of p beside an equal q is nothing: as much as that is a chance that no draft has to fall by)
+            const int owner = v.kind == LESS_ROW && total <= NOTHING_LEFT ? -1 : beyond != 0 ? __ffsll((long long)beyond) - 1 : some != 0 ? 63 - __clzll((long long)some) : -1;
+            if (lane == owner) {
+                double before = lane ? below : 0.0, before_last = before;
+                int run = -1, last = -1;
+                for (int c = from; c < to && run < 0; ++c) {
                     if (sums[c] > 0.0) { last = c; before_last = before; }
+                    if (goal < before + sums[c]) run = c;
                     before += sums[c];
                 }
+                the_run = run >= 0 ? run : last;
+                before_run = before_last;                  // (a run that holds the goal weighs something: the last seen)
+                target = goal;
             }
-            the_run = run >= 0 ? run : last;               // (rounding, or u = 1: the last run that weighs anything; -1: none does)
-            before_run = run >= 0 ? before : before_last;
-            target = goal;
+            if (owner < 0 && lane == 0) the_run = -1;
         }
         __syncthreads();
         if (the_run >= 0 || v.kind == PLAIN) break;
@@ -278,37 +396,43 @@ __global__ __launch_bounds__(NT) void pick_kernel(Inputs in, const Verdict* __re
         return;
     }
     const int begin = run * CHUNK, end = min(in.vocab, begin + CHUNK), lo = begin + tid * PER;
+    const Drawn drawn(v, t);
+    float a[PER], b[PER];
+#pragma unroll
+    for (int j = 0; j < PER; ++j) a[j] = row[min(lo + j, end - 1)];
+    if (v.kind == LESS_ROW)
+#pragma unroll
+        for (int j = 0; j < PER; ++j) b[j] = drafter[min(lo + j, end - 1)];
     double w[PER], mine = 0.0;
+    if (drawn.plain()) {
 #pragma unroll
-    for (int u = 0; u < PER; ++u) {
-        w[u] = lo + u < end ? drawn_weight(v, row, drafter, lo + u, inv_t) : 0.0;
-        mine += w[u];
-    }
-    double upto = mine;
+        for (int j = 0; j < PER; ++j) w[j] = drawn.operator()<true>(a[j], b[j], lo + j);
+    } else {
 #pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-        const double below = __shfl_up(upto, off, 64);
-        if (lane >= off) upto += below;
+        for (int j = 0; j < PER; ++j) w[j] = drawn.operator()<false>(a[j], b[j], lo + j);
     }
-    if (lane == 63) wave_total[wave] = upto;
-    if (tid == 0) winner = 0x7fffffff;
     int last = -1;                                         // the last token that weighs anything
 #pragma unroll
-    for (int u = 0; u < PER; ++u)
-        if (w[u] > 0.0) last = lo + u;
+    for (int j = 0; j < PER; ++j) {
+        if (lo + j >= end) w[j] = 0.0;
+        mine += w[j];
+        if (w[j] > 0.0) last = lo + j;
+    }
+    const double upto = scan_f64(mine, lane), below = __shfl_up(upto, 1, 64);
+    if (lane == 63) wave_total[wave] = upto;
+    if (tid == 0) winner = 0x7fffffff;
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) last = max(last, __shfl_xor(last, off, 64));
     if (lane == 0) last_of_wave[wave] = last;
-    const double below_lane = __shfl_up(upto, 1, 64);
     __syncthreads();
     double walk = before_run;
     for (int k = 0; k < wave; ++k) walk += wave_total[k];
-    if (lane) walk += below_lane;
+    if (lane) walk += below;
     int hit = 0x7fffffff;
 #pragma unroll
-    for (int u = 0; u < PER; ++u) {
-        walk += w[u];
-        if (hit == 0x7fffffff && w[u] > 0.0 && walk > target) hit = lo + u;
+    for (int j = 0; j < PER; ++j) {
+        walk += w[j];
+        if (hit == 0x7fffffff && w[j] > 0.0 && walk > target) hit = lo + j;
     }
     if (hit != 0x7fffffff) atomicMin(&winner, hit);
     __syncthreads();
@@ -346,10 +470,8 @@ GI_API int gi_verify_drafts(const float* logits, int n_rows, long stride, const 
     int* part_i = (int*)(part_m + rows * n_chunks);
     parts_kernel<<<dim3(n_chunks, n_requests, drafter != nullptr ? 2 * K + 1 : K + 1), NT, 0, stream>>>(in, part_m, part_i, part_s);
     GI_CHECK_LAUNCH("verify_drafts (parts)");
-    judge_kernel<<<n_requests, NT, 0, stream>>>(in, part_m, part_i, part_s, verdicts, tokens, counts);
+    judge_kernel<<<dim3(n_chunks, n_requests), NT, 0, stream>>>(in, part_m, part_i, part_s, verdicts, rest, tokens, counts);
     GI_CHECK_LAUNCH("verify_drafts (judge)");
-    rest_kernel<<<dim3(n_chunks, n_requests), NT, 0, stream>>>(in, verdicts, rest);
-    GI_CHECK_LAUNCH("verify_drafts (rest)");
     pick_kernel<<<n_requests, NT, 0, stream>>>(in, verdicts, part_m, part_s, rest, tokens);
     GI_CHECK_LAUNCH("verify_drafts (pick)");
     return 0;

@@ -48,6 +48,7 @@ def verify(logits, drafts, temperature, uniform, draft_logits=None, n_drafts=Non
                         q = softmax(draft_logits[r, j], t)
                         stays = inside and float(uniform[r, j]) * q[x] < p[x]
                         rest = np.maximum(p - q, 0.0)
+                        rest = p if rest.sum() <= 1e-12 else rest
                     elif inside:
                         stays = float(uniform[r, j]) < p[x]
                         rest = p.copy()
