@@ -18,8 +18,8 @@ namespace {
 
 constexpr int CHUNK = 4096;                 // logits of a row that a workgroup takes
 constexpr int NT = 256;
-constexpr int PER = CHUNK / NT;             // ... and a thread: in the pick as many consecutive ones
-constexpr int MAX_CHUNKS = 1024;            // runs of a row that the pick holds in LDS (a vocabulary of 4 M tokens)
+constexpr int PER = CHUNK / NT;             // ... and a thread
+constexpr int MAX_CHUNKS = 1024;            // runs of a row: as many as the threads that draw (a vocabulary of 4 M tokens)
 constexpr int MAX_DRAFTS = 64;
 constexpr int MAX_ROWS = 2 * MAX_DRAFTS + 1;
 
@@ -56,10 +56,11 @@ __device__ __forceinline__ int drafts_of(const Inputs& in, int r, long& first) {
 
 __device__ __forceinline__ float number(float v) { return v == v ? v : -INFINITY; }        // (what is no number is no token)
 
-// 2^m for -1100 <= m <= 0: with n the nearest integer and |f| <= 1/2, 2^n (1 + f q(f)), q the polynomial through (2^f - 1) / f at nine Chebyshev points of [-1/2, 1/2]; off by less than
-// 4e-14 relative, less than a draw over a million tokens can notice.
+// 2^m for m <= 0, 0 below 2^-1020 and for what is no number: with n the nearest integer (what is left in the low bits of a sum with 1.5 * 2^52) and |f| <= 1/2, 2^n (1 + f q(f)), q the polynomial
+// through (2^f - 1) / f at nine Chebyshev points of [-1/2, 1/2]; off by less than 4e-14 relative, less than a draw over a million tokens can notice.  No conversions and no scaling by an instruction of its
+// own: those run at a quarter of the rate.
 __device__ __forceinline__ double exp2_below(double m) {
-    const double n = rint(m), f = m - n;
+    const double shifted = m + 6755399441055744.0, n = shifted - 6755399441055744.0, f = m - n;
     double q = 1.0203114674825208e-07;
     q = fma(f, q, 1.3255227922924584e-06);
     q = fma(f, q, 1.5252686963534207e-05);
@@ -69,26 +70,18 @@ __device__ __forceinline__ double exp2_below(double m) {
     q = fma(f, q, 0.05550410866476055);
     q = fma(f, q, 0.24022650695812997);
     q = fma(f, q, 0.6931471805599455);
-    return ldexp(fma(f, q, 1.0), (int)n);
+    const long long w = __double_as_longlong(fma(f, q, 1.0)), at = __double_as_longlong(shifted);
+    const int high = (int)(w >> 32) + ((int)at << 20);
+    return m > -1020.0 ? __hiloint2double(high, (int)w) : 0.0;
 }
 
 // Weights exp((l - top) / T) of a row whose largest logit is `top`: 1 for the largest, 0 for what is no token (-infinity, NaN).
 struct Weigher {
     double top, per;                        // log2(e) / T
-    bool plain;                             // what is no token may be taken as the lowest number: it weighs nothing either
-    float top_f;
-
-    __device__ Weigher(float largest, float t) : top((double)largest), per(1.4426950408889634 / (double)t), top_f(largest) {
-        plain = largest < INFINITY && (3.4028234663852886e38 + top) * per > 1100.0;
-    }
-    __device__ double fast(float l) const { return exp2_below(fmax(((double)fmaxf(l, -3.4028234663852886e38f) - top) * per, -1100.0)); }
-    __device__ double any(float l) const {
-        if (plain) return fast(l);
-        l = number(l);
-        if (l == top_f) return l == -INFINITY ? 0.0 : 1.0;
-        const double d = (double)l - top;
-        return d > -1e300 ? exp2_below(fmax(d * per, -1100.0)) : 0.0;
-    }
+    bool plain;                             // the largest is not infinite
+    __device__ Weigher(float largest, float t) : top((double)largest), per(1.4426950408889634 / (double)t), plain(largest < INFINITY) {}
+    __device__ double fast(float l) const { return exp2_below(((double)l - top) * per); }
+    __device__ double any(float l) const { return plain ? fast(l) : l == INFINITY ? 1.0 : 0.0; }
 };
 
 __device__ __forceinline__ double wave_sum_f64(double v) {
@@ -338,13 +331,14 @@ __device__ __forceinline__ double scan_f64(double v, int lane) {               /
 }
 
 // The draw: one workgroup a request.  The run is found among the runs' sums (by a prefix sum over a wave's lanes, which share the runs out, and a walk over one lane's), then the token in the run: a
-// thread owns PER consecutive tokens, a prefix sum over the threads finds the thread, which walks its tokens.
-__global__ __launch_bounds__(NT) void pick_kernel(Inputs in, const Verdict* __restrict__ verdicts, const float* __restrict__ part_m, const double* __restrict__ part_s,
-                                                  const double* __restrict__ rest, int* __restrict__ tokens) {
+// thread owns four consecutive tokens, a prefix sum over the threads finds the thread, which walks its tokens.
+constexpr int PICK_NT = 1024, PICK_WAVES = PICK_NT / 64, PICK_PER = CHUNK / PICK_NT;
+__global__ __launch_bounds__(PICK_NT) void pick_kernel(Inputs in, const Verdict* __restrict__ verdicts, const float* __restrict__ part_m, const double* __restrict__ part_s,
+                                                       const double* __restrict__ rest, int* __restrict__ tokens) {
     __shared__ double sums[MAX_CHUNKS];
-    __shared__ double wave_total[4];
+    __shared__ double wave_total[PICK_WAVES];
     __shared__ double target, before_run;
-    __shared__ int the_run, winner, last_of_wave[4];
+    __shared__ int the_run, winner, last_one;
     const int r = blockIdx.x, tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
     Verdict v = verdicts[r];
     if (v.kind == DONE) return;
@@ -354,11 +348,10 @@ __global__ __launch_bounds__(NT) void pick_kernel(Inputs in, const Verdict* __re
     const float* row = in.logits + (first + v.row) * in.stride;
     const float* drafter = v.kind == LESS_ROW ? in.drafter + r * in.drafter_request + v.row * in.drafter_row : row;
     const size_t parts = ((size_t)r * (2 * in.K + 1) + v.row) * in.n_chunks;
-    const Weigher weigh(v.top_p, t);
     for (int attempt = 0; attempt < 2; ++attempt) {
-        for (int c = tid; c < in.n_chunks; c += NT) {
-            const bool own = v.kind == LESS_ROW || (v.kind == LESS_TOKEN && v.x / CHUNK == c);
-            sums[c] = own ? rest[(size_t)r * in.n_chunks + c] : part_s[parts + c] * weigh.any(part_m[parts + c]);
+        if (tid < in.n_chunks) {                           // (MAX_CHUNKS threads)
+            const bool own = v.kind == LESS_ROW || (v.kind == LESS_TOKEN && v.x / CHUNK == tid);
+            sums[tid] = own ? rest[(size_t)r * in.n_chunks + tid] : part_s[parts + tid] * Weigher(v.top_p, t).any(part_m[parts + tid]);
         }
         __syncthreads();
         if (wave == 0) {
@@ -385,6 +378,8 @@ __global__ __launch_bounds__(NT) void pick_kernel(Inputs in, const Verdict* __re
             }
             if (owner < 0 && lane == 0) the_run = -1;
         }
+        if (tid == 0) winner = 0x7fffffff;
+        if (tid == 64) last_one = -1;
         __syncthreads();
         if (the_run >= 0 || v.kind == PLAIN) break;
         v.kind = PLAIN;                                    // nothing is left of p beside q: p itself
@@ -395,52 +390,36 @@ __global__ __launch_bounds__(NT) void pick_kernel(Inputs in, const Verdict* __re
         if (tid == 0) tokens[(size_t)r * (in.K + 1) + v.kept] = 0;
         return;
     }
-    const int begin = run * CHUNK, end = min(in.vocab, begin + CHUNK), lo = begin + tid * PER;
+    const int begin = run * CHUNK, end = min(in.vocab, begin + CHUNK), lo = begin + tid * PICK_PER;
     const Drawn drawn(v, t);
-    float a[PER], b[PER];
-#pragma unroll
-    for (int j = 0; j < PER; ++j) a[j] = row[min(lo + j, end - 1)];
-    if (v.kind == LESS_ROW)
-#pragma unroll
-        for (int j = 0; j < PER; ++j) b[j] = drafter[min(lo + j, end - 1)];
-    double w[PER], mine = 0.0;
-    if (drawn.plain()) {
-#pragma unroll
-        for (int j = 0; j < PER; ++j) w[j] = drawn.operator()<true>(a[j], b[j], lo + j);
-    } else {
-#pragma unroll
-        for (int j = 0; j < PER; ++j) w[j] = drawn.operator()<false>(a[j], b[j], lo + j);
-    }
+    double w[PICK_PER], mine = 0.0;
     int last = -1;                                         // the last token that weighs anything
 #pragma unroll
-    for (int j = 0; j < PER; ++j) {
+    for (int j = 0; j < PICK_PER; ++j) {
+        const int i = min(lo + j, end - 1);
+        w[j] = drawn.operator()<false>(row[i], drafter[i], i);
         if (lo + j >= end) w[j] = 0.0;
         mine += w[j];
         if (w[j] > 0.0) last = lo + j;
     }
     const double upto = scan_f64(mine, lane), below = __shfl_up(upto, 1, 64);
     if (lane == 63) wave_total[wave] = upto;
-    if (tid == 0) winner = 0x7fffffff;
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) last = max(last, __shfl_xor(last, off, 64));
-    if (lane == 0) last_of_wave[wave] = last;
     __syncthreads();
     double walk = before_run;
     for (int k = 0; k < wave; ++k) walk += wave_total[k];
     if (lane) walk += below;
     int hit = 0x7fffffff;
 #pragma unroll
-    for (int j = 0; j < PER; ++j) {
+    for (int j = 0; j < PICK_PER; ++j) {
         walk += w[j];
         if (hit == 0x7fffffff && w[j] > 0.0 && walk > target) hit = lo + j;
     }
-    if (hit != 0x7fffffff) atomicMin(&winner, hit);
+    // the lowest token that reaches beyond the goal: of a wave, then of all
+    const unsigned long long hits = __ballot(hit != 0x7fffffff), some = __ballot(last >= 0);
+    if (hits != 0 && lane == __ffsll((long long)hits) - 1) atomicMin(&winner, hit);
+    if (some != 0 && lane == 63 - __clzll((long long)some)) atomicMax(&last_one, last);
     __syncthreads();
-    if (tid == 0) {
-        int pick = winner;
-        if (pick == 0x7fffffff) pick = max(max(last_of_wave[0], last_of_wave[1]), max(last_of_wave[2], last_of_wave[3]));
-        tokens[(size_t)r * (in.K + 1) + v.kept] = max(pick, 0);
-    }
+    if (tid == 0) tokens[(size_t)r * (in.K + 1) + v.kept] = max(winner != 0x7fffffff ? winner : last_one, 0);
 }
 
 }  // namespace
@@ -472,7 +451,7 @@ GI_API int gi_verify_drafts(const float* logits, int n_rows, long stride, const 
     GI_CHECK_LAUNCH("verify_drafts (parts)");
     judge_kernel<<<dim3(n_chunks, n_requests), NT, 0, stream>>>(in, part_m, part_i, part_s, verdicts, rest, tokens, counts);
     GI_CHECK_LAUNCH("verify_drafts (judge)");
-    pick_kernel<<<n_requests, NT, 0, stream>>>(in, verdicts, part_m, part_s, rest, tokens);
+    pick_kernel<<<n_requests, PICK_NT, 0, stream>>>(in, verdicts, part_m, part_s, rest, tokens);
     GI_CHECK_LAUNCH("verify_drafts (pick)");
     return 0;
 }
