@@ -59,17 +59,22 @@ __device__ __forceinline__ float number(float v) { return v == v ? v : -INFINITY
 // 2^m for m <= 0, 0 below 2^-1020 and for what is no number: with n the nearest integer (what is left in the low bits of a sum with 1.5 * 2^52) and |f| <= 1/2, 2^n (1 + f q(f)), q the polynomial
 // through (2^f - 1) / f at nine Chebyshev points of [-1/2, 1/2]; off by less than 4e-14 relative, less than a draw over a million tokens can notice.  No conversions and no scaling by an instruction of its
 // own: those run at a quarter of the rate.
+__device__ __forceinline__ double horner(double f, double q, double c) {        // f q + c, the coefficient in scalar registers: as the accumulator it would be moved there for every step
+    double out;
+    asm("v_fma_f64 %0, %1, %2, %3" : "=v"(out) : "v"(f), "v"(q), "s"(c));
+    return out;
+}
 __device__ __forceinline__ double exp2_below(double m) {
     const double shifted = m + 6755399441055744.0, n = shifted - 6755399441055744.0, f = m - n;
     double q = 1.0203114674825208e-07;
-    q = fma(f, q, 1.3255227922924584e-06);
-    q = fma(f, q, 1.5252686963534207e-05);
-    q = fma(f, q, 0.00015403455840537416);
-    q = fma(f, q, 0.001333355817880503);
-    q = fma(f, q, 0.009618129159412746);
-    q = fma(f, q, 0.05550410866476055);
-    q = fma(f, q, 0.24022650695812997);
-    q = fma(f, q, 0.6931471805599455);
+    q = horner(f, q, 1.3255227922924584e-06);
+    q = horner(f, q, 1.5252686963534207e-05);
+    q = horner(f, q, 0.00015403455840537416);
+    q = horner(f, q, 0.001333355817880503);
+    q = horner(f, q, 0.009618129159412746);
+    q = horner(f, q, 0.05550410866476055);
+    q = horner(f, q, 0.24022650695812997);
+    q = horner(f, q, 0.6931471805599455);
     const long long w = __double_as_longlong(fma(f, q, 1.0)), at = __double_as_longlong(shifted);
     const int high = (int)(w >> 32) + ((int)at << 20);
     return m > -1020.0 ? __hiloint2double(high, (int)w) : 0.0;
@@ -90,82 +95,98 @@ __device__ __forceinline__ double wave_sum_f64(double v) {
     return v;
 }
 
-// A thread's logits of a run: numbers i, of which `v[4 u + c]` is number begin + 4 (tid + NT u) + c where four may be loaded at once, begin + tid + NT (4 u + c) otherwise; behind `end` the last one again.
+// A thread's logits of a run: `v[4 u + c]` is number begin + 4 (tid + NT u) + c where four may be loaded at once, number begin + tid + NT (4 u + c) otherwise; -infinity behind `end`.
 struct RunOf {
     int begin, end;
     bool fours;
     __device__ RunOf(const float* row, int run, int vocab) : begin(run * CHUNK), end(min(vocab, run * CHUNK + CHUNK)), fours((vocab & 3) == 0 && ((size_t)row & 15) == 0) {}
     __device__ int at(int j) const { return fours ? begin + 4 * ((int)threadIdx.x + NT * (j >> 2)) + (j & 3) : begin + (int)threadIdx.x + NT * j; }
     __device__ void load(const float* __restrict__ row, float (&v)[PER]) const {
-        if (fours) {
+        const float* from = row + begin;
+        const int there = end - begin;
+        int tid = threadIdx.x;
+        asm volatile("" : "+v"(tid));                       // (worked out anew for every row: kept over a loop, the sixteen places would cost registers, and waves)
+        if (fours && there == CHUNK) {
 #pragma unroll
             for (int u = 0; u < PER / 4; ++u) {
-                const float4 w = *reinterpret_cast<const float4*>(row + min(at(4 * u), end - 4));
+                const float4 w = reinterpret_cast<const float4*>(from + 4 * NT * u)[tid];
                 v[4 * u] = w.x; v[4 * u + 1] = w.y; v[4 * u + 2] = w.z; v[4 * u + 3] = w.w;
+            }
+        } else if (fours) {
+#pragma unroll
+            for (int u = 0; u < PER / 4; ++u) {
+                const int i = 4 * (tid + NT * u);
+                const float4 w = *reinterpret_cast<const float4*>(from + min(i, there - 4));
+                const bool in = i < there;
+                v[4 * u] = in ? w.x : -INFINITY; v[4 * u + 1] = in ? w.y : -INFINITY; v[4 * u + 2] = in ? w.z : -INFINITY; v[4 * u + 3] = in ? w.w : -INFINITY;
             }
         } else {
 #pragma unroll
-            for (int j = 0; j < PER; ++j) v[j] = row[min(at(j), end - 1)];
+            for (int j = 0; j < PER; ++j) {
+                const int i = tid + NT * j;
+                const float w = from[min(i, there - 1)];
+                v[j] = i < there ? w : -INFINITY;
+            }
         }
     }
 };
 
-// Largest logit (with its lowest index) and sum of exp((l - that) / T) of every run: workgroup (run, request, row), rows 0 .. K the target's, K + 1 .. 2 K the drafter's.
+// Largest logit (with its lowest index) and sum of exp((l - that) / T) of every run: workgroup (run, request, group of rows).  Of the rows that the request has, the target's 0 .. n and the drafter's 0 .. n - 1 behind
+// them, every gridDim.z-th is a workgroup's.
 __global__ __launch_bounds__(NT) void parts_kernel(Inputs in, float* __restrict__ part_m, int* __restrict__ part_i, double* __restrict__ part_s) {
-    __shared__ float sv[4];
-    __shared__ int si[4];
-    __shared__ double red[4];
-    const int r = blockIdx.y, z = blockIdx.z, tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+    __shared__ float sv[2][4];
+    __shared__ int si[2][4];
+    __shared__ double red[2][4];
+    const int r = blockIdx.y, tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
     long first;
     const int n = drafts_of(in, r, first);
+    if (n < 0) return;
     const float t = in.temperature[r];
     const bool greedy = arg_max_asked(t);
-    if (n < 0 || (z <= in.K ? z > n : (z - in.K - 1 >= n || greedy))) return;
-    const float* row = z <= in.K ? in.logits + (first + z) * in.stride : in.drafter + r * in.drafter_request + (z - in.K - 1) * in.drafter_row;
-    const RunOf run(row, blockIdx.x, in.vocab);
-    float v[PER];
-    run.load(row, v);
-    float bv = -INFINITY;
+    const int n_rows = n + 1 + (greedy || in.drafter == nullptr ? 0 : n);
+    for (int i = blockIdx.z, turn = 0; i < n_rows; i += gridDim.z, turn ^= 1) {          // (two places for what meets in LDS in turn: one barrier a meeting)
+        const float* row = i <= n ? in.logits + (first + i) * in.stride : in.drafter + r * in.drafter_request + (i - n - 1) * in.drafter_row;
+        const RunOf run(row, blockIdx.x, in.vocab);
+        float v[PER];
+        run.load(row, v);
+        float bv = -INFINITY;
 #pragma unroll
-    for (int j = 0; j < PER; ++j) bv = fmaxf(bv, v[j]);                // (a number again behind the end is no larger; NaN is passed over)
-    bv = wave_max(bv);
-    if (lane == 0) sv[wave] = bv;
-    __syncthreads();
-    bv = fmaxf(fmaxf(sv[0], sv[1]), fmaxf(sv[2], sv[3]));
-    const size_t at = ((size_t)r * (2 * in.K + 1) + z) * in.n_chunks + blockIdx.x;
-    if (greedy) {                                                       // the lowest place of the largest (of -infinity where there are only such and NaN)
-        int bi = 0x7fffffff;
+        for (int j = 0; j < PER; ++j) bv = fmaxf(bv, v[j]);            // (NaN is passed over)
+        bv = wave_max(bv);
+        if (lane == 0) sv[turn][wave] = bv;
+        barrier_lds();
+        bv = fmaxf(fmaxf(sv[turn][0], sv[turn][1]), fmaxf(sv[turn][2], sv[turn][3]));
+        const size_t at = ((size_t)r * (2 * in.K + 1) + (i <= n ? i : in.K + i - n)) * in.n_chunks + blockIdx.x;
+        if (greedy) {                                                   // the lowest place of the largest (of -infinity where there are only such and NaN)
+            int mine = PER;
 #pragma unroll
-        for (int j = 0; j < PER; ++j)
-            if (number(v[j]) == bv && run.at(j) < run.end) bi = min(bi, run.at(j));
+            for (int j = PER - 1; j >= 0; --j) mine = number(v[j]) == bv ? j : mine;
+            int bi = mine < PER && run.at(mine) < run.end ? run.at(mine) : 0x7fffffff;       // (a thread's numbers ascend)
 #pragma unroll
-        for (int off = 32; off > 0; off >>= 1) bi = min(bi, __shfl_xor(bi, off, 64));
-        if (lane == 0) si[wave] = bi;
-        __syncthreads();
+            for (int off = 32; off > 0; off >>= 1) bi = min(bi, __shfl_xor(bi, off, 64));
+            if (lane == 0) si[turn][wave] = bi;
+            barrier_lds();
+            if (tid == 0) {
+                part_m[at] = bv;
+                part_i[at] = min(min(si[turn][0], si[turn][1]), min(si[turn][2], si[turn][3]));
+            }
+            continue;
+        }
+        const Weigher weigh(bv, t);
+        double sum = 0.0;
+        if (weigh.plain) {
+#pragma unroll
+            for (int j = 0; j < PER; ++j) sum += weigh.fast(v[j]);
+        } else {
+            for (int k = run.begin + tid; k < run.end; k += NT) sum += weigh.any(row[k]);
+        }
+        sum = wave_sum_f64(sum);
+        if (lane == 0) red[turn][wave] = sum;
+        barrier_lds();
         if (tid == 0) {
             part_m[at] = bv;
-            part_i[at] = min(min(si[0], si[1]), min(si[2], si[3]));
+            part_s[at] = ((red[turn][0] + red[turn][1]) + red[turn][2]) + red[turn][3];
         }
-        return;
-    }
-    const Weigher weigh(bv, t);
-    double sum = 0.0;
-    if (weigh.plain) {
-#pragma unroll
-        for (int j = 0; j < PER; ++j) {
-            const double w = weigh.fast(v[j]);
-            sum += run.at(j) < run.end ? w : 0.0;
-        }
-    } else {
-        for (int j = 0; j < PER; ++j)
-            if (run.at(j) < run.end) sum += weigh.any(v[j]);
-    }
-    sum = wave_sum_f64(sum);
-    if (lane == 0) red[wave] = sum;
-    __syncthreads();
-    if (tid == 0) {
-        part_m[at] = bv;
-        part_s[at] = ((red[0] + red[1]) + red[2]) + red[3];
     }
 }
 
@@ -176,11 +197,13 @@ struct Drawn {
     int kind, x;
     __device__ Drawn(const Verdict& v, float t) : p(v.top_p, t), q(v.top_q, t), over_p(v.sum_p > 0.0 ? 1.0 / v.sum_p : 0.0), over_q(v.sum_q > 0.0 ? 1.0 / v.sum_q : 0.0), kind(v.kind), x(v.x) {}
     __device__ bool plain() const { return p.plain && (kind != LESS_ROW || q.plain); }
-    template <bool PLAIN_ROWS>
-    __device__ double operator()(float target, float drafter, int i) const {
-        const double w = PLAIN_ROWS ? p.fast(target) : p.any(target);
-        if (kind == LESS_ROW) return fmax(w * over_p - (PLAIN_ROWS ? q.fast(drafter) : q.any(drafter)) * over_q, 0.0);
-        return kind == LESS_TOKEN && i == x ? 0.0 : w;
+    __device__ double weight(float target, float drafter, bool left_out) const {       // of plain rows
+        const double w = p.fast(target);
+        return kind == LESS_ROW ? fmax(w * over_p - q.fast(drafter) * over_q, 0.0) : left_out ? 0.0 : w;
+    }
+    __device__ double any(float target, float drafter, int i) const {
+        const double w = p.any(target);
+        return kind == LESS_ROW ? fmax(w * over_p - q.any(drafter) * over_q, 0.0) : kind == LESS_TOKEN && i == x ? 0.0 : w;
     }
 };
 
@@ -307,13 +330,13 @@ __global__ __launch_bounds__(NT) void judge_kernel(Inputs in, const float* __res
     if (run.fours == other.fours && drawn.plain()) {
         run.load(row, a);
         if (v.kind == LESS_ROW) other.load(drafter, b);
+        int left_out = -1;                                  // which of this thread's numbers x is
+        if (v.kind == LESS_TOKEN)
+            for (int j = 0; j < PER; ++j) left_out = run.at(j) == v.x ? j : left_out;
 #pragma unroll
-        for (int j = 0; j < PER; ++j) {
-            const double w = drawn.operator()<true>(a[j], b[j], run.at(j));
-            sum += run.at(j) < run.end ? w : 0.0;
-        }
+        for (int j = 0; j < PER; ++j) sum += drawn.weight(a[j], b[j], j == left_out);       // (nothing behind the end)
     } else {
-        for (int i = run.begin + tid; i < run.end; i += NT) sum += drawn.operator()<false>(row[i], drafter[i], i);
+        for (int i = run.begin + tid; i < run.end; i += NT) sum += drawn.any(row[i], drafter[i], i);
     }
     sum = wave_sum_f64(sum);
     if ((tid & 63) == 0) red[tid >> 6] = sum;
@@ -397,7 +420,7 @@ __global__ __launch_bounds__(PICK_NT) void pick_kernel(Inputs in, const Verdict*
 #pragma unroll
     for (int j = 0; j < PICK_PER; ++j) {
         const int i = min(lo + j, end - 1);
-        w[j] = drawn.operator()<false>(row[i], drafter[i], i);
+        w[j] = drawn.any(row[i], drafter[i], i);
         if (lo + j >= end) w[j] = 0.0;
         mine += w[j];
         if (w[j] > 0.0) last = lo + j;
@@ -447,7 +470,9 @@ GI_API int gi_verify_drafts(const float* logits, int n_rows, long stride, const 
     Verdict* verdicts = (Verdict*)(rest + (size_t)n_requests * n_chunks);
     float* part_m = (float*)(verdicts + n_requests);
     int* part_i = (int*)(part_m + rows * n_chunks);
-    parts_kernel<<<dim3(n_chunks, n_requests, drafter != nullptr ? 2 * K + 1 : K + 1), NT, 0, stream>>>(in, part_m, part_i, part_s);
+    const int most = drafter != nullptr ? 2 * K + 1 : K + 1;
+    const int groups = (int)min((long)most, max(1l, 32 * (long)gi_compute_units() / ((long)n_chunks * n_requests)));
+    parts_kernel<<<dim3(n_chunks, n_requests, groups), NT, 0, stream>>>(in, part_m, part_i, part_s);
     GI_CHECK_LAUNCH("verify_drafts (parts)");
     judge_kernel<<<dim3(n_chunks, n_requests), NT, 0, stream>>>(in, part_m, part_i, part_s, verdicts, rest, tokens, counts);
     GI_CHECK_LAUNCH("verify_drafts (judge)");
