@@ -348,11 +348,16 @@ def _ptr(t):
 
 def _here(what, *tensors):
     """The operands lie on the device whose stream the kernels are launched on."""
-    _dev(*tensors)
-    current = torch.cuda.current_device()
+    current = -1
     for t in tensors:
-        if t is not None and t.device.index != current:
-            raise KernelError(f"{what}: an operand lies on {t.device}, the current device is cuda:{current}")
+        if t is not None:
+            device = t.get_device()
+            if device < 0:
+                raise KernelError("kernel operands must lie in device memory")
+            if current < 0:
+                current = _raw_device() if _raw_device is not None else torch.cuda.current_device()
+            if device != current:
+                raise KernelError(f"{what}: an operand lies on cuda:{device}, the current device is cuda:{current}")
 
 
 def device_arch() -> str:
@@ -2180,20 +2185,20 @@ def verify_drafts(logits, drafts, temperature, uniform, tokens, counts, draft_lo
     from max(p - q, 0) where a draft fell (from p, where less than 1e-12 of that is left: a draft outside the vocabulary may fall with q equal to p) and from p where none did.  Logits of -infinity or NaN are no tokens (a row of nothing else lets no draft stay and gives token
     0), a draft outside the vocabulary falls.  A request whose rows do not lie among those given gets count 0."""
     what = "verify_drafts"
-    if not (logits.dtype == torch.float32 and logits.dim() == 2 and logits.shape[1] > 0 and (logits.stride(1) == 1 or logits.shape[1] == 1)):
+    f32, i32 = torch.float32, torch.int32
+    if not (logits.dtype == f32 and logits.dim() == 2 and logits.shape[1] > 0 and (logits.stride(1) == 1 or logits.shape[1] == 1)):
         raise KernelError(f"{what}: logits must be float32 [rows, vocab] with unit inner stride")
-    if not (drafts.dtype == torch.int32 and drafts.dim() == 2 and drafts.is_contiguous()):
+    if not (drafts.dtype == i32 and drafts.dim() == 2 and drafts.is_contiguous()):
         raise KernelError(f"{what}: drafts must be a contiguous int32 [requests, K] tensor")
     (n_rows, vocab), (n, k) = logits.shape, drafts.shape
     if k > VERIFY_MAX_DRAFTS:
         raise KernelError(f"{what}: {k} drafts a request, at most {VERIFY_MAX_DRAFTS} are taken")
-    for t, name, shape in ((temperature, "temperature", (n,)), (uniform, "uniform", (n, k + 1))):
-        if not (t.dtype == torch.float32 and t.is_contiguous() and t.shape == shape):
-            raise KernelError(f"{what}: {name} must be a contiguous float32 tensor of shape {shape}")
-    for t, name, shape in ((tokens, "tokens", (n, k + 1)), (counts, "counts", (n,)), (n_drafts, "n_drafts", (n,)), (first_row, "first_row", (n,))):
-        if t is not None and not (t.dtype == torch.int32 and t.is_contiguous() and t.shape == shape):
-            raise KernelError(f"{what}: {name} must be a contiguous int32 tensor of shape {shape}")
-    if draft_logits is not None and not (draft_logits.dtype == torch.float32 and draft_logits.shape == (n, k, vocab) and (draft_logits.stride(2) == 1 or vocab == 1)):
+    one, wide = (n,), (n, k + 1)
+    for t, name, dtype, shape in ((temperature, "temperature", f32, one), (uniform, "uniform", f32, wide), (tokens, "tokens", i32, wide), (counts, "counts", i32, one),
+                                  (n_drafts, "n_drafts", i32, one), (first_row, "first_row", i32, one)):
+        if t is not None and not (t.dtype == dtype and t.shape == shape and t.is_contiguous()):
+            raise KernelError(f"{what}: {name} must be a contiguous {dtype} tensor of shape {shape}")
+    if draft_logits is not None and not (draft_logits.dtype == f32 and draft_logits.shape == (n, k, vocab) and (draft_logits.stride(2) == 1 or vocab == 1)):
         raise KernelError(f"{what}: draft_logits must be float32 {(n, k, vocab)} with unit inner stride")
     if first_row is None and n_drafts is None and n_rows < n * (k + 1):
         raise KernelError(f"{what}: {n} requests of {k} drafts need {n * (k + 1)} rows of logits, there are {n_rows}")
@@ -2201,17 +2206,33 @@ def verify_drafts(logits, drafts, temperature, uniform, tokens, counts, draft_lo
         return tokens, counts
     if n_rows == 0:
         raise KernelError(f"{what}: there are no rows of logits")
+    if n_rows > 1 and logits.stride(0) < vocab:
+        raise KernelError(f"{what}: the rows of logits overlap")
     _here(what, logits, drafts, temperature, uniform, tokens, counts, draft_logits, n_drafts, first_row)
-    scratch = torch.empty(lib().gi_verify_drafts_scratch_bytes(n, k, vocab), dtype=torch.uint8, device=logits.device)
-    drafter = draft_logits if k > 0 else None
-    _call("gi_verify_drafts", logits.data_ptr(), n_rows, logits.stride(0) if n_rows > 1 else max(logits.stride(0), vocab), _ptr(drafter), drafter.stride(0) if drafter is not None else 0,
-          drafter.stride(1) if drafter is not None else 0, drafts.data_ptr(), _ptr(n_drafts), _ptr(first_row), temperature.data_ptr(), uniform.data_ptr(), tokens.data_ptr(),
-          counts.data_ptr(), scratch.data_ptr(), n, k, vocab, _stream())
+    scratch = torch.empty(_verify_scratch(n, k, vocab), dtype=torch.uint8, device=logits.device)
+    apart, between = (draft_logits.stride(0), draft_logits.stride(1)) if draft_logits is not None else (0, 0)
+    _call("gi_verify_drafts", logits.data_ptr(), n_rows, max(logits.stride(0), vocab), _ptr(draft_logits) if k else None, apart, between, drafts.data_ptr(), _ptr(n_drafts), _ptr(first_row),
+          temperature.data_ptr(), uniform.data_ptr(), tokens.data_ptr(), counts.data_ptr(), scratch.data_ptr(), n, k, vocab, _stream())
     return tokens, counts
+
+
+@lru_cache(maxsize=1024)
+def _verify_scratch(n, k, vocab) -> int:
+    return lib().gi_verify_drafts_scratch_bytes(n, k, vocab)
 
 
 # ------------------------------------------------------------------------------------------------ adapters
 ADAPTER_MAX_SLICES, ADAPTER_MAX_RANK = 4, 256
+
+
+@lru_cache(maxsize=1024)
+def _adapter_slices(slices):
+    return (c_int * len(slices))(*slices)
+
+
+@lru_cache(maxsize=4096)
+def _adapter_scratch(x_code, w_code, n, width, rank, n_slices) -> int:
+    return lib().gi_adapters_scratch_floats(x_code, w_code, n, width, rank, n_slices)
 
 
 def adapters_check(x, a, b, ids, out, scales, base, slices):
@@ -2219,26 +2240,26 @@ def adapters_check(x, a, b, ids, out, scales, base, slices):
     what = "adapters_add"
     if not (x.dim() == 2 and a.dim() == 3 and b.dim() == 3 and out.dim() == 2):
         raise KernelError(f"{what}: x [rows, width], a [adapters, ranks, width], b [adapters, columns, rank] and out [rows, columns] are needed")
-    (n, width), (n_adapters, columns, rank) = x.shape, b.shape
-    slices = (columns,) if slices is None else tuple(int(c) for c in slices)
+    (n, width), (n_adapters, columns, rank), shape = x.shape, b.shape, out.shape
+    slices = (columns,) if slices is None else tuple(slices)
     if not (1 <= len(slices) <= ADAPTER_MAX_SLICES and min(slices) > 0 and sum(slices) == columns):
         raise KernelError(f"{what}: slices {slices} are not 1 to {ADAPTER_MAX_SLICES} positive numbers that add up to the {columns} columns")
-    if not (a.shape == (n_adapters, len(slices) * rank, width) and out.shape == (n, columns) and base.shape == (n, columns)):
+    if not (a.shape == (n_adapters, len(slices) * rank, width) and shape == (n, columns) and (base is out or base.shape == shape)):
         raise KernelError(f"{what}: x {tuple(x.shape)}, a {tuple(a.shape)}, b {tuple(b.shape)}, base {tuple(base.shape)} and out {tuple(out.shape)} do not fit ({len(slices)} projections)")
-    if 0 in (width, rank, n_adapters):
+    if not (width and rank and n_adapters):
         raise KernelError(f"{what}: {n_adapters} adapters of rank {rank} beside a width of {width} have no entries")
     if rank > ADAPTER_MAX_RANK:
         raise KernelError(f"{what}: rank {rank}, at most {ADAPTER_MAX_RANK} is taken")
     if not (a.dtype == b.dtype and a.is_contiguous() and b.is_contiguous()):
         raise KernelError(f"{what}: a and b must be contiguous and of one dtype")
-    if not (ids.dtype == torch.int32 and ids.is_contiguous() and ids.shape == (n,)):
+    if not (ids.dtype == torch.int32 and ids.shape == (n,) and ids.is_contiguous()):
         raise KernelError(f"{what}: ids must be a contiguous int32 [rows] tensor")
-    if scales is not None and not (scales.dtype == torch.float32 and scales.is_contiguous() and scales.shape == (n_adapters,)):
+    if scales is not None and not (scales.dtype == torch.float32 and scales.shape == (n_adapters,) and scales.is_contiguous()):
         raise KernelError(f"{what}: scales must be a contiguous float32 [adapters] tensor")
-    for t, name in ((x, "x"), (a, "a"), (base, "base"), (out, "out")):
-        _code(t, f"{what}: {name}")
-    for t, name in ((x, "x"), (base, "base"), (out, "out")):
-        if not ((t.stride(1) == 1 or t.shape[1] == 1) and (n <= 1 or t.stride(0) >= t.shape[1])):
+    for t, name in ((x, "x"), (a, "a"), (out, "out")) if base is out else ((x, "x"), (a, "a"), (base, "base"), (out, "out")):
+        if t.dtype not in _CODE:
+            _code(t, f"{what}: {name}")
+        if t is not a and not ((t.stride(1) == 1 or t.shape[1] == 1) and (n <= 1 or t.stride(0) >= t.shape[1])):
             raise KernelError(f"{what}: {name} must have unit inner stride and rows that do not overlap")
     if n:
         _here(what, x, a, b, ids, out, scales, base)
@@ -2257,10 +2278,11 @@ def adapters_add(x, a, b, ids, out, scales=None, base=None, slices=None):
     (n, width), (n_adapters, columns, rank) = x.shape, b.shape
     if n == 0:
         return out
-    t = torch.empty(lib().gi_adapters_scratch_floats(_CODE[x.dtype], _CODE[a.dtype], n, width, rank, len(slices)), dtype=torch.float32, device=x.device)
-    _call("gi_adapters_add", x.data_ptr(), _CODE[x.dtype], max(x.stride(0), width), a.data_ptr(), b.data_ptr(), _CODE[a.dtype], ids.data_ptr(), _ptr(scales), base.data_ptr(),
-          _CODE[base.dtype], max(base.stride(0), columns), out.data_ptr(), _CODE[out.dtype], max(out.stride(0), columns), t.data_ptr(), n, width, columns, rank, len(slices),
-          (c_int * len(slices))(*slices), n_adapters, _stream())
+    x_code, w_code = _CODE[x.dtype], _CODE[a.dtype]
+    scratch = torch.empty(_adapter_scratch(x_code, w_code, n, width, rank, len(slices)), dtype=torch.float32, device=x.device)
+    _call("gi_adapters_add", x.data_ptr(), x_code, max(x.stride(0), width), a.data_ptr(), b.data_ptr(), w_code, ids.data_ptr(), _ptr(scales), base.data_ptr(), _CODE[base.dtype],
+          max(base.stride(0), columns), out.data_ptr(), _CODE[out.dtype], max(out.stride(0), columns), scratch.data_ptr(), n, width, columns, rank, len(slices), _adapter_slices(slices),
+          n_adapters, _stream())
     return out
 
 
