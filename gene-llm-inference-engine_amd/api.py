@@ -18,7 +18,7 @@ from typing import Iterable, List, Optional, Sequence
 import torch
 
 from .kernels import ops
-from .engine import Engine, EngineConfig, EngineRequest, Runner, generate, load_model, random_model
+from .engine import Engine, EngineConfig, EngineRequest, Runner, generate, generate_with_drafts, load_model, random_model
 from .sampling import Sampler, SamplerConfig
 
 
@@ -73,8 +73,11 @@ class LLM:
         return self._profile.report(self.runner.rows_run - rows, self.runner.steps_run - steps, time.perf_counter() - since)
 
     def generate(self, prompt_ids: Sequence[int], steps: int = 0, temperature: float = 0.8, top_k: int = 0, top_p: float = 1.0,
-                 seed: int = 1, on_token=None):
+                 seed: int = 1, on_token=None, drafter: Optional["LLM"] = None, n_drafts: int = 4):
+        """drafter: a cheaper model of the same vocabulary, which proposes up to n_drafts tokens a step (`engine.generate_with_drafts`)."""
         sampler = Sampler(SamplerConfig(temperature, top_k, top_p, seed), self.model.spec.vocab_size)
+        if drafter is not None:
+            return generate_with_drafts(self.runner, drafter.runner, sampler, prompt_ids, n_drafts, steps, self.end_tokens, on_token)
         return generate(self.runner, sampler, prompt_ids, steps, self.end_tokens, on_token)
 
     def engine(self, config: Optional[EngineConfig] = None) -> Engine:

@@ -438,6 +438,11 @@ class CacheManager:
         for g in self.groups:
             g.sync(upload, stage)
 
+    @property
+    def rewinds(self) -> bool:
+        """Whether a request can be cut to any length: no fixed-size state, and no group that gives pages back on the way."""
+        return not self._state_needed and not any(g.need.forgets for g in self.groups)
+
     # --------------------------------------------------------------------------------- views
     def kv(self, entry: int):
         """(cache of the entry's layer [page, 2, kv_head, place, hd], device page table, window)."""

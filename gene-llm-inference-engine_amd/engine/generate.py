@@ -14,7 +14,8 @@ import time
 from dataclasses import dataclass, field
 from typing import Callable, Iterable, List, Optional, Sequence
 
-from ..sampling import Sampler, sample_rows_on_device
+from ..cache.pages import OutOfPages
+from ..sampling import Sampler, SamplerConfig, kept_drafts, sample_rows_on_device, verify_rows
 from .runner import Runner, StepEntry
 
 
@@ -26,6 +27,8 @@ class GenerateResult:
     prefill_ms: float = 0.0          # the prompt, including the sampling of the first new token
     decode_ms: float = 0.0
     decode_steps: int = 0
+    drafted_tokens: int = 0          # tokens that a drafter proposed, and how many of them stayed
+    kept_tokens: int = 0
 
 
 def generate(runner: Runner, sampler: Sampler, prompt_tokens: Sequence[int], max_positions: int = 0,
@@ -95,6 +98,121 @@ def generate(runner: Runner, sampler: Sampler, prompt_tokens: Sequence[int], max
                 token = nxt
         if result.generated_tokens:
             result.decode_ms = (time.perf_counter() - t_first) * 1e3
+    finally:
+        runner.close(request)
+    return result
+
+
+def generate_with_drafts(runner: Runner, drafter: Runner, sampler: Sampler, prompt_tokens: Sequence[int], n_drafts: int = 4, max_positions: int = 0,
+                         end_tokens: Iterable[int] = (), on_token: Optional[Callable[[int], None]] = None, prefill_rows: Optional[int] = None, request="generate",
+                         draft=None, judge=None) -> GenerateResult:
+    """`generate` with a second, cheaper model of the same vocabulary that runs ahead: `drafter` proposes up to `n_drafts` tokens one by one, a single step of `runner`
+    brings the logits at all their places, and of the proposals as many stay as leave the sequence distributed as the target's own
+    (`sampling.verify_rows`; a greedy sampler's tokens are `generate`'s, and so are those of one with top-k or top-p, whose proposals stay where they are what its own draw gives:
+    all but for the rounding of bfloat16 products, which add up in another order for several rows than for one).
+    What was fed beyond is cut off again, so neither model may keep a state or give pages back behind a window.
+    The drafter draws at the sampler's settings from numbers of its own.  draft(logits, sampler) -> token and judge(logits, drafts, sampler, draft_logits) -> new tokens replace the device's
+    (tests without a GPU use them)."""
+    import torch
+    prompt = [int(t) for t in prompt_tokens]
+    if not prompt:
+        raise ValueError("generate: prompt has no tokens")
+    if n_drafts < 1 or n_drafts > 64:
+        raise ValueError(f"generate: 1 to 64 drafts can be judged at once, not {n_drafts}")
+    vocab = runner.model.spec.vocab_size
+    if drafter is runner or drafter.model.spec.vocab_size != vocab:
+        raise ValueError("generate: the drafter must be another runner whose model has the same vocabulary")
+    for r, what in ((runner, "target"), (drafter, "drafter")):
+        if not r.cache.rewinds:
+            raise ValueError(f"generate: the {what} keeps a state or gives pages back; drafts that fall could not be taken back")
+        if len(prompt) > r.max_positions:
+            raise ValueError(f"generate: prompt of {len(prompt)} tokens does not fit in the context length {r.max_positions} of the {what}")
+    context = runner.max_positions
+    steps = context if max_positions <= 0 else min(max_positions, context)
+    end_tokens = set(int(t) for t in end_tokens)
+    config = sampler.config
+    own = Sampler(SamplerConfig(config.temperature, config.top_k, config.top_p, config.seed ^ 0x6472616674), vocab)
+    filtered = sampler.kind == "filtered"
+    most = min(n_drafts, runner.max_rows - 1)
+    result = GenerateResult(prompt_tokens=prompt)
+    tokens = list(prompt)                                     # all that is known; runner holds tokens[:pos]
+
+    def feed(r, upto):
+        while r.cache.length(request) < upto:
+            at = r.cache.length(request)
+            r.step([StepEntry(request, tokens[at:min(at + min(prefill_rows or r.max_rows, r.max_rows), upto)], ())])
+
+    runner.open(request)
+    try:
+        drafter.open(request)
+        try:
+            pos = min(len(prompt) - 1, steps)
+            t_start = t_first = time.perf_counter()
+            feed(runner, pos)
+            proposals = torch.zeros((1, max(most, 1)), dtype=torch.int32, device=getattr(drafter.model, "device", "cpu"))
+            rows = None
+            while pos < steps:
+                k = max(0, min(most, steps - pos - 1, drafter.max_positions - pos))
+                drafts: List[int] = []
+                if k:
+                    try:
+                        # what the drafter has not seen (the last token, and the one before where all of its proposals stayed), then one proposal after the other
+                        feed(drafter, pos)
+                        logits = drafter.step([StepEntry(request, [tokens[pos]], (0,))])
+                        if rows is None and not filtered and not sampler.config.greedy:
+                            rows = torch.empty((1, most, vocab), dtype=torch.float32, device=logits.device)
+                        for j in range(k):
+                            if rows is not None:
+                                rows[0, j].copy_(logits[0])
+                            token = sample_rows_on_device(logits, [own]) if draft is None else torch.tensor([draft(logits[0], own)], dtype=torch.int32)
+                            proposals[0, j:j + 1].copy_(token)
+                            if j + 1 == k:
+                                break
+                            if getattr(drafter, "can_step_from_device", False):           # (the host need not know the proposal to have the next one made)
+                                logits = drafter.step_from_device([request], token)
+                            else:
+                                logits = drafter.step([StepEntry(request, [int(token[0])], (0,))])
+                        drafts = proposals[0, :k].tolist()
+                    except OutOfPages:                        # (what has been proposed so far is lost)
+                        k, drafts = 0, []
+                try:
+                    logits = runner.step([StepEntry(request, [tokens[pos]] + drafts, tuple(range(k + 1)))])
+                except OutOfPages:
+                    if not k:
+                        raise
+                    k, drafts = 0, []                         # the last pages are the target's own
+                    logits = runner.step([StepEntry(request, [tokens[pos]], (0,))])
+                beside = rows[:, :k] if rows is not None and k else None
+                if judge is not None:
+                    new = judge(logits, drafts, sampler, beside)
+                elif filtered:
+                    new = kept_drafts(logits, drafts, sampler)
+                else:
+                    new = verify_rows(logits, proposals[:, :k].contiguous(), [sampler], beside)[0]
+                result.drafted_tokens += k
+                result.kept_tokens += len(new) - 1
+                if not result.generated_tokens:
+                    t_first = time.perf_counter()
+                    result.prefill_ms = (t_first - t_start) * 1e3
+                else:
+                    result.decode_steps += 1
+                pos += len(new)
+                runner.truncate(request, pos)
+                drafter.truncate(request, min(drafter.cache.length(request), pos))
+                for token in new:
+                    tokens.append(int(token))
+                    result.generated_tokens.append(int(token))
+                    if token in end_tokens:
+                        result.stopped_by_end_token = True
+                        break
+                    if on_token is not None:
+                        on_token(int(token))
+                if result.stopped_by_end_token:
+                    break
+            if result.generated_tokens:
+                result.decode_ms = (time.perf_counter() - t_first) * 1e3
+        finally:
+            drafter.close(request)
     finally:
         runner.close(request)
     return result

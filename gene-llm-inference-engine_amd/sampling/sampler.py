@@ -10,6 +10,9 @@ Rules (src/sampler/sampler.h:1-14, src/sampler/sampler.cpp:25-129):
      u times the kept mass; without filtering the walk is in index order.
 All of it runs on the device, on the logits where the step left them; `filtered_draw` states
 steps 2-4 on the host as the reference has them, for one row.
+
+Drafted tokens (`verify_rows_on_device`; the reference has none): of tokens that something cheaper than the target proposed, as many
+stay as leave the sequence distributed as if the target had drawn every token.
 """
 from __future__ import annotations
 
@@ -207,3 +210,69 @@ def sample_rows_on_device(logits: torch.Tensor, samplers: Sequence[Sampler]) -> 
 def sample_rows(logits: torch.Tensor, samplers: Sequence[Sampler]) -> List[int]:
     """`sample_rows_on_device`, with the tokens brought to the host."""
     return sample_rows_on_device(logits, samplers).tolist()
+
+
+def verify_rows_on_device(logits: torch.Tensor, drafts: torch.Tensor, samplers: Sequence[Sampler], draft_logits=None, n_drafts=None):
+    """Judges drafted tokens (`ops.verify_drafts`): request i brings drafts[i, :n_drafts[i]] (int32 [n, K] on the device; n_drafts: numbers, None for K
+    each) and the next n_drafts[i] + 1 rows of `logits`, the target's before each draft and behind the last.  draft_logits: float32 [n, K, vocab], what the
+    drafts were drawn from at the sampler's temperature; None: drafts without probabilities.  Nothing waits; the tokens that stay and the one behind
+    them (int32 [n, K + 1], -1 beyond) and how many those are (int32 [n]) stay on the device.  A sampler that is not greedy draws one
+    uniform number for every draft of its request and one for the token behind.  Samplers with top-k or top-p are refused: their rows are drawn from and compared (`kept_drafts`)."""
+    n, k = drafts.shape
+    brought = [k] * n if n_drafts is None else [int(c) for c in n_drafts]
+    if n != len(samplers) or n != len(brought):
+        raise ValueError(f"drafts of {n} requests for {len(samplers)} samplers and {len(brought)} numbers of drafts")
+    if any(not 0 <= c <= k for c in brought):
+        raise ValueError(f"a request brings 0 to {k} of its {k} drafts, not {brought}")
+    if logits.shape[0] != sum(brought) + n:
+        raise ValueError(f"{logits.shape[0]} rows of logits for {sum(brought)} drafts of {n} requests")
+    if any(s.kind == "filtered" for s in samplers):
+        raise ValueError("drafts are judged against whole distributions: a sampler with top-k or top-p has another")
+    host = np.zeros(n * (k + 4), dtype=np.float32)
+    uniform, ints = host[n:n * (k + 2)].reshape(n, k + 1), host.view(np.int32)
+    row = 0
+    for i, s in enumerate(samplers):
+        if s.kind != "greedy":
+            host[i] = s.temperature
+            for j in range(brought[i]):
+                uniform[i, j] = s.next_uniform()
+            uniform[i, k] = s.next_uniform()
+        ints[n * (k + 2) + i], ints[n * (k + 3) + i] = brought[i], row
+        row += brought[i] + 1
+    dev = logits.device
+    params = _to_device(host, dev)
+    numbers = params.view(torch.int32)
+    tokens = torch.empty((n, k + 1), dtype=torch.int32, device=dev)
+    counts = torch.empty(n, dtype=torch.int32, device=dev)
+    return ops.verify_drafts(logits, drafts, params[:n], params[n:n * (k + 2)].view(n, k + 1), tokens, counts, draft_logits=draft_logits,
+                             n_drafts=numbers[n * (k + 2):n * (k + 3)], first_row=numbers[n * (k + 3):])
+
+
+def verify_rows(logits: torch.Tensor, drafts: torch.Tensor, samplers: Sequence[Sampler], draft_logits=None, n_drafts=None) -> List[List[int]]:
+    """`verify_rows_on_device`, with every request's new tokens brought to the host."""
+    tokens, counts = verify_rows_on_device(logits, drafts, samplers, draft_logits, n_drafts)
+    return [row[:c] for row, c in zip(tokens.tolist(), counts.tolist())]
+
+
+def kept_drafts(logits: torch.Tensor, drafts: Sequence[int], sampler: Sampler, sample=sample_rows) -> List[int]:
+    """One request's new tokens where the sampler filters: every row of `logits` (before each draft and behind the last) is drawn from as
+    a step without drafts would, and drafts stay while they are what was drawn.  The tokens are those of the same sampler without drafts, and its stream of uniform numbers ends
+    where it would have; a draft stays less often than against the whole distribution."""
+    states = []
+
+    class Each:                                                   # the sampler for every row in turn, with the stream's states in between kept
+        config, kind, temperature = sampler.config, sampler.kind, sampler.temperature
+
+        @staticmethod
+        def next_uniform():
+            u = sampler.next_uniform()
+            states.append(sampler.stream.state)
+            return u
+
+    drawn = sample(logits, [Each] * logits.shape[0])
+    kept = 0
+    while kept < len(drafts) and drawn[kept] == int(drafts[kept]):
+        kept += 1
+    if states:
+        sampler.stream.state = states[kept]
+    return [int(t) for t in drawn[:kept + 1]]
