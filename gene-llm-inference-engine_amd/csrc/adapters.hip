@@ -673,6 +673,80 @@ __global__ __launch_bounds__(256) void adapters_up_few_kernel(const float* __res
 
 bool aligned(const void* p, int bytes) { return (size_t)p % bytes == 0; }
 
+// Both ways in one launch, where making a row's sums anew for every strip of its columns costs less than a second launch: a wave makes every fourth sum, then a thread has its columns as above.
+__global__ __launch_bounds__(256) void adapters_both_few_kernel(const bf16_t* __restrict__ x, long ldx, const bf16_t* __restrict__ a, const bf16_t* __restrict__ b, const float* __restrict__ scales,
+                                                                const int* __restrict__ ids, Rows io, int width, int rank, Slices slices, int n_adapters) {
+    __shared__ float t[MAX_RANK];
+    const int row = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int s = 0;
+    while (s + 1 < slices.n && (int)blockIdx.x >= slices.strip[s + 1]) ++s;
+    const int begin = slices.begin[s] + ((int)blockIdx.x - slices.strip[s]) * 256 * FEW_COLUMNS + threadIdx.x, end = slices.begin[s + 1];
+    const int e = ids[row];
+    const bool some = e >= 0 && e < n_adapters;
+    if (!some && io.base == io.out) return;
+    float was[FEW_COLUMNS], sum[FEW_COLUMNS];
+#pragma unroll
+    for (int c = 0; c < FEW_COLUMNS; ++c) {
+        was[c] = number1(io.base, (size_t)row * io.ldb + min(begin + 256 * c, end - 1), io.low_base);
+        sum[c] = 0.f;
+    }
+    if (some) {
+        const bf16_t* br[FEW_COLUMNS];
+        uint4 v[FEW_COLUMNS];
+#pragma unroll
+        for (int c = 0; c < FEW_COLUMNS; ++c) {
+            br[c] = b + ((size_t)e * slices.begin[slices.n] + min(begin + 256 * c, end - 1)) * rank;
+            v[c] = *reinterpret_cast<const uint4*>(br[c]);
+        }
+        const float scale = scales != nullptr ? scales[e] : 1.f;
+        const bf16_t* xr = x + (size_t)row * ldx;
+        const bf16_t* ae = a + ((size_t)e * slices.n + s) * rank * width;
+        for (int k0 = 0; k0 < rank; k0 += 16) {            // four sums of a wave at a time
+            float four[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 2
+            for (int k = 8 * lane; k < width; k += 512) {
+                const uint4 xv = *reinterpret_cast<const uint4*>(xr + k);
+                uint4 av[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) av[i] = *reinterpret_cast<const uint4*>(ae + (size_t)min(k0 + wave + 4 * i, rank - 1) * width + k);
+                const uint32_t xw[4] = {xv.x, xv.y, xv.z, xv.w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const uint32_t aw[4] = {av[i].x, av[i].y, av[i].z, av[i].w};
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) {
+                        four[i] = fmaf(__uint_as_float(xw[u] << 16), __uint_as_float(aw[u] << 16), four[i]);
+                        four[i] = fmaf(__uint_as_float(xw[u] & 0xffff0000u), __uint_as_float(aw[u] & 0xffff0000u), four[i]);
+                    }
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                four[i] = wave_sum(four[i]);
+                if (lane == 0 && k0 + wave + 4 * i < rank) t[k0 + wave + 4 * i] = four[i];
+            }
+        }
+        __syncthreads();
+        for (int k = 0; k < rank; k += 8) {
+#pragma unroll
+            for (int c = 0; c < FEW_COLUMNS; ++c) {
+                const uint32_t w[4] = {v[c].x, v[c].y, v[c].z, v[c].w};
+                if (k + 8 < rank) v[c] = *reinterpret_cast<const uint4*>(br[c] + k + 8);
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    sum[c] = fmaf(t[k + 2 * u], __uint_as_float(w[u] << 16), sum[c]);
+                    sum[c] = fmaf(t[k + 2 * u + 1], __uint_as_float(w[u] & 0xffff0000u), sum[c]);
+                }
+            }
+        }
+#pragma unroll
+        for (int c = 0; c < FEW_COLUMNS; ++c) was[c] = fmaf(scale, sum[c], was[c]);
+    }
+#pragma unroll
+    for (int c = 0; c < FEW_COLUMNS; ++c)
+        if (begin + 256 * c < end) store1(io.out, (size_t)row * io.ldo + begin + 256 * c, was[c], io.low_out);
+}
+
 struct Call {
     const void* x; long ldx; const void* a; const void* b; const int* ids; const float* scales; Rows io; float* sums; Tile* list; int* n_listed;
     int n_rows, width, columns, rank, n_adapters, segment, n_segments;
@@ -780,15 +854,23 @@ bool few_rows(const Call& c) {
 void add_few(const Call& c) {
     const int ranks = c.rank * c.slices.n;
     const long items = (long)c.n_rows * ranks;
+    Slices slices = c.slices;
+    for (int s = 0; s < slices.n; ++s) slices.strip[s + 1] = slices.strip[s] + (slices.begin[s + 1] - slices.begin[s] + 256 * FEW_COLUMNS - 1) / (256 * FEW_COLUMNS);
+    const dim3 strips(slices.strip[slices.n], c.n_rows);
+    const long again = (long)c.rank * c.width * 2;         // bytes of A that every strip's workgroup reads
+    // One launch takes the host 3 us less than two, and the device as long as two where a workgroup reads 64 KB of A again (1 row of 2,048 onto 2,048 or 8,192, rank 16: 4.7 us either way); at 128 KB 5.7 us
+    // against 4.8, at 256 KB 9.0 against 5.4, and 40 rows onto 8,192 columns 6.4 to 7.2 against 5.6.
+    if (again <= 64 << 10 && again * strips.x * strips.y <= 16 << 20) {
+        adapters_both_few_kernel<<<strips, 256, 0, c.stream>>>((const bf16_t*)c.x, c.ldx, (const bf16_t*)c.a, (const bf16_t*)c.b, c.scales, c.ids, c.io, c.width, c.rank, slices, c.n_adapters);
+        return;
+    }
     const int rg = items >= 4096 ? 4 : 1;
     const dim3 grid((ranks + rg - 1) / rg, c.n_rows);
 #define GI_FEW(RG) adapters_down_few_kernel<RG><<<grid, 256, 0, c.stream>>>((const bf16_t*)c.x, c.ldx, (const bf16_t*)c.a, c.ids, c.sums, c.width, ranks, c.n_adapters)
     if (rg == 1) GI_FEW(1);
     else GI_FEW(4);
 #undef GI_FEW
-    Slices slices = c.slices;
-    for (int s = 0; s < slices.n; ++s) slices.strip[s + 1] = slices.strip[s] + (slices.begin[s + 1] - slices.begin[s] + 256 * FEW_COLUMNS - 1) / (256 * FEW_COLUMNS);
-    adapters_up_few_kernel<<<dim3(slices.strip[slices.n], c.n_rows), 256, 0, c.stream>>>(c.sums, (const bf16_t*)c.b, c.scales, c.ids, c.io, c.rank, slices, c.n_adapters);
+    adapters_up_few_kernel<<<strips, 256, 0, c.stream>>>(c.sums, (const bf16_t*)c.b, c.scales, c.ids, c.io, c.rank, slices, c.n_adapters);
 }
 
 // In 32 bits a segment is always the same.  Otherwise there are as many as give every compute unit (of 256) a workgroup: the sums of every segment are written and read again, and with two workgroups a unit

@@ -2238,50 +2238,60 @@ def _adapter_scratch(x_code, w_code, n, width, rank, n_slices) -> int:
 def adapters_check(x, a, b, ids, out, scales, base, slices):
     """The columns of the packed projections, once `adapters_add` can take the operands; KernelError if not."""
     what = "adapters_add"
-    if not (x.dim() == 2 and a.dim() == 3 and b.dim() == 3 and out.dim() == 2):
+    xs, as_, bs, shape = x.shape, a.shape, b.shape, out.shape
+    if not (len(xs) == 2 and len(as_) == 3 and len(bs) == 3 and len(shape) == 2):
         raise KernelError(f"{what}: x [rows, width], a [adapters, ranks, width], b [adapters, columns, rank] and out [rows, columns] are needed")
-    (n, width), (n_adapters, columns, rank), shape = x.shape, b.shape, out.shape
-    slices = (columns,) if slices is None else tuple(slices)
-    if not (1 <= len(slices) <= ADAPTER_MAX_SLICES and min(slices) > 0 and sum(slices) == columns):
-        raise KernelError(f"{what}: slices {slices} are not 1 to {ADAPTER_MAX_SLICES} positive numbers that add up to the {columns} columns")
-    if not (a.shape == (n_adapters, len(slices) * rank, width) and shape == (n, columns) and (base is out or base.shape == shape)):
-        raise KernelError(f"{what}: x {tuple(x.shape)}, a {tuple(a.shape)}, b {tuple(b.shape)}, base {tuple(base.shape)} and out {tuple(out.shape)} do not fit ({len(slices)} projections)")
-    if not (width and rank and n_adapters):
-        raise KernelError(f"{what}: {n_adapters} adapters of rank {rank} beside a width of {width} have no entries")
+    (n, width), (n_adapters, columns, rank) = xs, bs
+    if slices is None:
+        slices = (columns,)
+    else:
+        slices = tuple(slices)
+        if not (1 <= len(slices) <= ADAPTER_MAX_SLICES and min(slices) > 0 and sum(slices) == columns):
+            raise KernelError(f"{what}: slices {slices} are not 1 to {ADAPTER_MAX_SLICES} positive numbers that add up to the {columns} columns")
+    if not (as_ == (n_adapters, len(slices) * rank, width) and shape == (n, columns) and (base is out or base.shape == shape)):
+        raise KernelError(f"{what}: x {tuple(xs)}, a {tuple(as_)}, b {tuple(bs)}, base {tuple(base.shape)} and out {tuple(shape)} do not fit ({len(slices)} projections)")
+    if not (width and rank and n_adapters and columns):
+        raise KernelError(f"{what}: {n_adapters} adapters of rank {rank} between a width of {width} and {columns} columns have no entries")
     if rank > ADAPTER_MAX_RANK:
         raise KernelError(f"{what}: rank {rank}, at most {ADAPTER_MAX_RANK} is taken")
-    if not (a.dtype == b.dtype and a.is_contiguous() and b.is_contiguous()):
+    dtype = a.dtype
+    if not (dtype == b.dtype and a.is_contiguous() and b.is_contiguous()):
         raise KernelError(f"{what}: a and b must be contiguous and of one dtype")
     if not (ids.dtype == torch.int32 and ids.shape == (n,) and ids.is_contiguous()):
         raise KernelError(f"{what}: ids must be a contiguous int32 [rows] tensor")
     if scales is not None and not (scales.dtype == torch.float32 and scales.shape == (n_adapters,) and scales.is_contiguous()):
         raise KernelError(f"{what}: scales must be a contiguous float32 [adapters] tensor")
-    for t, name in ((x, "x"), (a, "a"), (out, "out")) if base is out else ((x, "x"), (a, "a"), (base, "base"), (out, "out")):
-        if t.dtype not in _CODE:
+    if not (x.dtype in _CODE and dtype in _CODE and base.dtype in _CODE and out.dtype in _CODE):
+        for t, name in ((x, "x"), (a, "a"), (base, "base"), (out, "out")):
             _code(t, f"{what}: {name}")
-        if t is not a and not ((t.stride(1) == 1 or t.shape[1] == 1) and (n <= 1 or t.stride(0) >= t.shape[1])):
-            raise KernelError(f"{what}: {name} must have unit inner stride and rows that do not overlap")
+    if not (x.is_contiguous() and out.is_contiguous() and (base is out or base.is_contiguous())):
+        for t, name in ((x, "x"), (base, "base"), (out, "out")):
+            if not ((t.stride(1) == 1 or t.shape[1] == 1) and (n <= 1 or t.stride(0) >= t.shape[1])):
+                raise KernelError(f"{what}: {name} must have unit inner stride and rows that do not overlap")
     if n:
         _here(what, x, a, b, ids, out, scales, base)
     return slices
 
 
-def adapters_add(x, a, b, ids, out, scales=None, base=None, slices=None):
+def adapters_add(x, a, b, ids, out, scales=None, base=None, slices=None, checked=None):
     """out[t] = base[t] + scales[e] * (b[e] @ (a[e] @ x[t])) with e = ids[t], the low-rank adapter of row t's request; out[t] = base[t] where ids[t] is
     none of 0 .. adapters-1.  x float32 or bfloat16 [rows, width], a [adapters, rank, width] and b [adapters, columns, rank] of one dtype
     (either), contiguous; ids int32 [rows] in any order; scales float32 [adapters], None for 1; base float32 or bfloat16 [rows, columns], None: out itself (it may
     also be given as both, but otherwise out shares no memory with an operand); out likewise.  slices: the columns of the projections that out packs, in their order
     (at most ADAPTER_MAX_SLICES); a then holds a block of `rank` rows for each, [adapters, len(slices) * rank, width].  Adapters of smaller rank are filled up with zeros.
-    Sums are in 32 bits; a row's result does not depend on what the other rows hold, and with float32 x not on how many there are either."""
-    base = out if base is None else base
-    slices = adapters_check(x, a, b, ids, out, scales, base, slices)
+    Sums are in 32 bits; a row's result does not depend on what the other rows hold, and with float32 x not on how many there are either.
+    checked: what `adapters_check` gave for these operands, if it has been asked."""
+    if base is None:
+        base = out
+    slices = adapters_check(x, a, b, ids, out, scales, base, slices) if checked is None else checked
     (n, width), (n_adapters, columns, rank) = x.shape, b.shape
     if n == 0:
         return out
-    x_code, w_code = _CODE[x.dtype], _CODE[a.dtype]
-    scratch = torch.empty(_adapter_scratch(x_code, w_code, n, width, rank, len(slices)), dtype=torch.float32, device=x.device)
+    x_code, w_code, n_slices = _CODE[x.dtype], _CODE[a.dtype], len(slices)
+    scratch = torch.empty(_adapter_scratch(x_code, w_code, n, width, rank, n_slices), dtype=torch.float32, device=x.device)
+    base_row, out_row = base.stride(0), out.stride(0)
     _call("gi_adapters_add", x.data_ptr(), x_code, max(x.stride(0), width), a.data_ptr(), b.data_ptr(), w_code, ids.data_ptr(), _ptr(scales), base.data_ptr(), _CODE[base.dtype],
-          max(base.stride(0), columns), out.data_ptr(), _CODE[out.dtype], max(out.stride(0), columns), scratch.data_ptr(), n, width, columns, rank, len(slices), _adapter_slices(slices),
+          max(base_row, columns), out.data_ptr(), _CODE[out.dtype], max(out_row, columns), scratch.data_ptr(), n, width, columns, rank, n_slices, _adapter_slices(slices),
           n_adapters, _stream())
     return out
 

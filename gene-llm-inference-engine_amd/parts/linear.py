@@ -58,12 +58,12 @@ def _linear_adapted(a, weight, out, accumulate, gated, ctx, adapters):
         a = a.materialize()
     if accumulate and out.dtype != torch.float32:
         raise ops.KernelError("a product with adapters adds onto float32 rows only")
-    ops.adapters_check(a, adapters.down, adapters.up, adapters.ids, out, adapters.scales, out, adapters.slices)      # (before the shared product changes out)
+    slices = ops.adapters_check(a, adapters.down, adapters.up, adapters.ids, out, adapters.scales, out, adapters.slices)      # (before the shared product changes out)
     if out.dtype == torch.float32:
         shared = linear(a, weight, out, accumulate, ctx=ctx)
     else:                                           # in 32 bits until the adapters' share is in
         shared = linear(a, weight, torch.empty(out.shape, dtype=torch.float32, device=out.device), ctx=ctx)
-    return ops.adapters_add(a, adapters.down, adapters.up, adapters.ids, out, scales=adapters.scales, base=shared, slices=adapters.slices)
+    return ops.adapters_add(a, adapters.down, adapters.up, adapters.ids, out, adapters.scales, shared, checked=slices)
 
 
 def linear_xielu(a, weight: torch.Tensor, params: torch.Tensor, columns: int, dtype: torch.dtype, out: torch.Tensor = None, into: torch.Tensor = None):
