@@ -398,7 +398,7 @@ struct Rows {                               // base and out
     bool low_base, low_out, vectors;        // bfloat16; columns come in fours that may be loaded and stored at once
 };
 
-constexpr int PIECES = 3;                   // bfloat16 numbers that hold a 32-bit one: each the rounding of what the ones before leave, 8 bits of the 24 each
+constexpr int PIECES = 3;                   // bfloat16 numbers that hold a 32-bit one: each the first 8 bits of what the ones before leave of its 24, cut off, so that none passes the number
 
 // One run along the ranks of 16 columns of B.
 template <bool LOW> struct Run { uint4 v; };
@@ -521,9 +521,14 @@ __global__ __launch_bounds__(UP_NT) void adapters_up_kernel(const float* __restr
                 if constexpr (LOW) {
 #pragma unroll
                     for (int p = 0; p < PIECES; ++p) {
-                        const uint2 two = uint2{f32x2_to_bf16x2(v[q][0], v[q][1]), f32x2_to_bf16x2(v[q][2], v[q][3])};
-                        *reinterpret_cast<uint2*>(held + p * apart + r * pitch + k) = two;
-                        v[q] -= numbers4(uint4{two.x, two.y, 0u, 0u}, true);
+                        uint32_t top[4];
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) {
+                            top[c] = __float_as_uint(v[q][c]) & 0xffff0000u;
+                            const float left = v[q][c] - __uint_as_float(top[c]);
+                            v[q][c] = left == left ? left : 0.f;                       // (nothing is left of an infinity, or of no number)
+                        }
+                        *reinterpret_cast<uint2*>(held + p * apart + r * pitch + k) = uint2{top[0] >> 16 | top[1], top[2] >> 16 | top[3]};
                     }
                 } else {
                     *reinterpret_cast<floatx4*>(held + r * pitch + k) = v[q];
@@ -585,45 +590,31 @@ __global__ __launch_bounds__(UP_NT) void adapters_up_kernel(const float* __restr
 
 // ------------------------------------------------------------------ a few rows
 // Decoded rows, as a rule each with an adapter of its own: nothing is shared, the adapters' bytes bound it, and what counts is that all of them are asked for at once and few waits
-// follow one another.  Every row is taken alone, without tiles.  Down: a workgroup has a row and RG ranks, its threads share out the width.
-template <int RG>
+// follow one another.  Every row is taken alone, without tiles.  Down: a workgroup has a row and one rank, its threads share out the width.  (With four ranks, which share the row's numbers, 8 rows of
+// 4,096 onto 4,096, rank 32, take 6.2 us instead of 5.6, 128 rows 18.8 instead of 18.0; rows that share an adapter of 2 MB gain a tenth.)
 __global__ __launch_bounds__(256) void adapters_down_few_kernel(const bf16_t* __restrict__ x, long ldx, const bf16_t* __restrict__ a, const int* __restrict__ ids, float* __restrict__ sums,
                                                                 int width, int ranks, int n_adapters) {
-    __shared__ float red[4][RG];
-    const int row = blockIdx.y, first = blockIdx.x * RG, tid = threadIdx.x;
+    __shared__ float red[4];
+    const int row = blockIdx.y, tid = threadIdx.x;
     const int e = ids[row];
     if (e < 0 || e >= n_adapters) return;
     const bf16_t* xr = x + (size_t)row * ldx;
-    const bf16_t* ar[RG];
-#pragma unroll
-    for (int i = 0; i < RG; ++i) ar[i] = a + ((size_t)e * ranks + min(first + i, ranks - 1)) * width;
-    float sum[RG];
-#pragma unroll
-    for (int i = 0; i < RG; ++i) sum[i] = 0.f;
+    const bf16_t* ar = a + ((size_t)e * ranks + blockIdx.x) * width;
+    float sum = 0.f;
 #pragma unroll 2
     for (int k = 8 * tid; k < width; k += 2048) {
-        const uint4 xv = *reinterpret_cast<const uint4*>(xr + k);
-        uint4 av[RG];
+        const uint4 xv = *reinterpret_cast<const uint4*>(xr + k), av = *reinterpret_cast<const uint4*>(ar + k);
+        const uint32_t xw[4] = {xv.x, xv.y, xv.z, xv.w}, aw[4] = {av.x, av.y, av.z, av.w};
 #pragma unroll
-        for (int i = 0; i < RG; ++i) av[i] = *reinterpret_cast<const uint4*>(ar[i] + k);
-        const uint32_t xw[4] = {xv.x, xv.y, xv.z, xv.w};
-#pragma unroll
-        for (int i = 0; i < RG; ++i) {
-            const uint32_t aw[4] = {av[i].x, av[i].y, av[i].z, av[i].w};
-#pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                sum[i] = fmaf(__uint_as_float(xw[u] << 16), __uint_as_float(aw[u] << 16), sum[i]);
-                sum[i] = fmaf(__uint_as_float(xw[u] & 0xffff0000u), __uint_as_float(aw[u] & 0xffff0000u), sum[i]);
-            }
+        for (int u = 0; u < 4; ++u) {
+            sum = fmaf(__uint_as_float(xw[u] << 16), __uint_as_float(aw[u] << 16), sum);
+            sum = fmaf(__uint_as_float(xw[u] & 0xffff0000u), __uint_as_float(aw[u] & 0xffff0000u), sum);
         }
     }
-#pragma unroll
-    for (int i = 0; i < RG; ++i) {
-        sum[i] = wave_sum(sum[i]);
-        if ((tid & 63) == 0) red[tid >> 6][i] = sum[i];
-    }
+    sum = wave_sum(sum);
+    if ((tid & 63) == 0) red[tid >> 6] = sum;
     __syncthreads();
-    if (tid < RG && first + tid < ranks) sums[(size_t)row * ranks + first + tid] = (red[0][tid] + red[1][tid]) + (red[2][tid] + red[3][tid]);
+    if (tid == 0) sums[(size_t)row * ranks + blockIdx.x] = (red[0] + red[1]) + (red[2] + red[3]);
 }
 
 // Up: a thread has FEW_COLUMNS columns, 256 apart, of a row; the row's sums come as scalars.
@@ -846,14 +837,16 @@ int up(const Call& c) {
     return up_sized<LOW, W, false, 0>(c, slices, strip);
 }
 
-// bfloat16 rows that may be loaded 8 numbers at a time, few enough that loading an adapter once for every row that takes it costs less than tiles that share it.
+// bfloat16 rows that may be loaded 8 numbers at a time, few enough that loading an adapter once for every row that takes it costs less than tiles that share it.  Only the device knows which rows share:
+// with an adapter a row tiles lose by far (64 rows of 4,096 onto 4,096, rank 32: 10.7 us against 54; 256 rows 31 against 188), with one for all the two meet at some 160 MB loaded (256 such rows: 134 MB,
+// 13.4 us against 15.3; 128 rows of 8,192 onto 2,048, rank 64: 168 MB, 19.5 against 27.8; 256: 36 against 22; 256 rows of 4,096 onto 14,336, rank 16: 151 MB, 17.1 against 16.7).
 bool few_rows(const Call& c) {
-    return c.n_rows <= 64 && c.rank % 8 == 0 && c.width % 8 == 0 && c.ldx % 8 == 0 && aligned(c.x, 16) && aligned(c.a, 16) && aligned(c.b, 16);
+    const long loaded = 2l * c.n_rows * c.rank * ((long)c.slices.n * c.width + c.columns);
+    return c.n_rows <= 256 && loaded <= 160 << 20 && c.rank % 8 == 0 && c.width % 8 == 0 && c.ldx % 8 == 0 && aligned(c.x, 16) && aligned(c.a, 16) && aligned(c.b, 16);
 }
 
 void add_few(const Call& c) {
     const int ranks = c.rank * c.slices.n;
-    const long items = (long)c.n_rows * ranks;
     Slices slices = c.slices;
     for (int s = 0; s < slices.n; ++s) slices.strip[s + 1] = slices.strip[s] + (slices.begin[s + 1] - slices.begin[s] + 256 * FEW_COLUMNS - 1) / (256 * FEW_COLUMNS);
     const dim3 strips(slices.strip[slices.n], c.n_rows);
@@ -864,12 +857,7 @@ void add_few(const Call& c) {
         adapters_both_few_kernel<<<strips, 256, 0, c.stream>>>((const bf16_t*)c.x, c.ldx, (const bf16_t*)c.a, (const bf16_t*)c.b, c.scales, c.ids, c.io, c.width, c.rank, slices, c.n_adapters);
         return;
     }
-    const int rg = items >= 4096 ? 4 : 1;
-    const dim3 grid((ranks + rg - 1) / rg, c.n_rows);
-#define GI_FEW(RG) adapters_down_few_kernel<RG><<<grid, 256, 0, c.stream>>>((const bf16_t*)c.x, c.ldx, (const bf16_t*)c.a, c.ids, c.sums, c.width, ranks, c.n_adapters)
-    if (rg == 1) GI_FEW(1);
-    else GI_FEW(4);
-#undef GI_FEW
+    adapters_down_few_kernel<<<dim3(ranks, c.n_rows), 256, 0, c.stream>>>((const bf16_t*)c.x, c.ldx, (const bf16_t*)c.a, c.ids, c.sums, c.width, ranks, c.n_adapters);
     adapters_up_few_kernel<<<strips, 256, 0, c.stream>>>(c.sums, (const bf16_t*)c.b, c.scales, c.ids, c.io, c.rank, slices, c.n_adapters);
 }
 
