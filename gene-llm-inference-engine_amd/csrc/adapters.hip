@@ -838,11 +838,12 @@ int up(const Call& c) {
 }
 
 // bfloat16 rows that may be loaded 8 numbers at a time, few enough that loading an adapter once for every row that takes it costs less than tiles that share it.  Only the device knows which rows share:
-// with an adapter a row tiles lose by far (64 rows of 4,096 onto 4,096, rank 32: 10.7 us against 54; 256 rows 31 against 188), with one for all the two meet at some 160 MB loaded (256 such rows: 134 MB,
-// 13.4 us against 15.3; 128 rows of 8,192 onto 2,048, rank 64: 168 MB, 19.5 against 27.8; 256: 36 against 22; 256 rows of 4,096 onto 14,336, rank 16: 151 MB, 17.1 against 16.7).
+// with an adapter a row tiles lose by far (64 rows of 4,096 onto 4,096, rank 32: 10.7 us against 54; 256: 31 against 188; 512 of 2,048 onto 2,048, rank 16: 17.5 against 135), with one for all the two meet
+// at some 150 MB loaded (256 of 4,096 onto 4,096: 134 MB, 13.4 us against 15.3; 512 of 2,048 onto 2,048: 67 MB, 10.5 against 12.6; 512 onto 8,192: 168 MB, 18.7 against 15.3; 256 of 8,192 onto 2,048,
+// rank 64: 336 MB, 36 against 22) and at fewer where there are more rows (768 of 2,048 onto 2,048: 100 MB, 13.7 against 13.6; 1,024: 134 MB, 18.3 against 14.2).
 bool few_rows(const Call& c) {
     const long loaded = 2l * c.n_rows * c.rank * ((long)c.slices.n * c.width + c.columns);
-    return c.n_rows <= 256 && loaded <= 160 << 20 && c.rank % 8 == 0 && c.width % 8 == 0 && c.ldx % 8 == 0 && aligned(c.x, 16) && aligned(c.a, 16) && aligned(c.b, 16);
+    return c.n_rows <= 512 && loaded <= 160 << 20 && c.rank % 8 == 0 && c.width % 8 == 0 && c.ldx % 8 == 0 && aligned(c.x, 16) && aligned(c.a, 16) && aligned(c.b, 16);
 }
 
 void add_few(const Call& c) {

@@ -74,7 +74,8 @@ def run(c, result=F32, in_place=False):
 
 SIZES = [(1, 1, 1, 1, 1), (1, 8, 16, 8, 2), (1, 2048, 2048, 16, 3), (3, 65, 33, 5, 2), (7, 256, 129, 16, 8), (16, 512, 512, 32, 4), (17, 264, 200, 24, 5), (33, 520, 264, 1, 33), (64, 1024, 1000, 64, 70),
          (65, 1000, 72, 12, 3), (100, 2049, 130, 7, 9), (129, 640, 384, 128, 3), (250, 328, 520, 130, 4), (515, 4096, 256, 16, 6), (70, 72, 4104, 40, 2), (300, 31, 31, 31, 31),
-         (130, 96, 80, 256, 2), (20, 96, 80, 256, 2), (200, 100, 50, 225, 9), (1200, 1536, 1100, 48, 3)]
+         (130, 96, 80, 256, 2), (20, 96, 80, 256, 2), (200, 100, 50, 225, 9), (1200, 1536, 1100, 48, 3),
+         (600, 328, 520, 128, 4), (530, 96, 80, 256, 2), (520, 264, 200, 24, 5), (1025, 1000, 72, 40, 1100)]
 
 
 @pytest.mark.parametrize("n,width,columns,rank,adapters", SIZES)
@@ -85,7 +86,7 @@ def test_against_64_bits(n, width, columns, rank, adapters, dtypes):
         assert_right(run(c), c)
 
 
-@pytest.mark.parametrize("n", [1, 5, 64, 90, 300])
+@pytest.mark.parametrize("n", [1, 5, 64, 90, 300, 560])
 @pytest.mark.parametrize("base", [F32, BF16])
 @pytest.mark.parametrize("result", [F32, BF16])
 @pytest.mark.parametrize("dtype", [F32, BF16])
@@ -98,7 +99,7 @@ def test_dtypes_of_base_and_result_and_in_place(n, base, result, dtype):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
-@pytest.mark.parametrize("n", [1, 9, 200])
+@pytest.mark.parametrize("n", [1, 9, 200, 570])
 @pytest.mark.parametrize("slices,rank", [((256, 64, 64), 16), ((100, 29), 8), ((1, 500, 3, 8), 5), ((40, 40, 40, 40), 64)])
 def test_packed_projections(n, slices, rank, dtype):
     for scales in (True, False):
@@ -108,7 +109,7 @@ def test_packed_projections(n, slices, rank, dtype):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
-@pytest.mark.parametrize("n", [1, 70, 260])
+@pytest.mark.parametrize("n", [1, 70, 260, 515])
 def test_rows_without_an_adapter_are_the_base(n, dtype):
     c = make(n, 128, 200, 16, 4, dtype=dtype, ids=-1)
     c["x"][:] = float("nan")                                  # (nothing of theirs is read into a result)
@@ -123,7 +124,7 @@ def test_rows_without_an_adapter_are_the_base(n, dtype):
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_a_row_of_no_numbers_stays_its_own(dtype):
     """NaN and infinities of one request's rows, or of an adapter that others do not take, reach no other row."""
-    for n in (8, 96, 256, 400):
+    for n in (8, 96, 256, 600):
         c = make(n, 256, 144, 16, 4, dtype=dtype, ids="mixed")
         c["ids"][:4] = torch.tensor([0, 1, 2, 3], dtype=torch.int32)
         clean = run(c)
@@ -140,7 +141,7 @@ def test_a_row_of_no_numbers_stays_its_own(dtype):
         assert torch.equal(torch.cat([others[:, :5], others[:, 6:]], 1), torch.cat([clean[ids == 2][:, :5], clean[ids == 2][:, 6:]], 1))
 
 
-@pytest.mark.parametrize("n", [1, 20, 300])
+@pytest.mark.parametrize("n", [1, 20, 600])
 def test_sums_that_bfloat16_cannot_hold(n):
     """Sums A x at the end of 32 bits, beyond bfloat16's, stay the numbers that they are, and infinite ones infinite."""
     c = make(n, 64, 48, 8, 1, dtype=BF16, ids=0)
@@ -171,7 +172,7 @@ def test_a_32_bit_row_has_the_same_bits_in_every_batch(w_dtype, width, rank):
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_strides_and_places(dtype):
-    for n in (5, 150, 270):
+    for n in (5, 150, 530):
         c = make(n, 192, 96, 16, 3, dtype=dtype, ids="runs")
         wide = torch.full((n, 400), 9.0, dtype=dtype, device=DEV)
         for first in (0, 3, 8):                               # rows that begin at 16 bytes and that do not
@@ -192,7 +193,7 @@ def test_strides_and_places(dtype):
 
 
 def test_captured_and_replayed_with_other_requests():
-    for n in (6, 140, 300):
+    for n in (6, 140, 600):
         cs = [make(n, 512, 640, 16, 4, seed=s, ids="runs") for s in range(3)]
         held = {k: v.clone() if torch.is_tensor(v) else v for k, v in cs[0].items()}
         out = torch.empty_like(held["base"])
@@ -214,7 +215,7 @@ def test_captured_and_replayed_with_other_requests():
 
 
 def test_two_streams_at_once():
-    cs = [make(n, 1024, 512, 32, 3, seed=n, ids="runs") for n in (200, 400)]
+    cs = [make(n, 1024, 512, 32, 3, seed=n, ids="runs") for n in (200, 700)]
     want = [run(c) for c in cs]
     outs, streams = [torch.empty_like(c["base"]) for c in cs], [torch.cuda.Stream() for _ in cs]
     torch.cuda.synchronize()
@@ -239,7 +240,7 @@ def test_offsets_beyond_32_bits():
     many = 2 ** 31 // (16 * 8192) + 2
     a = torch.zeros((many, 16, 8192), dtype=BF16, device=DEV)
     b = torch.zeros((many, 40, 16), dtype=BF16, device=DEV)
-    for n in (3, 130, 500):
+    for n in (3, 130, 520):
         c = make(n, 8192, 40, 16, 3, ids="mixed")
         place = torch.tensor([0, many // 2, many - 1], device=DEV)
         a[place], b[place] = c["a"], c["b"]
@@ -252,7 +253,7 @@ def test_offsets_beyond_32_bits():
 
 @pytest.mark.parametrize("result", [F32, BF16])
 @pytest.mark.parametrize("dtype", [F32, BF16])
-@pytest.mark.parametrize("n", [1, 40, 300])
+@pytest.mark.parametrize("n", [1, 40, 300, 600])
 def test_beside_the_shared_projection(n, dtype, result):
     from geneinfer_amd.parts.linear import RowAdapters, linear
     c = make(n, 512, 384, 16, 5, dtype=dtype, ids="runs")
