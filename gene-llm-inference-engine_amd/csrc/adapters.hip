@@ -18,7 +18,8 @@ constexpr int MAX_SLICES = 4;
 constexpr int MAX_RANK = 256;
 constexpr int DOWN_WAVES = 2, DOWN_NT = 64 * DOWN_WAVES, UP_WAVES = 4, UP_NT = 64 * UP_WAVES;
 constexpr int SEGMENT = 256;                // of the width: the least that a workgroup of the way down takes
-constexpr int EXACT_SEGMENT = 256;          // what it always takes in 32 bits, where the order of a sum must not depend on the batch
+constexpr int EXACT_SEGMENT = 256;          // what it always takes in 32 bits, where the order of a sum must not depend on the batch (at 512 numbers 301 rows of 1,024 take 16.3 us instead of 13.0,
+                                            // 64 of 4,096 17.2 instead of 15.4, 2,048 of 4,096 28.9 instead of 31.3)
 constexpr int TILE = 64;                    // rows
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -228,7 +229,7 @@ __device__ __forceinline__ void store_sums(floatx4 (&sum)[4][MT], unsigned char*
 // Rows of one type, 16-byte loads.  Global memory goes straight into LDS (a lane's 16 bytes land behind the lane's before it), every wave through a ring of its own, so that no barrier stands in the loop: in registers the
 // operands' layout, neighbouring lanes in different rows, would take a load through the first-level cache in 64 pieces of 16 bytes instead of 16 whole sectors.  A stage is 64 rows of x and 16 MT of A,
 // 128 bytes each, its 16-byte chunk c of a row at place c ^ (row / 2 % 8), so that 16 rows' chunks lie in different banks.
-template <int MT> constexpr int stages_of() { return MT <= 2 ? 3 : 2; }
+constexpr int STAGES = 2;                   // (a third makes no difference of 1%: other workgroups of the unit load meanwhile)
 template <int MT> constexpr int stage_bytes() { return (TILE + 16 * MT) * 128; }
 
 template <bool LOW, int MT>
@@ -236,7 +237,7 @@ __global__ __launch_bounds__(DOWN_NT) void adapters_down_kernel(const typename P
                                                            float* __restrict__ sums, Down d) {
     typedef Piece<LOW> P;
     typedef typename P::T T;
-    constexpr int STAGES = stages_of<MT>(), BYTES = stage_bytes<MT>(), LOADS = BYTES / 1024, STEP = P::BLOCK * DOWN_WAVES;
+    constexpr int BYTES = stage_bytes<MT>(), LOADS = BYTES / 1024, STEP = P::BLOCK * DOWN_WAVES;
     extern __shared__ __align__(16) unsigned char ring[];
     __shared__ int before[COUNTS];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, at = lane & 15, group = lane >> 4;
@@ -426,7 +427,7 @@ __device__ __forceinline__ floatx4 times(const Held<false>& t, const Run<false>&
 // row of B: 64 accesses to the first-level cache a load); where the strip is no wider than 64 columns the waves share out the rows.  In the product D = M N the rows are M's and the columns
 // N's: number n of the four products of a step has columns 4 l + n, l = 0 .. 15, so that a lane ends with four neighbours and sixteen lanes with whole lines of base and out.  As on the way down no
 // row's values meet another's.  ALIGNED: runs of B, and fours of columns of base and out, may be loaded at once, and columns come in fours.  KS: runs of ranks that a wave keeps; 0 for any number,
-// loaded again for every 16 rows.  LOW_BASE, LOW_OUT: of aligned ones whether they are bfloat16 (a branch on it where they are loaded would have every load waited for); `io` says it of others.
+// loaded again for every 16 rows (8,192 rows of 14,336 columns, rank 16: 239 us kept, 272 loaded again).  LOW_BASE, LOW_OUT: of aligned ones whether they are bfloat16 (a branch on it where they are loaded would have every load waited for); `io` says it of others.
 template <bool LOW, typename W, bool ALIGNED, int KS, bool LOW_BASE, bool LOW_OUT>
 __global__ __launch_bounds__(UP_NT) void adapters_up_kernel(const float* __restrict__ sums, const W* __restrict__ b, const float* __restrict__ scales, const Tile* __restrict__ list,
                                                             const int* __restrict__ n_listed, Rows io, int n_rows, int rank, int n_segments, Slices slices, int strip_columns, int n_adapters) {
@@ -748,7 +749,7 @@ struct Call {
 // At most so many tiles: every 64th row begins one, and every row may.  Workgroups beyond the work there is leave at once, ones short of it come again.
 long most_tiles(int n_rows) { return n_rows; }
 // ... and about so many where the rows are a few requests'.
-long usual_tiles(int n_rows) { return (n_rows + TILE - 1) / TILE + 4; }
+long usual_tiles(int n_rows) { return (n_rows + TILE - 1) / TILE; }
 
 // Lets a kernel have `bytes` of LDS, asked for once per device.
 constexpr int MAX_DEVICES = 64;
@@ -764,7 +765,7 @@ int raise_lds(const void* kernel, int bytes, bool (&raised)[MAX_DEVICES]) {
 
 template <bool LOW, int MT>
 int down_sized(const Call& c, Down d) {
-    constexpr int lds = DOWN_WAVES * stages_of<MT>() * stage_bytes<MT>();
+    constexpr int lds = DOWN_WAVES * STAGES * stage_bytes<MT>();
     static_assert(lds >= DOWN_WAVES * 4 * MT * 1024, "the waves' sums meet in the ring");
     d.n_parts = d.n_segments * ((d.ranks + 16 * MT - 1) / (16 * MT));
     const long items = most_tiles(c.n_rows) * d.n_parts;
@@ -825,11 +826,13 @@ int up_sized(const Call& c, const Slices& slices, int strip) {
 
 template <bool LOW, typename W>
 int up(const Call& c) {
-    // A strip's workgroup first makes its rows' sums, so strips are as long as leaves every compute unit (of 256) two or three workgroups: aimed at 200, 350, 700 and 1,400 of them, 4,096 rows of 4,096 columns
-    // and rank 64 take 52, 52, 46 and 45 us, 2,048 rows of 2,048 columns and rank 32 12.3, 10.4, 10.4 and 14.6.
+    // A strip's workgroup first makes its rows' sums, so strips are as long as leaves every compute unit (of 256) two or three workgroups: aimed at 350 and 700 of them, 1,024 rows of 2,048 32-bit columns and
+    // rank 64 take 36.4 and 29.1 us both ways, 2,048 rows of 2,048 columns and rank 32 19.1 either way.  All four waves have columns of their own, 256 a step of the strip (strips of other multiples of 64:
+    // 531 rows 31.0 us instead of 26.5), or, where there are no 256 for each, rows of the same 64 (301 rows of 1,024 in 32 bits: 13.0 us instead of 14.5).  Strips end at 512 columns (8,192 rows of 14,336
+    // columns: 236 us at 256, 219 at 512, 239 at 1,024).
     const long even = usual_tiles(c.n_rows) * c.columns / 700;
     const int steps = (c.rank + Piece<LOW>::BLOCK / 2 - 1) / (Piece<LOW>::BLOCK / 2);
-    const int strip = even <= 64 ? 64 : (int)min((even + 255) / 256 * 256, 1024l);
+    const int strip = even <= 64 ? 64 : (int)min((even + 255) / 256 * 256, 512l);
     Slices slices = c.slices;
     for (int s = 0; s < slices.n; ++s) slices.strip[s + 1] = slices.strip[s] + (slices.begin[s + 1] - slices.begin[s] + strip - 1) / strip;
     if (c.io.vectors && c.rank % Piece<LOW>::RUN == 0 && aligned(c.b, Piece<LOW>::RUN * sizeof(W)))
