@@ -2245,7 +2245,7 @@ def adapters_check(x, a, b, ids, out, scales, base, slices):
     if slices is None:
         slices = (columns,)
     else:
-        slices = tuple(slices)
+        slices = tuple(map(int, slices))
         if not (1 <= len(slices) <= ADAPTER_MAX_SLICES and min(slices) > 0 and sum(slices) == columns):
             raise KernelError(f"{what}: slices {slices} are not 1 to {ADAPTER_MAX_SLICES} positive numbers that add up to the {columns} columns")
     if not (as_ == (n_adapters, len(slices) * rank, width) and shape == (n, columns) and (base is out or base.shape == shape)):
@@ -2268,6 +2268,8 @@ def adapters_check(x, a, b, ids, out, scales, base, slices):
         for t, name in ((x, "x"), (base, "base"), (out, "out")):
             if not ((t.stride(1) == 1 or t.shape[1] == 1) and (n <= 1 or t.stride(0) >= t.shape[1])):
                 raise KernelError(f"{what}: {name} must have unit inner stride and rows that do not overlap")
+    if base is not out and n and base.data_ptr() == out.data_ptr() and not (base.dtype == out.dtype and (n == 1 or base.stride(0) == out.stride(0))):
+        raise KernelError(f"{what}: base and out begin at the same place, but their rows or dtypes differ")
     if n:
         _here(what, x, a, b, ids, out, scales, base)
     return slices

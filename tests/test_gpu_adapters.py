@@ -251,6 +251,27 @@ def test_offsets_beyond_32_bits():
         assert_right(out, c)
 
 
+def test_the_most_rows_and_one_more():
+    n = 2 ** 20
+    for runs in ("mixed", "runs"):
+        c = make(n, 8, 8, 8, 5, ids=runs)
+        assert_right(run(c), c)
+    x, ids, out = torch.zeros((n + 1, 8), dtype=BF16, device=DEV), torch.zeros(n + 1, dtype=torch.int32, device=DEV), torch.zeros((n + 1, 8), device=DEV)
+    with pytest.raises(ops().KernelError, match="too many"):
+        ops().adapters_add(x, c["a"], c["b"], ids, out)
+
+
+def test_the_widest_rows():
+    for n in (2, 513):
+        c = make(n, 2 ** 16 + 8, 16, 8, 2, ids="mixed")
+        assert_right(run(c), c)
+    x, a, b = (torch.zeros(shape, dtype=BF16, device=DEV) for shape in ((1, 2 ** 24 + 8), (1, 8, 2 ** 24 + 8), (1, 8, 8)))
+    with pytest.raises(ops().KernelError, match="too many"):
+        ops().adapters_add(x, a, b, torch.zeros(1, dtype=torch.int32, device=DEV), torch.zeros((1, 8), device=DEV))
+    c = make(2, 2 ** 24, 8, 8, 1, ids=0)
+    assert_right(run(c), c)
+
+
 @pytest.mark.parametrize("result", [F32, BF16])
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("n", [1, 40, 300, 600])

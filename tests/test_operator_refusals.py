@@ -48,6 +48,14 @@ def test_adapters_refuse(change, message):
         ops.adapters_add(**{**adapter_args(), **change})
 
 
+def test_base_and_out_at_one_place_must_be_the_same():
+    args = adapter_args()
+    room = torch.zeros(5, 24)
+    for base, out in ((room.view(10, 12)[:5], room[:, :12]), (room.view(torch.bfloat16)[:, :12], room[:, :12])):
+        with pytest.raises(ops.KernelError, match="same place"):
+            ops.adapters_add(**{**args, "base": base, "out": out})
+
+
 def test_adapters_of_no_rows_change_nothing():
     args = adapter_args(n=0)
     assert ops.adapters_add(**args) is args["out"]
