@@ -11,7 +11,9 @@
 // comes out a token off.  So weights exp((l - max) / T) and all sums are held in 64 bits, which this chip computes at the rate of 32.
 //
 // Three launches.  All rows once, in runs of 4,096 logits: the runs' maxima and sums.  Then, per request and run, the verdict (every workgroup of a request comes to it by itself, from the runs' numbers) and,
-// where a draft fell, the run's share of what is drawn from.  Then a request's draw.
+// where a draft fell, the run's share of what is drawn from.  Then a request's draw.  What bounds them: of many rows the logits' bytes and, as much, the weights' instructions (64 requests, 401 rows of 128,256
+// tokens, 206 MB: 51 + 20 + 9 us); of a few the waits that follow one another (one request with 4 drafts, 9 such rows: 4.5 + 8.7 + 7.0 us).  A last workgroup that draws by itself instead of a third launch has
+// to see what the others wrote: with the fences for that one request takes 29.7 us instead of 20.5, 64 take 121 instead of 81.
 #include "common.h"
 
 namespace {
@@ -56,36 +58,37 @@ __device__ __forceinline__ int drafts_of(const Inputs& in, int r, long& first) {
 
 __device__ __forceinline__ float number(float v) { return v == v ? v : -INFINITY; }        // (what is no number is no token)
 
-// 2^m for m <= 0, 0 below 2^-1020 and for what is no number: with n the nearest integer (what is left in the low bits of a sum with 1.5 * 2^52) and |f| <= 1/2, 2^n (1 + f q(f)), q the polynomial
-// through (2^f - 1) / f at nine Chebyshev points of [-1/2, 1/2]; off by less than 4e-14 relative, less than a draw over a million tokens can notice.  No conversions and no scaling by an instruction of its
-// own: those run at a quarter of the rate.
+// Weights exp((l - top) / T) of a row whose largest logit is `top`: 1 for the largest, 0 for what is no token (-infinity, NaN) and below 2^-1020.  With m = (l - top) log2(e) / T, n the nearest integer (what is left in
+// the low bits of a sum with 1.5 * 2^52) and f = m - n, 2^m is 2^n (1 + f q(f)), q the polynomial through (2^f - 1) / f at eight Chebyshev points of [-1/2, 1/2]: off by 2e-12 relative, less than a draw over a
+// million tokens can notice.  No scaling by an instruction of its own: those, as conversions, run at a quarter of the rate, and instructions are what bounds a sum over many rows (four fifths of the cycles issue
+// one; a polynomial of nine points and a product of its own for m: 55 us for 401 rows of 128,256 tokens that now take 51).
 __device__ __forceinline__ double horner(double f, double q, double c) {        // f q + c, the coefficient in scalar registers: as the accumulator it would be moved there for every step
     double out;
     asm("v_fma_f64 %0, %1, %2, %3" : "=v"(out) : "v"(f), "v"(q), "s"(c));
     return out;
 }
-__device__ __forceinline__ double exp2_below(double m) {
-    const double shifted = m + 6755399441055744.0, n = shifted - 6755399441055744.0, f = m - n;
-    double q = 1.0203114674825208e-07;
-    q = horner(f, q, 1.3255227922924584e-06);
-    q = horner(f, q, 1.5252686963534207e-05);
-    q = horner(f, q, 0.00015403455840537416);
-    q = horner(f, q, 0.001333355817880503);
-    q = horner(f, q, 0.009618129159412746);
-    q = horner(f, q, 0.05550410866476055);
-    q = horner(f, q, 0.24022650695812997);
-    q = horner(f, q, 0.6931471805599455);
-    const long long w = __double_as_longlong(fma(f, q, 1.0)), at = __double_as_longlong(shifted);
-    const int high = (int)(w >> 32) + ((int)at << 20);
-    return m > -1020.0 ? __hiloint2double(high, (int)w) : 0.0;
-}
-
-// Weights exp((l - top) / T) of a row whose largest logit is `top`: 1 for the largest, 0 for what is no token (-infinity, NaN).
 struct Weigher {
-    double top, per;                        // log2(e) / T
+    double top, per, least;                 // log2(e) / T, never 0; logits so far below the largest weigh less than 2^-1020
     bool plain;                             // the largest is not infinite
-    __device__ Weigher(float largest, float t) : top((double)largest), per(1.4426950408889634 / (double)t), plain(largest < INFINITY) {}
-    __device__ double fast(float l) const { return exp2_below(((double)l - top) * per); }
+    __device__ Weigher(float largest, float t) : top((double)largest), per(fmax(1.4426950408889634 / (double)t, 1e-300)), least(fmax(-707.0 * (double)t, -1e303)), plain(largest < INFINITY) {}
+    __device__ double power(double below) const {                               // of a logit so far below the largest, not less than `least`
+        const double shifted = fma(below, per, 6755399441055744.0), f = fma(below, per, 6755399441055744.0 - shifted);
+        double q = 1.325080551750225e-06;
+        q = horner(f, q, 1.5303700711365693e-05);
+        q = horner(f, q, 0.00015403475186530786);
+        q = horner(f, q, 0.0013333478473685416);
+        q = horner(f, q, 0.00961812913523614);
+        q = horner(f, q, 0.055504109063258665);
+        q = horner(f, q, 0.24022650695888503);
+        q = horner(f, q, 0.6931471805568324);
+        const long long w = __double_as_longlong(fma(f, q, 1.0)), n = __double_as_longlong(shifted);
+        return __hiloint2double((int)(w >> 32) + ((int)n << 20), (int)w);
+    }
+    __device__ double fast(float l) const {
+        const double below = (double)l - top;
+        return below > least ? power(below) : 0.0;
+    }
+    __device__ double beside_1(float l) const { return power(fmax((double)l - top, least)); }      // to be added to 1 or more: 2^-1020 instead of 0, an instruction less
     __device__ double any(float l) const { return plain ? fast(l) : l == INFINITY ? 1.0 : 0.0; }
 };
 
@@ -132,7 +135,7 @@ struct RunOf {
 };
 
 // Largest logit (with its lowest index) and sum of exp((l - that) / T) of every run: workgroup (run, request, group of rows).  Of the rows that the request has, the target's 0 .. n and the drafter's 0 .. n - 1 behind
-// them, every gridDim.z-th is a workgroup's.
+// them, every gridDim.z-th is a workgroup's.  4.5 us for 9 rows of 128,256 tokens, 8.0 for 192 greedy ones of 32,003 (3.1 TB/s), 51 for 401 of 128,256 (4.0 TB/s; the loads alone take 40).
 __global__ __launch_bounds__(NT) void parts_kernel(Inputs in, float* __restrict__ part_m, int* __restrict__ part_i, double* __restrict__ part_s) {
     __shared__ float sv[2][4];
     __shared__ int si[2][4];
@@ -176,7 +179,7 @@ __global__ __launch_bounds__(NT) void parts_kernel(Inputs in, float* __restrict_
         double sum = 0.0;
         if (weigh.plain) {
 #pragma unroll
-            for (int j = 0; j < PER; ++j) sum += weigh.fast(v[j]);
+            for (int j = 0; j < PER; ++j) sum += weigh.beside_1(v[j]);
         } else {
             for (int k = run.begin + tid; k < run.end; k += NT) sum += weigh.any(row[k]);
         }
@@ -185,7 +188,7 @@ __global__ __launch_bounds__(NT) void parts_kernel(Inputs in, float* __restrict_
         barrier_lds();
         if (tid == 0) {
             part_m[at] = bv;
-            part_s[at] = ((red[turn][0] + red[turn][1]) + red[turn][2]) + red[turn][3];
+            part_s[at] = bv > -INFINITY ? ((red[turn][0] + red[turn][1]) + red[turn][2]) + red[turn][3] : 0.0;
         }
     }
 }
@@ -208,7 +211,8 @@ struct Drawn {
 };
 
 // Which drafts stay, and the sums over runs of what is drawn from, where the parts do not hold them already: every run of a request whose drafter's row is taken off, and the run that a draft is
-// left out of.  Workgroup (run, request); run 0's writes what the request has so far.
+// left out of.  Workgroup (run, request); run 0's writes what the request has so far.  8.7 us for one request with 4 drafts, 20 for 64 with up to 7, most of whose two rows of 128,256 are read again (17.7 MB of
+// them from memory, the rest is still in the last-level cache).
 __global__ __launch_bounds__(NT) void judge_kernel(Inputs in, const float* __restrict__ part_m, const int* __restrict__ part_i, const double* __restrict__ part_s, Verdict* __restrict__ verdicts,
                                                    double* __restrict__ rest, int* __restrict__ tokens, int* __restrict__ counts) {
     __shared__ float top[MAX_ROWS];
@@ -354,7 +358,7 @@ __device__ __forceinline__ double scan_f64(double v, int lane) {               /
 }
 
 // The draw: one workgroup a request.  The run is found among the runs' sums (by a prefix sum over a wave's lanes, which share the runs out, and a walk over one lane's), then the token in the run: a
-// thread owns four consecutive tokens, a prefix sum over the threads finds the thread, which walks its tokens.
+// thread owns four consecutive tokens, a prefix sum over the threads finds the thread, which walks its tokens.  7 us for one request, 9 for 64, all of it waits; with 256 threads, sixteen tokens each, 12 for one.
 constexpr int PICK_NT = 1024, PICK_WAVES = PICK_NT / 64, PICK_PER = CHUNK / PICK_NT;
 __global__ __launch_bounds__(PICK_NT) void pick_kernel(Inputs in, const Verdict* __restrict__ verdicts, const float* __restrict__ part_m, const double* __restrict__ part_s,
                                                        const double* __restrict__ rest, int* __restrict__ tokens) {
@@ -471,6 +475,8 @@ GI_API int gi_verify_drafts(const float* logits, int n_rows, long stride, const 
     float* part_m = (float*)(verdicts + n_requests);
     int* part_i = (int*)(part_m + rows * n_chunks);
     const int most = drafter != nullptr ? 2 * K + 1 : K + 1;
+    // A workgroup adds up several of a request's rows where there are more than 32 workgroups a compute unit without: their start costs as much as a short run.  Aimed at 8, 16, 32 and 200 of them, 64 requests with up to
+    // 15 rows of 128,256 tokens took 99, 89, 83 and 95 us in all; a few requests have a workgroup for every row and run either way.
     const int groups = (int)min((long)most, max(1l, 32 * (long)gi_compute_units() / ((long)n_chunks * n_requests)));
     parts_kernel<<<dim3(n_chunks, n_requests, groups), NT, 0, stream>>>(in, part_m, part_i, part_s);
     GI_CHECK_LAUNCH("verify_drafts (parts)");
