@@ -16,7 +16,7 @@ namespace {
 
 constexpr int MAX_SLICES = 4;
 constexpr int MAX_RANK = 256;
-constexpr int DOWN_WAVES = 2, DOWN_NT = 64 * DOWN_WAVES, UP_WAVES = 4, UP_NT = 64 * UP_WAVES;
+constexpr int ANY_WAVES = 4, UP_WAVES = 4, UP_NT = 64 * UP_WAVES;
 constexpr int SEGMENT = 256;                // of the width: the least that a workgroup of the way down takes
 constexpr int EXACT_SEGMENT = 256;          // what it always takes in 32 bits, where the order of a sum must not depend on the batch (at 512 numbers 301 rows of 1,024 take 16.3 us instead of 13.0,
                                             // 64 of 4,096 17.2 instead of 15.4, 2,048 of 4,096 28.9 instead of 31.3)
@@ -112,6 +112,7 @@ __device__ __forceinline__ void load_piece(Piece<false>& p, const T* __restrict_
 
 // The tiles of a batch, counted by every workgroup: a tile begins at every 64th row and where a row's adapter is not its neighbour's.
 constexpr int COUNTS = 1024;
+template <int WAVES>                        // of a workgroup
 struct Tiles {
     const int* ids;
     int n_rows, each, entries;              // rows; blocks of 64 rows that one count is of; counts
@@ -126,15 +127,15 @@ struct Tiles {
         each = (blocks + COUNTS - 1) / COUNTS;
         entries = (blocks + each - 1) / each;
         constexpr int AT_ONCE = 8;                                     // counts of a wave whose rows' numbers are asked for together
-        for (int c = wave; c < entries; c += AT_ONCE * DOWN_WAVES) {
+        for (int c = wave; c < entries; c += AT_ONCE * WAVES) {
             int sum[AT_ONCE] = {};
             for (int b = 0; b < each; ++b) {
 #pragma unroll
-                for (int u = 0; u < AT_ONCE; ++u) sum[u] += __popcll(begins((c + u * DOWN_WAVES) * each + b));       // (a block beyond the rows has none)
+                for (int u = 0; u < AT_ONCE; ++u) sum[u] += __popcll(begins((c + u * WAVES) * each + b));       // (a block beyond the rows has none)
             }
 #pragma unroll
             for (int u = 0; u < AT_ONCE; ++u)
-                if (lane == 0 && c + u * DOWN_WAVES < entries) before[c + u * DOWN_WAVES] = sum[u];
+                if (lane == 0 && c + u * WAVES < entries) before[c + u * WAVES] = sum[u];
         }
         __syncthreads();
         // every wave adds the counts up for itself and wave 0 lays the sums down
@@ -187,7 +188,7 @@ struct Tile {                               // of the list that the way down lea
 };
 
 // ------------------------------------------------------------------ down, in tiles
-// sums[segment][row][rank] of a tile, a segment of the width and a group of 16 MT ranks.  The two waves of a workgroup share out the segment, every second block of 128 bytes a row, so that none
+// sums[segment][row][rank] of a tile, a segment of the width and a group of 16 MT ranks.  A workgroup's waves share out the segment, every second block of 128 bytes a row, so that none
 // loads what the other does.  In the product D = M N the ranks are M's rows and the tile's rows N's columns: a lane of the result has values of one row only, and rows behind the tile's
 // last are loaded as that one and dropped.
 struct Down {
@@ -197,9 +198,9 @@ struct Down {
     long ldx;
 };
 
-template <int MT>
+template <int WAVES, int MT>
 __device__ __forceinline__ void store_sums(floatx4 (&sum)[4][MT], unsigned char* meet, float* __restrict__ sums, const Down& d, int segment, int first_row, int rows, int first_rank) {
-    // wave 0's and wave 1's, through `meet`: 8 KB * MT, which no wave reads as anything else any more
+    // the waves' meet in `meet`, 4 KB * MT of each, which no wave reads as anything else any more
     floatx4* at = (floatx4*)meet;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     __syncthreads();
@@ -209,11 +210,13 @@ __device__ __forceinline__ void store_sums(floatx4 (&sum)[4][MT], unsigned char*
         for (int i = 0; i < MT; ++i)
             if (16 * j < rows) at[(wave * 4 * MT + j * MT + i) * 64 + lane] = sum[j][i];
     __syncthreads();
-    for (int item = threadIdx.x; item < 4 * MT * 64; item += DOWN_NT) {
+    for (int item = threadIdx.x; item < 4 * MT * 64; item += 64 * WAVES) {
         const int l = item & 63, j = item / 64 / MT, i = item / 64 % MT;
         const int row = 16 * j + (l & 15), rank = first_rank + 16 * i + 4 * (l >> 4);
         if (row >= rows || rank >= d.ranks) continue;
-        const floatx4 s = at[item] + at[item + 4 * MT * 64];
+        floatx4 s = at[item];
+#pragma unroll
+        for (int w = 1; w < WAVES; ++w) s += at[item + w * 4 * MT * 64];
         float* to = sums + ((size_t)segment * d.n_rows + first_row + row) * d.ranks + rank;
         if ((d.ranks & 3) == 0) {
             *reinterpret_cast<floatx4*>(to) = s;
@@ -232,16 +235,16 @@ __device__ __forceinline__ void store_sums(floatx4 (&sum)[4][MT], unsigned char*
 constexpr int STAGES = 2;                   // (a third makes no difference of 1%: other workgroups of the unit load meanwhile)
 template <int MT> constexpr int stage_bytes() { return (TILE + 16 * MT) * 128; }
 
-template <bool LOW, int MT>
-__global__ __launch_bounds__(DOWN_NT) void adapters_down_kernel(const typename Piece<LOW>::T* __restrict__ x, const typename Piece<LOW>::T* __restrict__ a, const int* __restrict__ ids,
+template <bool LOW, int MT, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void adapters_down_kernel(const typename Piece<LOW>::T* __restrict__ x, const typename Piece<LOW>::T* __restrict__ a, const int* __restrict__ ids,
                                                            float* __restrict__ sums, Down d) {
     typedef Piece<LOW> P;
     typedef typename P::T T;
-    constexpr int BYTES = stage_bytes<MT>(), LOADS = BYTES / 1024, STEP = P::BLOCK * DOWN_WAVES;
+    constexpr int BYTES = stage_bytes<MT>(), LOADS = BYTES / 1024, STEP = P::BLOCK * WAVES;
     extern __shared__ __align__(16) unsigned char ring[];
     __shared__ int before[COUNTS];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, at = lane & 15, group = lane >> 4;
-    Tiles tiles{ids, d.n_rows, 0, 0};
+    Tiles<WAVES> tiles{ids, d.n_rows, 0, 0};
     const int n_tiles = tiles.count(before);
     const long n_items = (long)n_tiles * d.n_parts;
     unsigned char* mine = ring + wave * STAGES * BYTES;
@@ -257,7 +260,7 @@ __global__ __launch_bounds__(DOWN_NT) void adapters_down_kernel(const typename P
         if (e < 0 || e >= d.n_adapters) continue;
         const int segment = part % d.n_segments, first_rank = part / d.n_segments * 16 * MT;
         const int begin = segment * d.segment, end = min(d.width, begin + d.segment), k0 = begin + wave * P::BLOCK;
-        const int whole = max(0, (end - k0 + (DOWN_WAVES - 1) * P::BLOCK) / STEP);          // this wave's blocks
+        const int whole = max(0, (end - k0 + (WAVES - 1) * P::BLOCK) / STEP);          // this wave's blocks
         const T* ae = a + (size_t)e * d.ranks * d.width;
         const T* from[LOADS];
 #pragma unroll
@@ -320,19 +323,19 @@ __global__ __launch_bounds__(DOWN_NT) void adapters_down_kernel(const typename P
                 for (int i = 0; i < MT; ++i) sum[j][i] = times(ap[i], xp, sum[j][i]);
             }
         }
-        store_sums<MT>(sum, ring, sums, d, segment, first_row, rows, first_rank);
+        store_sums<WAVES, MT>(sum, ring, sums, d, segment, first_row, rows, first_rank);
     }
 }
 
 // Operands of two types, or rows that do not begin at 16 bytes: through registers, in the same order.
 template <bool LOW, typename X, typename W, bool ALIGNED>
-__global__ __launch_bounds__(DOWN_NT) void adapters_down_any_kernel(const X* __restrict__ x, const W* __restrict__ a, const int* __restrict__ ids, float* __restrict__ sums, Down d) {
+__global__ __launch_bounds__(64 * ANY_WAVES) void adapters_down_any_kernel(const X* __restrict__ x, const W* __restrict__ a, const int* __restrict__ ids, float* __restrict__ sums, Down d) {
     typedef Piece<LOW> P;
     constexpr int MT = 2;
-    __shared__ __align__(16) unsigned char meet[DOWN_WAVES * 4 * MT * 1024];
+    __shared__ __align__(16) unsigned char meet[ANY_WAVES * 4 * MT * 1024];
     __shared__ int before[COUNTS];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, at = lane & 15, group = lane >> 4;
-    Tiles tiles{ids, d.n_rows, 0, 0};
+    Tiles<ANY_WAVES> tiles{ids, d.n_rows, 0, 0};
     const int n_tiles = tiles.count(before);
     const long n_items = (long)n_tiles * d.n_parts;
     for (long item = blockIdx.x; item < n_items; item += gridDim.x) {
@@ -357,7 +360,7 @@ __global__ __launch_bounds__(DOWN_NT) void adapters_down_any_kernel(const X* __r
         for (int j = 0; j < 4; ++j)
 #pragma unroll
             for (int i = 0; i < MT; ++i) sum[j][i] = floatx4{0.f, 0.f, 0.f, 0.f};
-        for (int k = begin + wave * P::BLOCK; k < end; k += P::BLOCK * DOWN_WAVES) {
+        for (int k = begin + wave * P::BLOCK; k < end; k += P::BLOCK * ANY_WAVES) {
             P ap[MT];
 #pragma unroll
             for (int i = 0; i < MT; ++i) load_piece<ALIGNED>(ap[i], ar[i], k, end, group);
@@ -370,7 +373,7 @@ __global__ __launch_bounds__(DOWN_NT) void adapters_down_any_kernel(const X* __r
                 for (int i = 0; i < MT; ++i) sum[j][i] = times(ap[i], xp, sum[j][i]);
             }
         }
-        store_sums<MT>(sum, meet, sums, d, segment, first_row, rows, first_rank);
+        store_sums<ANY_WAVES, MT>(sum, meet, sums, d, segment, first_row, rows, first_rank);
     }
 }
 
@@ -763,18 +766,28 @@ int raise_lds(const void* kernel, int bytes, bool (&raised)[MAX_DEVICES]) {
     return 0;
 }
 
-template <bool LOW, int MT>
-int down_sized(const Call& c, Down d) {
-    constexpr int lds = DOWN_WAVES * STAGES * stage_bytes<MT>();
-    static_assert(lds >= DOWN_WAVES * 4 * MT * 1024, "the waves' sums meet in the ring");
+template <bool LOW, int MT, int WAVES>
+int down_launch(const Call& c, Down d) {
+    constexpr int lds = WAVES * STAGES * stage_bytes<MT>();
+    static_assert(lds >= WAVES * 4 * MT * 1024 && lds + 4 * COUNTS <= 163840, "the waves' sums meet in the ring");
     d.n_parts = d.n_segments * ((d.ranks + 16 * MT - 1) / (16 * MT));
     const long items = most_tiles(c.n_rows) * d.n_parts;
     const int grid = (int)min(items, (long)gi_compute_units() * (163840 / (lds + 4 * COUNTS)));
     typedef typename Piece<LOW>::T T;
     static bool raised[MAX_DEVICES] = {};
-    if (raise_lds((const void*)adapters_down_kernel<LOW, MT>, lds, raised) != 0) return -1;
-    adapters_down_kernel<LOW, MT><<<grid, DOWN_NT, lds, c.stream>>>((const T*)c.x, (const T*)c.a, c.ids, c.sums, d);
+    if (raise_lds((const void*)adapters_down_kernel<LOW, MT, WAVES>, lds, raised) != 0) return -1;
+    adapters_down_kernel<LOW, MT, WAVES><<<grid, 64 * WAVES, lds, c.stream>>>((const T*)c.x, (const T*)c.a, c.ids, c.sums, d);
     return 0;
+}
+
+// Four waves share a tile's segment, always in 32 bits, where the order of sums must not depend on the batch, or two.  Twice as many loads are under way with four, but of their workgroups a compute unit holds one
+// only: they gain where its tiles are whole (16,384 rows of 1,024, rank 16, both ways: 45.2 us instead of 50.9; 4,096 of 14,336, rank 64: 78.9 instead of 81.7; 301 of 1,024 in 32 bits 11.5 instead of 12.9) and lose
+// where requests of one row bring many tiles more (531 rows of 4,096, of them 19 alone, rank 3 * 24: 22.1 instead of 20.5).  Those are few beside the tiles of 2,048 rows.
+template <bool LOW, int MT>
+int down_sized(const Call& c, const Down& d) {
+    if constexpr (LOW)
+        if (c.n_rows < 2048) return down_launch<LOW, MT, 2>(c, d);
+    return down_launch<LOW, MT, 4>(c, d);
 }
 
 template <bool LOW, typename X, typename W>
@@ -792,11 +805,11 @@ int down(const Call& c) {
     const int grid = (int)min(most_tiles(c.n_rows) * d.n_parts, (long)gi_compute_units() * 8);
     if constexpr (!std::is_same<X, W>::value) {
         if (even) {
-            adapters_down_any_kernel<LOW, X, W, true><<<grid, DOWN_NT, 0, c.stream>>>((const X*)c.x, (const W*)c.a, c.ids, c.sums, d);
+            adapters_down_any_kernel<LOW, X, W, true><<<grid, 64 * ANY_WAVES, 0, c.stream>>>((const X*)c.x, (const W*)c.a, c.ids, c.sums, d);
             return 0;
         }
     }
-    adapters_down_any_kernel<LOW, X, W, false><<<grid, DOWN_NT, 0, c.stream>>>((const X*)c.x, (const W*)c.a, c.ids, c.sums, d);
+    adapters_down_any_kernel<LOW, X, W, false><<<grid, 64 * ANY_WAVES, 0, c.stream>>>((const X*)c.x, (const W*)c.a, c.ids, c.sums, d);
     return 0;
 }
 

@@ -211,8 +211,8 @@ struct Drawn {
 };
 
 // Which drafts stay, and the sums over runs of what is drawn from, where the parts do not hold them already: every run of a request whose drafter's row is taken off, and the run that a draft is
-// left out of.  Workgroup (run, request); run 0's writes what the request has so far.  8.7 us for one request with 4 drafts, 20 for 64 with up to 7, most of whose two rows of 128,256 are read again (17.7 MB of
-// them from memory, the rest is still in the last-level cache).
+// left out of.  Workgroup (run, request); run 0's writes what the request has so far.  8.7 us for one request with 4 drafts, 20 for 64 with up to 7, which read two rows of 128,256 again
+// each (58 MB), once the verdict says which: its waits (6 us) have nothing beside them.
 __global__ __launch_bounds__(NT) void judge_kernel(Inputs in, const float* __restrict__ part_m, const int* __restrict__ part_i, const double* __restrict__ part_s, Verdict* __restrict__ verdicts,
                                                    double* __restrict__ rest, int* __restrict__ tokens, int* __restrict__ counts) {
     __shared__ float top[MAX_ROWS];
