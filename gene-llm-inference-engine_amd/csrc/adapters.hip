@@ -231,7 +231,9 @@ __device__ __forceinline__ void store_sums(floatx4 (&sum)[4][MT], unsigned char*
 
 // Rows of one type, 16-byte loads.  Global memory goes straight into LDS (a lane's 16 bytes land behind the lane's before it), every wave through a ring of its own, so that no barrier stands in the loop: in registers the
 // operands' layout, neighbouring lanes in different rows, would take a load through the first-level cache in 64 pieces of 16 bytes instead of 16 whole sectors.  A stage is 64 rows of x and 16 MT of A,
-// 128 bytes each, its 16-byte chunk c of a row at place c ^ (row / 2 % 8), so that 16 rows' chunks lie in different banks.
+// 128 bytes each, its 16-byte chunk c of a row at place c ^ (row / 2 % 8), so that 16 rows' chunks lie in different banks (the counters show no conflict).
+// 4,096 rows of 14,336, rank 64: 38 us for 117 MB, 9 of them for counting tiles, the first loads and joining the waves' sums (without the products the time is the same); 2,048 of 2,048, rank 32, 7.0;
+// 531 of 4,096, rank 3 * 24, 10.0; 301 of 2,048 in 32 bits, rank 10, 6.8.
 constexpr int STAGES = 2;                   // (a third makes no difference of 1%: other workgroups of the unit load meanwhile)
 template <int MT> constexpr int stage_bytes() { return (TILE + 16 * MT) * 128; }
 
@@ -327,7 +329,8 @@ __global__ __launch_bounds__(64 * WAVES) void adapters_down_kernel(const typenam
     }
 }
 
-// Operands of two types, or rows that do not begin at 16 bytes: through registers, in the same order.
+// Operands of two types, or rows that do not begin at 16 bytes: through registers, in the same order.  2,048 rows of 4,096 onto 4,096, rank 16, both ways: two types 30 us, as both of 32 bits; rows at odd places
+// 63 (32 bits, 30 at even ones) and 78 (bfloat16, 25): every number is a load of its own.
 template <bool LOW, typename X, typename W, bool ALIGNED>
 __global__ __launch_bounds__(64 * ANY_WAVES) void adapters_down_any_kernel(const X* __restrict__ x, const W* __restrict__ a, const int* __restrict__ ids, float* __restrict__ sums, Down d) {
     typedef Piece<LOW> P;
@@ -431,6 +434,8 @@ __device__ __forceinline__ floatx4 times(const Held<false>& t, const Run<false>&
 // N's: number n of the four products of a step has columns 4 l + n, l = 0 .. 15, so that a lane ends with four neighbours and sixteen lanes with whole lines of base and out.  As on the way down no
 // row's values meet another's.  ALIGNED: runs of B, and fours of columns of base and out, may be loaded at once, and columns come in fours.  KS: runs of ranks that a wave keeps; 0 for any number,
 // loaded again for every 16 rows (8,192 rows of 14,336 columns, rank 16: 239 us kept, 272 loaded again).  LOW_BASE, LOW_OUT: of aligned ones whether they are bfloat16 (a branch on it where they are loaded would have every load waited for); `io` says it of others.
+// 4,096 rows of 4,096 32-bit columns, rank 64: 41 us for the 134 MB of base and out (a copy of as much takes 25); 531 of 6,144, rank 24, onto bfloat16 10.3; 2,048 of 2,048, rank 32, 9.4; 301 of 2,048 in 32 bits,
+// rank 10, 10.6.  Asking for a whole tile's base at once instead of 16 rows ahead makes it no faster: 4,096 rows of 4,096 both ways 50 us instead of 47, with 256 registers instead of 141.
 template <bool LOW, typename W, bool ALIGNED, int KS, bool LOW_BASE, bool LOW_OUT>
 __global__ __launch_bounds__(UP_NT) void adapters_up_kernel(const float* __restrict__ sums, const W* __restrict__ b, const float* __restrict__ scales, const Tile* __restrict__ list,
                                                             const int* __restrict__ n_listed, Rows io, int n_rows, int rank, int n_segments, Slices slices, int strip_columns, int n_adapters) {
@@ -595,7 +600,7 @@ __global__ __launch_bounds__(UP_NT) void adapters_up_kernel(const float* __restr
 // ------------------------------------------------------------------ a few rows
 // Decoded rows, as a rule each with an adapter of its own: nothing is shared, the adapters' bytes bound it, and what counts is that all of them are asked for at once and few waits
 // follow one another.  Every row is taken alone, without tiles.  Down: a workgroup has a row and one rank, its threads share out the width.  (With four ranks, which share the row's numbers, 8 rows of
-// 4,096 onto 4,096, rank 32, take 6.2 us instead of 5.6, 128 rows 18.8 instead of 18.0; rows that share an adapter of 2 MB gain a tenth.)
+// 4,096 onto 4,096, rank 32, take 6.2 us instead of 5.6, 128 rows 18.8 instead of 18.0; rows that share an adapter of 2 MB gain a tenth.)  64 rows of 4,096, rank 16: 4.1 us.
 __global__ __launch_bounds__(256) void adapters_down_few_kernel(const bf16_t* __restrict__ x, long ldx, const bf16_t* __restrict__ a, const int* __restrict__ ids, float* __restrict__ sums,
                                                                 int width, int ranks, int n_adapters) {
     __shared__ float red[4];
@@ -621,7 +626,7 @@ __global__ __launch_bounds__(256) void adapters_down_few_kernel(const bf16_t* __
     if (tid == 0) sums[(size_t)row * ranks + blockIdx.x] = (red[0] + red[1]) + (red[2] + red[3]);
 }
 
-// Up: a thread has FEW_COLUMNS columns, 256 apart, of a row; the row's sums come as scalars.
+// Up: a thread has FEW_COLUMNS columns, 256 apart, of a row; the row's sums come as scalars.  64 rows of 14,336, rank 16: 8.1 us for 37 MB (4.5 TB/s).
 constexpr int FEW_COLUMNS = 2;
 __global__ __launch_bounds__(256) void adapters_up_few_kernel(const float* __restrict__ sums, const bf16_t* __restrict__ b, const float* __restrict__ scales, const int* __restrict__ ids,
                                                               Rows io, int rank, Slices slices, int n_adapters) {
@@ -668,7 +673,8 @@ __global__ __launch_bounds__(256) void adapters_up_few_kernel(const float* __res
 
 bool aligned(const void* p, int bytes) { return (size_t)p % bytes == 0; }
 
-// Both ways in one launch, where making a row's sums anew for every strip of its columns costs less than a second launch: a wave makes every fourth sum, then a thread has its columns as above.
+// Both ways in one launch, where making a row's sums anew for every strip of its columns costs less than a second launch: a wave makes every fourth sum, then a thread has its columns as above.  One
+// row of 2,048 onto 2,048, rank 16: 4.6 us, the waits of three loads that follow one another.
 __global__ __launch_bounds__(256) void adapters_both_few_kernel(const bf16_t* __restrict__ x, long ldx, const bf16_t* __restrict__ a, const bf16_t* __restrict__ b, const float* __restrict__ scales,
                                                                 const int* __restrict__ ids, Rows io, int width, int rank, Slices slices, int n_adapters) {
     __shared__ float t[MAX_RANK];
