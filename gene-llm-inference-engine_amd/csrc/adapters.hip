@@ -885,7 +885,7 @@ void add_few(const Call& c) {
 }
 
 // In 32 bits a segment is always the same.  Otherwise there are as many as give every compute unit (of 256) a workgroup: the sums of every segment are written and read again, and with two workgroups a unit
-// the way down gains less than the way up loses (4,096 rows of 14,336, rank 64: 39 + 46 us with seven segments, 41 + 42 with three; 531 rows of 4,096, rank 3 * 24: 12.0 + 12.7, 10.0 + 10.3).
+// the way down gains less than the way up loses (4,096 rows of 14,336, rank 64, both ways: 84 us aimed at 500 workgroups, 79 at 250, 114 at 125; 531 rows of 4,096, rank 3 * 24: 24.7 at 500, 20.3 at 250).
 int segment_of(int n_rows, int width, int ranks, bool low) {
     if (!low) return EXACT_SEGMENT;
     const long segments = max(250 / (usual_tiles(n_rows) * ((ranks + 63) / 64)), 1l);
