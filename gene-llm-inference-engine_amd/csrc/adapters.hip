@@ -18,8 +18,7 @@ constexpr int MAX_SLICES = 4;
 constexpr int MAX_RANK = 256;
 constexpr int ANY_WAVES = 4, UP_WAVES = 4, UP_NT = 64 * UP_WAVES;
 constexpr int SEGMENT = 256;                // of the width: the least that a workgroup of the way down takes
-constexpr int EXACT_SEGMENT = 256;          // what it always takes in 32 bits, where the order of a sum must not depend on the batch (at 512 numbers 301 rows of 1,024 take 16.3 us instead of 13.0,
-                                            // 64 of 4,096 17.2 instead of 15.4, 2,048 of 4,096 28.9 instead of 31.3)
+constexpr int EXACT_SEGMENTS = 12;          // in 32 bits, where the order of a sum must not depend on the batch, as many of the width at most, whatever the number of rows
 constexpr int TILE = 64;                    // rows
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -884,10 +883,11 @@ void add_few(const Call& c) {
     adapters_up_few_kernel<<<strips, 256, 0, c.stream>>>(c.sums, (const bf16_t*)c.b, c.scales, c.ids, c.io, c.rank, slices, c.n_adapters);
 }
 
-// In 32 bits a segment is always the same.  Otherwise there are as many as give every compute unit (of 256) a workgroup: the sums of every segment are written and read again, and with two workgroups a unit
+// In 32 bits only the width says how long a segment is: few rows want many (64 of 14,336 onto 4,096, rank 16: 18.8, 20.0 and 22.8 us with 16, 12 and 8 at most, 21.8 always at 256 numbers), many rows few
+// (2,048 of 4,096: 30.3, 26.3, 26.4 and 30.4 us; 4,096 of 14,336, rank 64: 180, 169, 155 and 246).  Otherwise there are as many as give every compute unit (of 256) a workgroup: the sums of every segment are written and read again, and with two workgroups a unit
 // the way down gains less than the way up loses (4,096 rows of 14,336, rank 64, both ways: 84 us aimed at 500 workgroups, 79 at 250, 114 at 125; 531 rows of 4,096, rank 3 * 24: 24.7 at 500, 20.3 at 250).
 int segment_of(int n_rows, int width, int ranks, bool low) {
-    if (!low) return EXACT_SEGMENT;
+    if (!low) return (width + EXACT_SEGMENTS * SEGMENT - 1) / (EXACT_SEGMENTS * SEGMENT) * SEGMENT;
     const long segments = max(250 / (usual_tiles(n_rows) * ((ranks + 63) / 64)), 1l);
     return (int)(((width + segments - 1) / segments + SEGMENT - 1) / SEGMENT * SEGMENT);
 }
