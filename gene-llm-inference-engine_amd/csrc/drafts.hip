@@ -218,18 +218,20 @@ __global__ __launch_bounds__(NT) void judge_kernel(Inputs in, const float* __res
     __shared__ float top[MAX_ROWS];
     __shared__ int arg[MAX_ROWS];
     __shared__ double whole[MAX_ROWS];
+    __shared__ int drafted[MAX_DRAFTS];
     __shared__ int stays;                                   // drafts before the first that falls
     __shared__ double red[4];
     const int r = blockIdx.y, tid = threadIdx.x, K = in.K, member = tid & 15;
+    int x = -1;                                             // this thread's draft, its logits, its number
+    float target_x = -INFINITY, drafter_x = -INFINITY, u = 0.f;
+    if (tid < K) x = in.drafts[(size_t)r * K + tid];        // (asked for before it is known whether the request brings it: the waits for both are one)
     long first;
     const int n = drafts_of(in, r, first);
     const float t = in.temperature[r];
     const bool greedy = arg_max_asked(t);
     if (greedy && blockIdx.x != 0) return;
-    int x = -1;                                             // this thread's draft, its logits, its number
-    float target_x = -INFINITY, drafter_x = -INFINITY, u = 0.f;
+    if (tid < K) drafted[tid] = x;
     if (tid < n) {
-        x = in.drafts[(size_t)r * K + tid];
         if (x < 0 || x >= in.vocab) x = -1;
         if (x >= 0 && !greedy) {
             target_x = in.logits[(first + tid) * in.stride + x];
@@ -307,7 +309,7 @@ __global__ __launch_bounds__(NT) void judge_kernel(Inputs in, const float* __res
         v.sum_p = whole[kept];
         v.kind = PLAIN;
         if (kept < n) {
-            v.x = in.drafts[(size_t)r * K + kept];
+            v.x = drafted[kept];
             if (in.drafter != nullptr) {
                 v.kind = LESS_ROW;
                 v.top_q = top[K + 1 + kept];
@@ -318,7 +320,7 @@ __global__ __launch_bounds__(NT) void judge_kernel(Inputs in, const float* __res
         }
     }
     if (blockIdx.x == 0) {
-        if (tid <= K) tokens[(size_t)r * (K + 1) + tid] = tid < kept ? in.drafts[(size_t)r * K + tid] : greedy && n >= 0 && tid == kept ? arg[kept] : -1;
+        if (tid <= K) tokens[(size_t)r * (K + 1) + tid] = tid < kept ? drafted[tid] : greedy && n >= 0 && tid == kept ? arg[kept] : -1;
         if (tid == 0) {
             counts[r] = n < 0 ? 0 : kept + 1;
             verdicts[r] = v;
@@ -367,6 +369,9 @@ __global__ __launch_bounds__(PICK_NT) void pick_kernel(Inputs in, const Verdict*
     __shared__ double target, before_run;
     __shared__ int the_run, winner, last_one;
     const int r = blockIdx.x, tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+    // (asked for beside the verdict; a run whose share the verdict did not need has none there, and it is not looked at)
+    const double left = tid < in.n_chunks ? rest[(size_t)r * in.n_chunks + tid] : 0.0;
+    const float u = in.uniform[(size_t)r * (in.K + 1) + in.K];
     Verdict v = verdicts[r];
     if (v.kind == DONE) return;
     long first;
@@ -378,7 +383,7 @@ __global__ __launch_bounds__(PICK_NT) void pick_kernel(Inputs in, const Verdict*
     for (int attempt = 0; attempt < 2; ++attempt) {
         if (tid < in.n_chunks) {                           // (MAX_CHUNKS threads)
             const bool own = v.kind == LESS_ROW || (v.kind == LESS_TOKEN && v.x / CHUNK == tid);
-            sums[tid] = own ? rest[(size_t)r * in.n_chunks + tid] : part_s[parts + tid] * Weigher(v.top_p, t).any(part_m[parts + tid]);
+            sums[tid] = own ? left : part_s[parts + tid] * Weigher(v.top_p, t).any(part_m[parts + tid]);
         }
         __syncthreads();
         if (wave == 0) {
@@ -386,7 +391,7 @@ __global__ __launch_bounds__(PICK_NT) void pick_kernel(Inputs in, const Verdict*
             double mine = 0.0;
             for (int c = from; c < to; ++c) mine += sums[c];
             const double upto = scan_f64(mine, lane), below = __shfl_up(upto, 1, 64), total = __shfl(upto, 63, 64);
-            const double goal = (double)in.uniform[(size_t)r * (in.K + 1) + in.K] * total;
+            const double goal = (double)u * total;
             const unsigned long long beyond = __ballot(goal < upto && mine > 0.0), some = __ballot(mine > 0.0);
             // the first lane whose runs end beyond the goal; by rounding, or for u = 1, the last that weighs anything
             // (what rounding leaves of p beside an equal q is nothing: as much as that is a chance that no draft has to fall by)
