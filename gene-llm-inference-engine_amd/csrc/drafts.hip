@@ -92,11 +92,32 @@ struct Weigher {
     __device__ double any(float l) const { return plain ? fast(l) : l == INFINITY ? 1.0 : 0.0; }
 };
 
-__device__ __forceinline__ double wave_sum_f64(double v) {
+// Sums and the like over lanes without a trip through LDS (the shuffles' way): what a reduction takes is the wait for its steps.  Every lane of the wave, or of its sixteen, ends with the same value.
+template <typename T> struct Words { int w[sizeof(T) / 4]; };
+template <int BY, typename T, typename Op>
+__device__ __forceinline__ T with_lane(T v, Op op) {               // v of lane l and of lane l ^ BY, or for less than 16, where v is the same every 2 BY lanes of sixteen, of the one BY before
+    Words<T> a = __builtin_bit_cast(Words<T>, v), b;
 #pragma unroll
-    for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
-    return v;
+    for (int i = 0; i < (int)sizeof(T) / 4; ++i) {
+        if constexpr (BY == 32) {                                   // halves swapped between two copies: the lower ones in both halves of one, the upper ones in the other
+            const auto both = __builtin_amdgcn_permlane32_swap(a.w[i], a.w[i], false, false);
+            a.w[i] = both[0];
+            b.w[i] = both[1];
+        } else if constexpr (BY == 16) {
+            const auto both = __builtin_amdgcn_permlane16_swap(a.w[i], a.w[i], false, false);
+            a.w[i] = both[0];
+            b.w[i] = both[1];
+        } else {
+            b.w[i] = __builtin_amdgcn_update_dpp(0, a.w[i], 0x120 + BY, 0xf, 0xf, false);        // (rotated within sixteen)
+        }
+    }
+    return op(__builtin_bit_cast(T, a), __builtin_bit_cast(T, b));
 }
+template <typename T, typename Op> __device__ __forceinline__ T over_16(T v, Op op) { return with_lane<1>(with_lane<2>(with_lane<4>(with_lane<8>(v, op), op), op), op); }
+template <typename T, typename Op> __device__ __forceinline__ T over_wave(T v, Op op) { return over_16(with_lane<16>(with_lane<32>(v, op), op), op); }
+struct Sum { __device__ double operator()(double a, double b) const { return a + b; } };
+struct Largest { __device__ float operator()(float a, float b) const { return fmaxf(a, b); } };
+struct Least { __device__ int operator()(int a, int b) const { return min(a, b); } };
 
 // A thread's logits of a run: `v[4 u + c]` is number begin + 4 (tid + NT u) + c where four may be loaded at once, number begin + tid + NT (4 u + c) otherwise; -infinity behind `end`.
 struct RunOf {
@@ -155,7 +176,7 @@ __global__ __launch_bounds__(NT) void parts_kernel(Inputs in, float* __restrict_
         float bv = -INFINITY;
 #pragma unroll
         for (int j = 0; j < PER; ++j) bv = fmaxf(bv, v[j]);            // (NaN is passed over)
-        bv = wave_max(bv);
+        bv = over_wave(bv, Largest());
         if (lane == 0) sv[turn][wave] = bv;
         barrier_lds();
         bv = fmaxf(fmaxf(sv[turn][0], sv[turn][1]), fmaxf(sv[turn][2], sv[turn][3]));
@@ -165,8 +186,7 @@ __global__ __launch_bounds__(NT) void parts_kernel(Inputs in, float* __restrict_
 #pragma unroll
             for (int j = PER - 1; j >= 0; --j) mine = number(v[j]) == bv ? j : mine;
             int bi = mine < PER && run.at(mine) < run.end ? run.at(mine) : 0x7fffffff;       // (a thread's numbers ascend)
-#pragma unroll
-            for (int off = 32; off > 0; off >>= 1) bi = min(bi, __shfl_xor(bi, off, 64));
+            bi = over_wave(bi, Least());
             if (lane == 0) si[turn][wave] = bi;
             barrier_lds();
             if (tid == 0) {
@@ -183,7 +203,7 @@ __global__ __launch_bounds__(NT) void parts_kernel(Inputs in, float* __restrict_
         } else {
             for (int k = run.begin + tid; k < run.end; k += NT) sum += weigh.any(row[k]);
         }
-        sum = wave_sum_f64(sum);
+        sum = over_wave(sum, Sum());
         if (lane == 0) red[turn][wave] = sum;
         barrier_lds();
         if (tid == 0) {
@@ -259,9 +279,7 @@ __global__ __launch_bounds__(NT) void judge_kernel(Inputs in, const float* __res
                     else s[j] = part_s[at + c];
                 }
             }
-            float bv = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
-#pragma unroll
-            for (int off = 8; off > 0; off >>= 1) bv = fmaxf(bv, __shfl_xor(bv, off, 64));
+            const float bv = over_16(fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])), Largest());
             const float now = fmaxf(largest, bv);
             if (greedy) {
                 if (now > largest) place = 0x7fffffff;      // (a place of an earlier run that holds as much is lower)
@@ -273,14 +291,11 @@ __global__ __launch_bounds__(NT) void judge_kernel(Inputs in, const float* __res
                 double more = 0.0;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) more += s[j] * weigh.any(m[j]);
-#pragma unroll
-                for (int off = 8; off > 0; off >>= 1) more += __shfl_xor(more, off, 64);
-                sum = sum * weigh.any(largest) + more;
+                sum = sum * weigh.any(largest) + over_16(more, Sum());
             }
             largest = now;
         }
-#pragma unroll
-        for (int off = 8; off > 0; off >>= 1) place = min(place, __shfl_xor(place, off, 64));
+        place = over_16(place, Least());
         if (member == 0) { top[z] = largest; arg[z] = place; whole[z] = sum; }
     }
     __syncthreads();
@@ -344,19 +359,34 @@ __global__ __launch_bounds__(NT) void judge_kernel(Inputs in, const float* __res
     } else {
         for (int i = run.begin + tid; i < run.end; i += NT) sum += drawn.any(row[i], drafter[i], i);
     }
-    sum = wave_sum_f64(sum);
+    sum = over_wave(sum, Sum());
     if ((tid & 63) == 0) red[tid >> 6] = sum;
     __syncthreads();
     if (tid == 0) rest[(size_t)r * in.n_chunks + blockIdx.x] = ((red[0] + red[1]) + red[2]) + red[3];
 }
 
-__device__ __forceinline__ double scan_f64(double v, int lane) {               // inclusive, over a wave
+// The sum of a wave's lanes up to each: within sixteen by lanes 1, 2, 4 and 8 before (0 where there are none), then the sixteen before, then the 32 before.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double before(double v) {
+    Words<double> a = __builtin_bit_cast(Words<double>, v);
 #pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-        const double below = __shfl_up(v, off, 64);
-        if (lane >= off) v += below;
-    }
-    return v;
+    for (int i = 0; i < 2; ++i) a.w[i] = __builtin_amdgcn_update_dpp(0, a.w[i], CTRL, ROWS, 0xf, false);
+    return __builtin_bit_cast(double, a);
+}
+__device__ __forceinline__ double scan_f64(double v) {
+    v += before<0x111, 0xf>(v);
+    v += before<0x112, 0xf>(v);
+    v += before<0x114, 0xf>(v);
+    v += before<0x118, 0xf>(v);
+    v += before<0x142, 0xa>(v);                             // (the last of the sixteen before, in the second and the fourth)
+    return v + before<0x143, 0xc>(v);                       // (the last of the first half, in the second)
+}
+
+__device__ __forceinline__ double last_lane(double v) {
+    Words<double> a = __builtin_bit_cast(Words<double>, v);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) a.w[i] = __builtin_amdgcn_readlane(a.w[i], 63);
+    return __builtin_bit_cast(double, a);
 }
 
 // The draw: one workgroup a request.  The run is found among the runs' sums (by a prefix sum over a wave's lanes, which share the runs out, and a walk over one lane's), then the token in the run: a
@@ -390,19 +420,19 @@ __global__ __launch_bounds__(PICK_NT) void pick_kernel(Inputs in, const Verdict*
             const int each = (in.n_chunks + 63) / 64, from = lane * each, to = min(in.n_chunks, from + each);
             double mine = 0.0;
             for (int c = from; c < to; ++c) mine += sums[c];
-            const double upto = scan_f64(mine, lane), below = __shfl_up(upto, 1, 64), total = __shfl(upto, 63, 64);
+            const double upto = scan_f64(mine), below = before<0x138, 0xf>(upto), total = last_lane(upto);       // (the lane before's, 0 for the first)
             const double goal = (double)u * total;
             const unsigned long long beyond = __ballot(goal < upto && mine > 0.0), some = __ballot(mine > 0.0);
             // the first lane whose runs end beyond the goal; by rounding, or for u = 1, the last that weighs anything
             // (what rounding leaves of p beside an equal q is nothing: as much as that is a chance that no draft has to fall by)
             const int owner = v.kind == LESS_ROW && total <= NOTHING_LEFT ? -1 : beyond != 0 ? __ffsll((long long)beyond) - 1 : some != 0 ? 63 - __clzll((long long)some) : -1;
             if (lane == owner) {
-                double before = lane ? below : 0.0, before_last = before;
+                double walked = below, before_last = walked;
                 int run = -1, last = -1;
                 for (int c = from; c < to && run < 0; ++c) {
-                    if (sums[c] > 0.0) { last = c; before_last = before; }
-                    if (goal < before + sums[c]) run = c;
-                    before += sums[c];
+                    if (sums[c] > 0.0) { last = c; before_last = walked; }
+                    if (goal < walked + sums[c]) run = c;
+                    walked += sums[c];
                 }
                 the_run = run >= 0 ? run : last;
                 before_run = before_last;                  // (a run that holds the goal weighs something: the last seen)
@@ -434,12 +464,12 @@ __global__ __launch_bounds__(PICK_NT) void pick_kernel(Inputs in, const Verdict*
         mine += w[j];
         if (w[j] > 0.0) last = lo + j;
     }
-    const double upto = scan_f64(mine, lane), below = __shfl_up(upto, 1, 64);
+    const double upto = scan_f64(mine), below = before<0x138, 0xf>(upto);
     if (lane == 63) wave_total[wave] = upto;
     __syncthreads();
     double walk = before_run;
     for (int k = 0; k < wave; ++k) walk += wave_total[k];
-    if (lane) walk += below;
+    walk += below;
     int hit = 0x7fffffff;
 #pragma unroll
     for (int j = 0; j < PICK_PER; ++j) {
