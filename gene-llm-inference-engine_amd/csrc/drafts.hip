@@ -67,10 +67,14 @@ __device__ __forceinline__ double horner(double f, double q, double c) {        
     asm("v_fma_f64 %0, %1, %2, %3" : "=v"(out) : "v"(f), "v"(q), "s"(c));
     return out;
 }
+struct Scale {                              // of a request: its division is done while loads are awaited
+    double per, least;                      // log2(e) / T, never 0; logits so far below the largest weigh less than 2^-1020
+    __device__ explicit Scale(float t) : per(fmax(1.4426950408889634 / (double)t, 1e-300)), least(fmax(-707.0 * (double)t, -1e303)) {}
+};
 struct Weigher {
-    double top, per, least;                 // log2(e) / T, never 0; logits so far below the largest weigh less than 2^-1020
+    double top, per, least;
     bool plain;                             // the largest is not infinite
-    __device__ Weigher(float largest, float t) : top((double)largest), per(fmax(1.4426950408889634 / (double)t, 1e-300)), least(fmax(-707.0 * (double)t, -1e303)), plain(largest < INFINITY) {}
+    __device__ Weigher(float largest, const Scale& s) : top((double)largest), per(s.per), least(s.least), plain(largest < INFINITY) {}
     __device__ double power(double below) const {                               // of a logit so far below the largest, not less than `least`
         const double shifted = fma(below, per, 6755399441055744.0), f = fma(below, per, 6755399441055744.0 - shifted);
         double q = 1.325080551750225e-06;
@@ -167,6 +171,7 @@ __global__ __launch_bounds__(NT) void parts_kernel(Inputs in, float* __restrict_
     if (n < 0) return;
     const float t = in.temperature[r];
     const bool greedy = arg_max_asked(t);
+    const Scale scale(t);
     const int n_rows = n + 1 + (greedy || in.drafter == nullptr ? 0 : n);
     for (int i = blockIdx.z, turn = 0; i < n_rows; i += gridDim.z, turn ^= 1) {          // (two places for what meets in LDS in turn: one barrier a meeting)
         const float* row = i <= n ? in.logits + (first + i) * in.stride : in.drafter + r * in.drafter_request + (i - n - 1) * in.drafter_row;
@@ -195,7 +200,7 @@ __global__ __launch_bounds__(NT) void parts_kernel(Inputs in, float* __restrict_
             }
             continue;
         }
-        const Weigher weigh(bv, t);
+        const Weigher weigh(bv, scale);
         double sum = 0.0;
         if (weigh.plain) {
 #pragma unroll
@@ -218,7 +223,7 @@ struct Drawn {
     Weigher p, q;
     double over_p, over_q;
     int kind, x;
-    __device__ Drawn(const Verdict& v, float t) : p(v.top_p, t), q(v.top_q, t), over_p(v.sum_p > 0.0 ? 1.0 / v.sum_p : 0.0), over_q(v.sum_q > 0.0 ? 1.0 / v.sum_q : 0.0), kind(v.kind), x(v.x) {}
+    __device__ Drawn(const Verdict& v, const Scale& s) : p(v.top_p, s), q(v.top_q, s), over_p(v.sum_p > 0.0 ? 1.0 / v.sum_p : 0.0), over_q(v.sum_q > 0.0 ? 1.0 / v.sum_q : 0.0), kind(v.kind), x(v.x) {}
     __device__ bool plain() const { return p.plain && (kind != LESS_ROW || q.plain); }
     __device__ double weight(float target, float drafter, bool left_out) const {       // of plain rows
         const double w = p.fast(target);
@@ -259,6 +264,7 @@ __global__ __launch_bounds__(NT) void judge_kernel(Inputs in, const float* __res
             u = in.uniform[(size_t)r * (K + 1) + tid];
         }
     }
+    const Scale scale(t);
     for (int z = tid >> 4; z < 2 * K + 1; z += NT / 16) {   // sixteen lanes a row
         if (n < 0 || (z <= K ? z > n : (in.drafter == nullptr || z - K - 1 >= n || greedy))) continue;
         const size_t at = ((size_t)r * (2 * K + 1) + z) * in.n_chunks;
@@ -287,7 +293,7 @@ __global__ __launch_bounds__(NT) void judge_kernel(Inputs in, const float* __res
                 for (int j = 0; j < 4; ++j)
                     if (c0 + member + 16 * j < in.n_chunks && m[j] == now) place = min(place, i[j]);
             } else {
-                const Weigher weigh(now, t);
+                const Weigher weigh(now, scale);
                 double more = 0.0;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) more += s[j] * weigh.any(m[j]);
@@ -307,9 +313,9 @@ __global__ __launch_bounds__(NT) void judge_kernel(Inputs in, const float* __res
                 stay = x == arg[tid];
             } else {
                 // u q / whole_q < p / whole_p; a row without a token has no probabilities (its sum and all its weights are 0)
-                const double p = whole[tid] > 0.0 ? Weigher(top[tid], t).any(target_x) / whole[tid] : 0.0;
+                const double p = whole[tid] > 0.0 ? Weigher(top[tid], scale).any(target_x) / whole[tid] : 0.0;
                 double q = 1.0;
-                if (in.drafter != nullptr) q = whole[K + 1 + tid] > 0.0 ? Weigher(top[K + 1 + tid], t).any(drafter_x) / whole[K + 1 + tid] : 0.0;
+                if (in.drafter != nullptr) q = whole[K + 1 + tid] > 0.0 ? Weigher(top[K + 1 + tid], scale).any(drafter_x) / whole[K + 1 + tid] : 0.0;
                 stay = (double)u * q < p;
             }
         }
@@ -347,7 +353,7 @@ __global__ __launch_bounds__(NT) void judge_kernel(Inputs in, const float* __res
     const RunOf run(row, blockIdx.x, in.vocab), other(drafter, blockIdx.x, in.vocab);
     float a[PER], b[PER];
     double sum = 0.0;
-    const Drawn drawn(v, t);
+    const Drawn drawn(v, scale);
     if (run.fours == other.fours && drawn.plain()) {
         run.load(row, a);
         if (v.kind == LESS_ROW) other.load(drafter, b);
@@ -382,10 +388,11 @@ __device__ __forceinline__ double scan_f64(double v) {
     return v + before<0x143, 0xc>(v);                       // (the last of the first half, in the second)
 }
 
-__device__ __forceinline__ double last_lane(double v) {
+__device__ __forceinline__ double of_lane(double v, int lane) {                // (the same lane for the wave)
+    lane = __builtin_amdgcn_readfirstlane(lane);
     Words<double> a = __builtin_bit_cast(Words<double>, v);
 #pragma unroll
-    for (int i = 0; i < 2; ++i) a.w[i] = __builtin_amdgcn_readlane(a.w[i], 63);
+    for (int i = 0; i < 2; ++i) a.w[i] = __builtin_amdgcn_readlane(a.w[i], lane);
     return __builtin_bit_cast(double, a);
 }
 
@@ -406,21 +413,21 @@ __global__ __launch_bounds__(PICK_NT) void pick_kernel(Inputs in, const Verdict*
     if (v.kind == DONE) return;
     long first;
     drafts_of(in, r, first);
-    const float t = in.temperature[r];
+    const Scale scale(in.temperature[r]);
     const float* row = in.logits + (first + v.row) * in.stride;
     const float* drafter = v.kind == LESS_ROW ? in.drafter + r * in.drafter_request + v.row * in.drafter_row : row;
     const size_t parts = ((size_t)r * (2 * in.K + 1) + v.row) * in.n_chunks;
     for (int attempt = 0; attempt < 2; ++attempt) {
         if (tid < in.n_chunks) {                           // (MAX_CHUNKS threads)
             const bool own = v.kind == LESS_ROW || (v.kind == LESS_TOKEN && v.x / CHUNK == tid);
-            sums[tid] = own ? left : part_s[parts + tid] * Weigher(v.top_p, t).any(part_m[parts + tid]);
+            sums[tid] = own ? left : part_s[parts + tid] * Weigher(v.top_p, scale).any(part_m[parts + tid]);
         }
         __syncthreads();
         if (wave == 0) {
             const int each = (in.n_chunks + 63) / 64, from = lane * each, to = min(in.n_chunks, from + each);
             double mine = 0.0;
             for (int c = from; c < to; ++c) mine += sums[c];
-            const double upto = scan_f64(mine), below = before<0x138, 0xf>(upto), total = last_lane(upto);       // (the lane before's, 0 for the first)
+            const double upto = scan_f64(mine), below = before<0x138, 0xf>(upto), total = of_lane(upto, 63);       // (the lane before's, 0 for the first)
             const double goal = (double)u * total;
             const unsigned long long beyond = __ballot(goal < upto && mine > 0.0), some = __ballot(mine > 0.0);
             // the first lane whose runs end beyond the goal; by rounding, or for u = 1, the last that weighs anything
@@ -453,7 +460,7 @@ __global__ __launch_bounds__(PICK_NT) void pick_kernel(Inputs in, const Verdict*
         return;
     }
     const int begin = run * CHUNK, end = min(in.vocab, begin + CHUNK), lo = begin + tid * PICK_PER;
-    const Drawn drawn(v, t);
+    const Drawn drawn(v, scale);
     double w[PICK_PER], mine = 0.0;
     int last = -1;                                         // the last token that weighs anything
 #pragma unroll
@@ -467,9 +474,9 @@ __global__ __launch_bounds__(PICK_NT) void pick_kernel(Inputs in, const Verdict*
     const double upto = scan_f64(mine), below = before<0x138, 0xf>(upto);
     if (lane == 63) wave_total[wave] = upto;
     __syncthreads();
-    double walk = before_run;
-    for (int k = 0; k < wave; ++k) walk += wave_total[k];
-    walk += below;
+    static_assert(PICK_WAVES == 16, "a wave's sixteen lanes add up the waves' sums");
+    const double totals = scan_f64(lane < PICK_WAVES ? wave_total[lane] : 0.0);
+    double walk = before_run + (wave > 0 ? of_lane(totals, wave - 1) : 0.0) + below;
     int hit = 0x7fffffff;
 #pragma unroll
     for (int j = 0; j < PICK_PER; ++j) {
