@@ -19,8 +19,6 @@
 namespace {
 
 constexpr int CHUNK = 4096;                 // logits of a row that a workgroup takes
-constexpr int NT = 256;
-constexpr int PER = CHUNK / NT;             // ... and a thread
 constexpr int MAX_CHUNKS = 1024;            // runs of a row: as many as the threads that draw (a vocabulary of 4 M tokens)
 constexpr int MAX_DRAFTS = 64;
 constexpr int MAX_ROWS = 2 * MAX_DRAFTS + 1;
@@ -123,8 +121,10 @@ struct Sum { __device__ double operator()(double a, double b) const { return a +
 struct Largest { __device__ float operator()(float a, float b) const { return fmaxf(a, b); } };
 struct Least { __device__ int operator()(int a, int b) const { return min(a, b); } };
 
-// A thread's logits of a run: `v[4 u + c]` is number begin + 4 (tid + NT u) + c where four may be loaded at once, number begin + tid + NT (4 u + c) otherwise; -infinity behind `end`.
+// A thread's logits of a run that NT threads share: `v[4 u + c]` is number begin + 4 (tid + NT u) + c where four may be loaded at once, number begin + tid + NT (4 u + c) otherwise; -infinity behind `end`.
+template <int NT>
 struct RunOf {
+    static constexpr int PER = CHUNK / NT;
     int begin, end;
     bool fours;
     __device__ RunOf(const float* row, int run, int vocab) : begin(run * CHUNK), end(min(vocab, run * CHUNK + CHUNK)), fours((vocab & 3) == 0 && ((size_t)row & 15) == 0) {}
@@ -161,10 +161,12 @@ struct RunOf {
 
 // Largest logit (with its lowest index) and sum of exp((l - that) / T) of every run: workgroup (run, request, group of rows).  Of the rows that the request has, the target's 0 .. n and the drafter's 0 .. n - 1 behind
 // them, every gridDim.z-th is a workgroup's.  4.5 us for 9 rows of 128,256 tokens, 8.0 for 192 greedy ones of 32,003 (3.1 TB/s), 51 for 401 of 128,256 (4.0 TB/s; the loads alone take 40).
-__global__ __launch_bounds__(NT) void parts_kernel(Inputs in, float* __restrict__ part_m, int* __restrict__ part_i, double* __restrict__ part_s) {
-    __shared__ float sv[2][4];
-    __shared__ int si[2][4];
-    __shared__ double red[2][4];
+constexpr int PARTS_NT = 256;
+__global__ __launch_bounds__(PARTS_NT) void parts_kernel(Inputs in, float* __restrict__ part_m, int* __restrict__ part_i, double* __restrict__ part_s) {
+    constexpr int NT = PARTS_NT, PER = CHUNK / NT, WAVES = NT / 64;
+    __shared__ float sv[2][WAVES];
+    __shared__ int si[2][WAVES];
+    __shared__ double red[2][WAVES];
     const int r = blockIdx.y, tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
     long first;
     const int n = drafts_of(in, r, first);
@@ -175,7 +177,7 @@ __global__ __launch_bounds__(NT) void parts_kernel(Inputs in, float* __restrict_
     const int n_rows = n + 1 + (greedy || in.drafter == nullptr ? 0 : n);
     for (int i = blockIdx.z, turn = 0; i < n_rows; i += gridDim.z, turn ^= 1) {          // (two places for what meets in LDS in turn: one barrier a meeting)
         const float* row = i <= n ? in.logits + (first + i) * in.stride : in.drafter + r * in.drafter_request + (i - n - 1) * in.drafter_row;
-        const RunOf run(row, blockIdx.x, in.vocab);
+        const RunOf<NT> run(row, blockIdx.x, in.vocab);
         float v[PER];
         run.load(row, v);
         float bv = -INFINITY;
@@ -184,7 +186,9 @@ __global__ __launch_bounds__(NT) void parts_kernel(Inputs in, float* __restrict_
         bv = over_wave(bv, Largest());
         if (lane == 0) sv[turn][wave] = bv;
         barrier_lds();
-        bv = fmaxf(fmaxf(sv[turn][0], sv[turn][1]), fmaxf(sv[turn][2], sv[turn][3]));
+        bv = sv[turn][0];
+#pragma unroll
+        for (int w = 1; w < WAVES; ++w) bv = fmaxf(bv, sv[turn][w]);
         const size_t at = ((size_t)r * (2 * in.K + 1) + (i <= n ? i : in.K + i - n)) * in.n_chunks + blockIdx.x;
         if (greedy) {                                                   // the lowest place of the largest (of -infinity where there are only such and NaN)
             int mine = PER;
@@ -195,8 +199,10 @@ __global__ __launch_bounds__(NT) void parts_kernel(Inputs in, float* __restrict_
             if (lane == 0) si[turn][wave] = bi;
             barrier_lds();
             if (tid == 0) {
+#pragma unroll
+                for (int w = 1; w < WAVES; ++w) bi = min(bi, si[turn][w]);
                 part_m[at] = bv;
-                part_i[at] = min(min(si[turn][0], si[turn][1]), min(si[turn][2], si[turn][3]));
+                part_i[at] = bi;
             }
             continue;
         }
@@ -212,8 +218,10 @@ __global__ __launch_bounds__(NT) void parts_kernel(Inputs in, float* __restrict_
         if (lane == 0) red[turn][wave] = sum;
         barrier_lds();
         if (tid == 0) {
+#pragma unroll
+            for (int w = 1; w < WAVES; ++w) sum += red[turn][w];
             part_m[at] = bv;
-            part_s[at] = bv > -INFINITY ? ((red[turn][0] + red[turn][1]) + red[turn][2]) + red[turn][3] : 0.0;
+            part_s[at] = bv > -INFINITY ? sum : 0.0;
         }
     }
 }
@@ -238,6 +246,7 @@ struct Drawn {
 // Which drafts stay, and the sums over runs of what is drawn from, where the parts do not hold them already: every run of a request whose drafter's row is taken off, and the run that a draft is
 // left out of.  Workgroup (run, request); run 0's writes what the request has so far.  8.7 us for one request with 4 drafts, 20 for 64 with up to 7, which read two rows of 128,256 again
 // each (58 MB), once the verdict says which: its waits (6 us) have nothing beside them.
+template <int NT>
 __global__ __launch_bounds__(NT) void judge_kernel(Inputs in, const float* __restrict__ part_m, const int* __restrict__ part_i, const double* __restrict__ part_s, Verdict* __restrict__ verdicts,
                                                    double* __restrict__ rest, int* __restrict__ tokens, int* __restrict__ counts) {
     __shared__ float top[MAX_ROWS];
@@ -245,7 +254,8 @@ __global__ __launch_bounds__(NT) void judge_kernel(Inputs in, const float* __res
     __shared__ double whole[MAX_ROWS];
     __shared__ int drafted[MAX_DRAFTS];
     __shared__ int stays;                                   // drafts before the first that falls
-    __shared__ double red[4];
+    constexpr int PER = CHUNK / NT, WAVES = NT / 64;
+    __shared__ double red[WAVES];
     const int r = blockIdx.y, tid = threadIdx.x, K = in.K, member = tid & 15;
     int x = -1;                                             // this thread's draft, its logits, its number
     float target_x = -INFINITY, drafter_x = -INFINITY, u = 0.f;
@@ -350,7 +360,7 @@ __global__ __launch_bounds__(NT) void judge_kernel(Inputs in, const float* __res
     if (v.kind != LESS_ROW && !(v.kind == LESS_TOKEN && v.x / CHUNK == (int)blockIdx.x)) return;
     const float* row = in.logits + (first + v.row) * in.stride;
     const float* drafter = v.kind == LESS_ROW ? in.drafter + r * in.drafter_request + v.row * in.drafter_row : row;
-    const RunOf run(row, blockIdx.x, in.vocab), other(drafter, blockIdx.x, in.vocab);
+    const RunOf<NT> run(row, blockIdx.x, in.vocab), other(drafter, blockIdx.x, in.vocab);
     float a[PER], b[PER];
     double sum = 0.0;
     const Drawn drawn(v, scale);
@@ -368,7 +378,11 @@ __global__ __launch_bounds__(NT) void judge_kernel(Inputs in, const float* __res
     sum = over_wave(sum, Sum());
     if ((tid & 63) == 0) red[tid >> 6] = sum;
     __syncthreads();
-    if (tid == 0) rest[(size_t)r * in.n_chunks + blockIdx.x] = ((red[0] + red[1]) + red[2]) + red[3];
+    if (tid == 0) {
+#pragma unroll
+        for (int w = 1; w < WAVES; ++w) sum += red[w];
+        rest[(size_t)r * in.n_chunks + blockIdx.x] = sum;
+    }
 }
 
 // The sum of a wave's lanes up to each: within sixteen by lanes 1, 2, 4 and 8 before (0 where there are none), then the sixteen before, then the 32 before.
@@ -520,9 +534,13 @@ GI_API int gi_verify_drafts(const float* logits, int n_rows, long stride, const 
     // A workgroup adds up several of a request's rows where there are more than 32 workgroups a compute unit without: their start costs as much as a short run.  Aimed at 8, 16, 32 and 200 of them, 64 requests with up to
     // 15 rows of 128,256 tokens took 99, 89, 83 and 95 us in all; a few requests have a workgroup for every row and run either way.
     const int groups = (int)min((long)most, max(1l, 32 * (long)gi_compute_units() / ((long)n_chunks * n_requests)));
-    parts_kernel<<<dim3(n_chunks, n_requests, groups), NT, 0, stream>>>(in, part_m, part_i, part_s);
+    parts_kernel<<<dim3(n_chunks, n_requests, groups), PARTS_NT, 0, stream>>>(in, part_m, part_i, part_s);
     GI_CHECK_LAUNCH("verify_drafts (parts)");
-    judge_kernel<<<dim3(n_chunks, n_requests), NT, 0, stream>>>(in, part_m, part_i, part_s, verdicts, rest, tokens, counts);
+    // 1,024 threads where there is a compute unit for every workgroup, 256 otherwise: 1 and 8 requests with 4 drafts of a model, 128,256 tokens, take 16.4 and 22.1 us in all instead of 17.6 and 23.6; 16 and 64 would take
+    // 33.5 and 105 instead of 31.3 and 84.  (The sums of all rows take longer with more threads even for one request.)
+    const dim3 runs(n_chunks, n_requests);
+    if ((long)n_chunks * n_requests <= gi_compute_units()) judge_kernel<1024><<<runs, 1024, 0, stream>>>(in, part_m, part_i, part_s, verdicts, rest, tokens, counts);
+    else judge_kernel<256><<<runs, 256, 0, stream>>>(in, part_m, part_i, part_s, verdicts, rest, tokens, counts);
     GI_CHECK_LAUNCH("verify_drafts (judge)");
     pick_kernel<<<n_requests, PICK_NT, 0, stream>>>(in, verdicts, part_m, part_s, rest, tokens);
     GI_CHECK_LAUNCH("verify_drafts (pick)");
