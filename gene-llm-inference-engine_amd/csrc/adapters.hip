@@ -9,6 +9,7 @@
 // row in scratch between them.  A few rows are taken one by one (the last kernels below).  More are cut into tiles: runs of neighbours with one adapter, ended at every 64th row too, as a
 // request's rows lie together.  How many tiles there are only the device knows: every workgroup of the way down counts them for itself and takes every so manieth piece of work, and they leave the way up a list.
 #include "common.h"
+#include "lanes.h"
 
 #include <type_traits>
 
@@ -117,7 +118,7 @@ struct Tiles {
     int n_rows, each, entries;              // rows; blocks of 64 rows that one count is of; counts
 
     __device__ unsigned long long begins(int block) const {            // the rows of a block at which tiles begin
-        const int lane = threadIdx.x & 63, i = block * TILE + lane, mine = ids[min(i, n_rows - 1)], neighbour = __shfl_up(mine, 1, 64);
+        const int lane = threadIdx.x & 63, i = block * TILE + lane, mine = ids[min(i, n_rows - 1)], neighbour = lane_before(mine);
         return __ballot(i < n_rows && (lane == 0 || mine != neighbour));
     }
     // before[c]: tiles before the rows of count c; the number of all tiles comes back.
@@ -144,14 +145,9 @@ struct Tiles {
         for (int u = 0; u < COUNTS / 64; ++u) {
             if (u * 64 >= entries) break;
             const int c = u * 64 + lane, v = c < entries ? before[c] : 0;
-            int upto = v;
-#pragma unroll
-            for (int off = 1; off < 64; off <<= 1) {
-                const int below = __shfl_up(upto, off, 64);
-                if (lane >= off) upto += below;
-            }
+            const int upto = sum_up_to(v);
             mine[u] = total + upto - v;
-            total += __shfl(upto, 63, 64);
+            total += of_lane(upto, 63);
         }
         __syncthreads();
         if (wave == 0)
@@ -619,7 +615,7 @@ __global__ __launch_bounds__(256) void adapters_down_few_kernel(const bf16_t* __
             sum = fmaf(__uint_as_float(xw[u] & 0xffff0000u), __uint_as_float(aw[u] & 0xffff0000u), sum);
         }
     }
-    sum = wave_sum(sum);
+    sum = over_wave(sum, Add());
     if ((tid & 63) == 0) red[tid >> 6] = sum;
     __syncthreads();
     if (tid == 0) sums[(size_t)row * ranks + blockIdx.x] = (red[0] + red[1]) + (red[2] + red[3]);
@@ -722,7 +718,7 @@ __global__ __launch_bounds__(256) void adapters_both_few_kernel(const bf16_t* __
             }
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                four[i] = wave_sum(four[i]);
+                four[i] = over_wave(four[i], Add());
                 if (lane == 0 && k0 + wave + 4 * i < rank) t[k0 + wave + 4 * i] = four[i];
             }
         }

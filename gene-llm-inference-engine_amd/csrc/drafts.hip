@@ -15,6 +15,7 @@
 // tokens, 206 MB: 51 + 20 + 9 us); of a few the waits that follow one another (one request with 4 drafts, 9 such rows: 4.5 + 8.7 + 7.0 us).  A last workgroup that draws by itself instead of a third launch has
 // to see what the others wrote: with the fences for that one request takes 29.7 us instead of 20.5, 64 take 121 instead of 81.
 #include "common.h"
+#include "lanes.h"
 
 namespace {
 
@@ -94,33 +95,6 @@ struct Weigher {
     __device__ double any(float l) const { return plain ? fast(l) : l == INFINITY ? 1.0 : 0.0; }
 };
 
-// Sums and the like over lanes without a trip through LDS (the shuffles' way): what a reduction takes is the wait for its steps.  Every lane of the wave, or of its sixteen, ends with the same value.
-template <typename T> struct Words { int w[sizeof(T) / 4]; };
-template <int BY, typename T, typename Op>
-__device__ __forceinline__ T with_lane(T v, Op op) {               // v of lane l and of lane l ^ BY, or for less than 16, where v is the same every 2 BY lanes of sixteen, of the one BY before
-    Words<T> a = __builtin_bit_cast(Words<T>, v), b;
-#pragma unroll
-    for (int i = 0; i < (int)sizeof(T) / 4; ++i) {
-        if constexpr (BY == 32) {                                   // halves swapped between two copies: the lower ones in both halves of one, the upper ones in the other
-            const auto both = __builtin_amdgcn_permlane32_swap(a.w[i], a.w[i], false, false);
-            a.w[i] = both[0];
-            b.w[i] = both[1];
-        } else if constexpr (BY == 16) {
-            const auto both = __builtin_amdgcn_permlane16_swap(a.w[i], a.w[i], false, false);
-            a.w[i] = both[0];
-            b.w[i] = both[1];
-        } else {
-            b.w[i] = __builtin_amdgcn_update_dpp(0, a.w[i], 0x120 + BY, 0xf, 0xf, false);        // (rotated within sixteen)
-        }
-    }
-    return op(__builtin_bit_cast(T, a), __builtin_bit_cast(T, b));
-}
-template <typename T, typename Op> __device__ __forceinline__ T over_16(T v, Op op) { return with_lane<1>(with_lane<2>(with_lane<4>(with_lane<8>(v, op), op), op), op); }
-template <typename T, typename Op> __device__ __forceinline__ T over_wave(T v, Op op) { return over_16(with_lane<16>(with_lane<32>(v, op), op), op); }
-struct Sum { __device__ double operator()(double a, double b) const { return a + b; } };
-struct Largest { __device__ float operator()(float a, float b) const { return fmaxf(a, b); } };
-struct Least { __device__ int operator()(int a, int b) const { return min(a, b); } };
-
 // A thread's logits of a run that NT threads share: `v[4 u + c]` is number begin + 4 (tid + NT u) + c where four may be loaded at once, number begin + tid + NT (4 u + c) otherwise; -infinity behind `end`.
 template <int NT>
 struct RunOf {
@@ -183,7 +157,7 @@ __global__ __launch_bounds__(PARTS_NT) void parts_kernel(Inputs in, float* __res
         float bv = -INFINITY;
 #pragma unroll
         for (int j = 0; j < PER; ++j) bv = fmaxf(bv, v[j]);            // (NaN is passed over)
-        bv = over_wave(bv, Largest());
+        bv = over_wave(bv, Larger());
         if (lane == 0) sv[turn][wave] = bv;
         barrier_lds();
         bv = sv[turn][0];
@@ -195,7 +169,7 @@ __global__ __launch_bounds__(PARTS_NT) void parts_kernel(Inputs in, float* __res
 #pragma unroll
             for (int j = PER - 1; j >= 0; --j) mine = number(v[j]) == bv ? j : mine;
             int bi = mine < PER && run.at(mine) < run.end ? run.at(mine) : 0x7fffffff;       // (a thread's numbers ascend)
-            bi = over_wave(bi, Least());
+            bi = over_wave(bi, Lesser());
             if (lane == 0) si[turn][wave] = bi;
             barrier_lds();
             if (tid == 0) {
@@ -214,7 +188,7 @@ __global__ __launch_bounds__(PARTS_NT) void parts_kernel(Inputs in, float* __res
         } else {
             for (int k = run.begin + tid; k < run.end; k += NT) sum += weigh.any(row[k]);
         }
-        sum = over_wave(sum, Sum());
+        sum = over_wave(sum, Add());
         if (lane == 0) red[turn][wave] = sum;
         barrier_lds();
         if (tid == 0) {
@@ -295,7 +269,7 @@ __global__ __launch_bounds__(NT) void judge_kernel(Inputs in, const float* __res
                     else s[j] = part_s[at + c];
                 }
             }
-            const float bv = over_16(fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])), Largest());
+            const float bv = over_16(fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])), Larger());
             const float now = fmaxf(largest, bv);
             if (greedy) {
                 if (now > largest) place = 0x7fffffff;      // (a place of an earlier run that holds as much is lower)
@@ -307,11 +281,11 @@ __global__ __launch_bounds__(NT) void judge_kernel(Inputs in, const float* __res
                 double more = 0.0;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) more += s[j] * weigh.any(m[j]);
-                sum = sum * weigh.any(largest) + over_16(more, Sum());
+                sum = sum * weigh.any(largest) + over_16(more, Add());
             }
             largest = now;
         }
-        place = over_16(place, Least());
+        place = over_16(place, Lesser());
         if (member == 0) { top[z] = largest; arg[z] = place; whole[z] = sum; }
     }
     __syncthreads();
@@ -375,7 +349,7 @@ __global__ __launch_bounds__(NT) void judge_kernel(Inputs in, const float* __res
     } else {
         for (int i = run.begin + tid; i < run.end; i += NT) sum += drawn.any(row[i], drafter[i], i);
     }
-    sum = over_wave(sum, Sum());
+    sum = over_wave(sum, Add());
     if ((tid & 63) == 0) red[tid >> 6] = sum;
     __syncthreads();
     if (tid == 0) {
@@ -383,31 +357,6 @@ __global__ __launch_bounds__(NT) void judge_kernel(Inputs in, const float* __res
         for (int w = 1; w < WAVES; ++w) sum += red[w];
         rest[(size_t)r * in.n_chunks + blockIdx.x] = sum;
     }
-}
-
-// The sum of a wave's lanes up to each: within sixteen by lanes 1, 2, 4 and 8 before (0 where there are none), then the sixteen before, then the 32 before.
-template <int CTRL, int ROWS>
-__device__ __forceinline__ double before(double v) {
-    Words<double> a = __builtin_bit_cast(Words<double>, v);
-#pragma unroll
-    for (int i = 0; i < 2; ++i) a.w[i] = __builtin_amdgcn_update_dpp(0, a.w[i], CTRL, ROWS, 0xf, false);
-    return __builtin_bit_cast(double, a);
-}
-__device__ __forceinline__ double scan_f64(double v) {
-    v += before<0x111, 0xf>(v);
-    v += before<0x112, 0xf>(v);
-    v += before<0x114, 0xf>(v);
-    v += before<0x118, 0xf>(v);
-    v += before<0x142, 0xa>(v);                             // (the last of the sixteen before, in the second and the fourth)
-    return v + before<0x143, 0xc>(v);                       // (the last of the first half, in the second)
-}
-
-__device__ __forceinline__ double of_lane(double v, int lane) {                // (the same lane for the wave)
-    lane = __builtin_amdgcn_readfirstlane(lane);
-    Words<double> a = __builtin_bit_cast(Words<double>, v);
-#pragma unroll
-    for (int i = 0; i < 2; ++i) a.w[i] = __builtin_amdgcn_readlane(a.w[i], lane);
-    return __builtin_bit_cast(double, a);
 }
 
 // The draw: one workgroup a request.  The run is found among the runs' sums (by a prefix sum over a wave's lanes, which share the runs out, and a walk over one lane's), then the token in the run: a
@@ -441,7 +390,7 @@ __global__ __launch_bounds__(PICK_NT) void pick_kernel(Inputs in, const Verdict*
             const int each = (in.n_chunks + 63) / 64, from = lane * each, to = min(in.n_chunks, from + each);
             double mine = 0.0;
             for (int c = from; c < to; ++c) mine += sums[c];
-            const double upto = scan_f64(mine), below = before<0x138, 0xf>(upto), total = of_lane(upto, 63);       // (the lane before's, 0 for the first)
+            const double upto = sum_up_to(mine), below = lane_before(upto), total = of_lane(upto, 63);       // (the lane before's, 0 for the first)
             const double goal = (double)u * total;
             const unsigned long long beyond = __ballot(goal < upto && mine > 0.0), some = __ballot(mine > 0.0);
             // the first lane whose runs end beyond the goal; by rounding, or for u = 1, the last that weighs anything
@@ -485,11 +434,11 @@ __global__ __launch_bounds__(PICK_NT) void pick_kernel(Inputs in, const Verdict*
         mine += w[j];
         if (w[j] > 0.0) last = lo + j;
     }
-    const double upto = scan_f64(mine), below = before<0x138, 0xf>(upto);
+    const double upto = sum_up_to(mine), below = lane_before(upto);
     if (lane == 63) wave_total[wave] = upto;
     __syncthreads();
     static_assert(PICK_WAVES == 16, "a wave's sixteen lanes add up the waves' sums");
-    const double totals = scan_f64(lane < PICK_WAVES ? wave_total[lane] : 0.0);
+    const double totals = sum_up_to(lane < PICK_WAVES ? wave_total[lane] : 0.0);
     double walk = before_run + (wave > 0 ? of_lane(totals, wave - 1) : 0.0) + below;
     int hit = 0x7fffffff;
 #pragma unroll
