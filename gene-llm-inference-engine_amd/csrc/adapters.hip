@@ -61,53 +61,56 @@ __device__ __forceinline__ floatx4 times(const float4& m, const float4& n, float
 }
 __device__ __forceinline__ floatx4 times(const Piece<false>& m, const Piece<false>& n, floatx4 sum) { return times(m.v[1], n.v[1], times(m.v[0], n.v[0], sum)); }
 
-// Numbers k .. k + RUN of a row, 0 from `end` on.  ALIGNED: `end` is a multiple of RUN, not 0, and the row begins at a whole run of loads.  What lies beyond is asked for at the last
-// run's place and dropped: a branch around a load would make the wave wait for all its loads where the first is used.
-template <bool ALIGNED>
+// Numbers k .. k + RUN of a row, 0 from `end` on, by loads of AT_ONCE numbers: `end` is a multiple of that, not 0, and the row begins at a whole run of loads.  What lies beyond is asked for at the last
+// load's place and dropped: a branch around a load would make the wave wait for all its loads where the first is used.
+template <int AT_ONCE>
 __device__ __forceinline__ uint4 load_run(const bf16_t* __restrict__ row, int k, int end) {
-    if (ALIGNED) {
+    if constexpr (AT_ONCE == 8) {
         const uint4 v = *reinterpret_cast<const uint4*>(row + min(k, end - 8));
         const bool in = k < end;
         return uint4{in ? v.x : 0u, in ? v.y : 0u, in ? v.z : 0u, in ? v.w : 0u};
-    }
-    uint32_t v[8];
+    } else if constexpr (AT_ONCE == 4) {
+        const uint2 v = *reinterpret_cast<const uint2*>(row + min(k, end - 4)), w = *reinterpret_cast<const uint2*>(row + min(k + 4, end - 4));
+        const bool in = k < end, more = k + 4 < end;
+        return uint4{in ? v.x : 0u, in ? v.y : 0u, more ? w.x : 0u, more ? w.y : 0u};
+    } else {
+        uint32_t v[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = k + i < end ? row[k + i] : 0u;
-    return uint4{v[0] | v[1] << 16, v[2] | v[3] << 16, v[4] | v[5] << 16, v[6] | v[7] << 16};
+        for (int i = 0; i < 8; ++i) v[i] = row[min(k + i, end - 1)];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = k + i < end ? v[i] : 0u;
+        return uint4{v[0] | v[1] << 16, v[2] | v[3] << 16, v[4] | v[5] << 16, v[6] | v[7] << 16};
+    }
 }
-template <bool ALIGNED>
-__device__ __forceinline__ float4 load_run_f32(const float* __restrict__ row, int k, int end) {
-    if (ALIGNED) {
-        const float4 v = *reinterpret_cast<const float4*>(row + min(k, end - 4));
-        const bool in = k < end;
-        return float4{in ? v.x : 0.f, in ? v.y : 0.f, in ? v.z : 0.f, in ? v.w : 0.f};
-    }
+template <int AT_ONCE, typename T>
+__device__ __forceinline__ float4 load_run_f32(const T* __restrict__ row, int k, int end) {
     float v[4];
+    if constexpr (AT_ONCE == 4) {
+        const int from = min(k, end - 4);
+        if constexpr (std::is_same<T, float>::value) {
+            const float4 w = *reinterpret_cast<const float4*>(row + from);
+            v[0] = w.x; v[1] = w.y; v[2] = w.z; v[3] = w.w;
+        } else {
+            const uint2 w = *reinterpret_cast<const uint2*>(row + from);
+            v[0] = __uint_as_float(w.x << 16); v[1] = __uint_as_float(w.x & 0xffff0000u); v[2] = __uint_as_float(w.y << 16); v[3] = __uint_as_float(w.y & 0xffff0000u);
+        }
+    } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = k + i < end ? row[k + i] : 0.f;
+        for (int i = 0; i < 4; ++i) v[i] = load_f32(row, (size_t)min(k + i, end - 1));
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = k + i < end ? v[i] : 0.f;
     return float4{v[0], v[1], v[2], v[3]};
 }
-template <bool ALIGNED>
-__device__ __forceinline__ float4 load_run_f32(const bf16_t* __restrict__ row, int k, int end) {
-    if (ALIGNED) {
-        const uint2 v = *reinterpret_cast<const uint2*>(row + min(k, end - 4));
-        const bool in = k < end;
-        return float4{in ? __uint_as_float(v.x << 16) : 0.f, in ? __uint_as_float(v.x & 0xffff0000u) : 0.f, in ? __uint_as_float(v.y << 16) : 0.f, in ? __uint_as_float(v.y & 0xffff0000u) : 0.f};
-    }
-    float v[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = k + i < end ? bf16_to_f32(row[k + i]) : 0.f;
-    return float4{v[0], v[1], v[2], v[3]};
-}
-template <bool ALIGNED, typename T>
+template <int AT_ONCE, typename T>
 __device__ __forceinline__ void load_piece(Piece<true>& p, const T* __restrict__ row, int k, int end, int group) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) p.v[h] = load_run<ALIGNED>((const bf16_t*)row, k + 32 * h + 8 * group, end);
+    for (int h = 0; h < 2; ++h) p.v[h] = load_run<AT_ONCE>((const bf16_t*)row, k + 32 * h + 8 * group, end);
 }
-template <bool ALIGNED, typename T>
+template <int AT_ONCE, typename T>
 __device__ __forceinline__ void load_piece(Piece<false>& p, const T* __restrict__ row, int k, int end, int group) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) p.v[h] = load_run_f32<ALIGNED>(row, k + 16 * h + 4 * group, end);
+    for (int h = 0; h < 2; ++h) p.v[h] = load_run_f32<AT_ONCE>(row, k + 16 * h + 4 * group, end);
 }
 
 // The tiles of a batch, counted by every workgroup: a tile begins at every 64th row and where a row's adapter is not its neighbour's.
@@ -310,12 +313,12 @@ __global__ __launch_bounds__(64 * WAVES) void adapters_down_kernel(const typenam
             const int k = k0 + whole * STEP;
             P ap[MT];
 #pragma unroll
-            for (int i = 0; i < MT; ++i) load_piece<true>(ap[i], ae + (size_t)min(first_rank + 16 * i + at, d.ranks - 1) * d.width, k, end, group);
+            for (int i = 0; i < MT; ++i) load_piece<P::RUN>(ap[i], ae + (size_t)min(first_rank + 16 * i + at, d.ranks - 1) * d.width, k, end, group);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 if (16 * j >= rows) break;
                 P xp;
-                load_piece<true>(xp, x + (size_t)(first_row + min(16 * j + at, rows - 1)) * d.ldx, k, end, group);
+                load_piece<P::RUN>(xp, x + (size_t)(first_row + min(16 * j + at, rows - 1)) * d.ldx, k, end, group);
 #pragma unroll
                 for (int i = 0; i < MT; ++i) sum[j][i] = times(ap[i], xp, sum[j][i]);
             }
@@ -361,12 +364,12 @@ __global__ __launch_bounds__(64 * ANY_WAVES) void adapters_down_any_kernel(const
         for (int k = begin + wave * P::BLOCK; k < end; k += P::BLOCK * ANY_WAVES) {
             P ap[MT];
 #pragma unroll
-            for (int i = 0; i < MT; ++i) load_piece<ALIGNED>(ap[i], ar[i], k, end, group);
+            for (int i = 0; i < MT; ++i) load_piece<ALIGNED ? P::RUN : 1>(ap[i], ar[i], k, end, group);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 if (16 * j >= rows) break;
                 P xp;
-                load_piece<ALIGNED>(xp, xr[j], k, end, group);
+                load_piece<ALIGNED ? P::RUN : 1>(xp, xr[j], k, end, group);
 #pragma unroll
                 for (int i = 0; i < MT; ++i) sum[j][i] = times(ap[i], xp, sum[j][i]);
             }
@@ -405,8 +408,8 @@ constexpr int PIECES = 3;                   // bfloat16 numbers that hold a 32-b
 // One run along the ranks of 16 columns of B.
 template <bool LOW> struct Run { uint4 v; };
 template <> struct Run<false> { float4 v; };
-template <bool ALIGNED, typename W> __device__ __forceinline__ void load_b(Run<true>& m, const W* row, int k, int rank) { m.v = load_run<ALIGNED>((const bf16_t*)row, k, rank); }
-template <bool ALIGNED, typename W> __device__ __forceinline__ void load_b(Run<false>& m, const W* row, int k, int rank) { m.v = load_run_f32<ALIGNED>(row, k, rank); }
+template <int AT_ONCE, typename W> __device__ __forceinline__ void load_b(Run<true>& m, const W* row, int k, int rank) { m.v = load_run<AT_ONCE>((const bf16_t*)row, k, rank); }
+template <int AT_ONCE, typename W> __device__ __forceinline__ void load_b(Run<false>& m, const W* row, int k, int rank) { m.v = load_run_f32<AT_ONCE>(row, k, rank); }
 
 // One run of a row's sums, in pieces; they lie `apart` numbers behind one another.
 template <bool LOW> struct Held { bf16x8 v[PIECES]; };
@@ -427,11 +430,11 @@ __device__ __forceinline__ floatx4 times(const Held<false>& t, const Run<false>&
 // Then a wave takes 64 columns at a time and of them 16 rows after 16 rows, with the columns' runs of B in registers throughout (loaded, they lie as the matrix cores want them, every lane in another
 // row of B: 64 accesses to the first-level cache a load); where the strip is no wider than 64 columns the waves share out the rows.  In the product D = M N the rows are M's and the columns
 // N's: number n of the four products of a step has columns 4 l + n, l = 0 .. 15, so that a lane ends with four neighbours and sixteen lanes with whole lines of base and out.  As on the way down no
-// row's values meet another's.  ALIGNED: runs of B, and fours of columns of base and out, may be loaded at once, and columns come in fours.  KS: runs of ranks that a wave keeps; 0 for any number,
+// row's values meet another's.  ALIGNED: fours of columns of base and out may be loaded at once, and columns come in fours.  AT_ONCE: numbers of B that one load brings.  KS: runs of ranks that a wave keeps; 0 for any number,
 // loaded again for every 16 rows (8,192 rows of 14,336 columns, rank 16: 239 us kept, 272 loaded again).  LOW_BASE, LOW_OUT: of aligned ones whether they are bfloat16 (a branch on it where they are loaded would have every load waited for); `io` says it of others.
 // 4,096 rows of 4,096 32-bit columns, rank 64: 41 us for the 134 MB of base and out (a copy of as much takes 25); 531 of 6,144, rank 24, onto bfloat16 10.3; 2,048 of 2,048, rank 32, 9.4; 301 of 2,048 in 32 bits,
 // rank 10, 10.6.  Asking for a whole tile's base at once instead of 16 rows ahead makes it no faster: 4,096 rows of 4,096 both ways 50 us instead of 47, with 256 registers instead of 141.
-template <bool LOW, typename W, bool ALIGNED, int KS, bool LOW_BASE, bool LOW_OUT>
+template <bool LOW, typename W, bool ALIGNED, int AT_ONCE, int KS, bool LOW_BASE, bool LOW_OUT>
 __global__ __launch_bounds__(UP_NT) void adapters_up_kernel(const float* __restrict__ sums, const W* __restrict__ b, const float* __restrict__ scales, const Tile* __restrict__ list,
                                                             const int* __restrict__ n_listed, Rows io, int n_rows, int rank, int n_segments, Slices slices, int strip_columns, int n_adapters) {
     typedef Piece<LOW> P;
@@ -467,7 +470,7 @@ __global__ __launch_bounds__(UP_NT) void adapters_up_kernel(const float* __restr
 #pragma unroll
             for (int k = 0; k < KS; ++k)
 #pragma unroll
-                for (int n = 0; n < 4; ++n) load_b<ALIGNED>(br[k][n], be + (size_t)(min(c0 + 4 * at, end - 4) + n) * rank, DEPTH * k + P::RUN * group, rank);
+                for (int n = 0; n < 4; ++n) load_b<AT_ONCE>(br[k][n], be + (size_t)(min(c0 + 4 * at, end - 4) + n) * rank, DEPTH * k + P::RUN * group, rank);
         };
         // Rows behind the last are taken as that one throughout, and columns behind the end as the last four: their lanes load and store what the lanes that own them do, at the same time.  Without a branch
         // around any store the wait for a load counts what was asked for behind it, and no load waits for a store's end.
@@ -564,7 +567,7 @@ __global__ __launch_bounds__(UP_NT) void adapters_up_kernel(const float* __restr
                 } else {
                     for (int k = 0; k < padded; k += DEPTH) {
 #pragma unroll
-                        for (int n = 0; n < 4; ++n) load_b<ALIGNED>(br[0][n], be + (size_t)(ALIGNED ? col + n : min(col + n, end - 1)) * rank, k + P::RUN * group, rank);
+                        for (int n = 0; n < 4; ++n) load_b<AT_ONCE>(br[0][n], be + (size_t)(ALIGNED ? col + n : min(col + n, end - 1)) * rank, k + P::RUN * group, rank);
                         load_row(t, row + k, apart);
 #pragma unroll
                         for (int n = 0; n < 4; ++n) sum[n] = times(t, br[0][n], sum[n]);
@@ -623,6 +626,13 @@ __global__ __launch_bounds__(256) void adapters_down_few_kernel(const bf16_t* __
 
 // Up: a thread has FEW_COLUMNS columns, 256 apart, of a row; the row's sums come as scalars.  64 rows of 14,336, rank 16: 8.1 us for 37 MB (4.5 TB/s).
 constexpr int FEW_COLUMNS = 2;
+template <int N> struct Some;               // N bfloat16 numbers, loaded at once
+template <> struct Some<8> { uint4 v; __device__ float operator[](int i) const { const uint32_t w[4] = {v.x, v.y, v.z, v.w}; return __uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16); } };
+template <> struct Some<4> { uint2 v; __device__ float operator[](int i) const { const uint32_t w[2] = {v.x, v.y}; return __uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16); } };
+template <> struct Some<2> { uint32_t v; __device__ float operator[](int i) const { return __uint_as_float(i & 1 ? v & 0xffff0000u : v << 16); } };
+template <> struct Some<1> { bf16_t v; __device__ float operator[](int) const { return bf16_to_f32(v); } };
+
+template <int N>                            // ranks of a column that one load brings
 __global__ __launch_bounds__(256) void adapters_up_few_kernel(const float* __restrict__ sums, const bf16_t* __restrict__ b, const float* __restrict__ scales, const int* __restrict__ ids,
                                                               Rows io, int rank, Slices slices, int n_adapters) {
     const int row = blockIdx.y;
@@ -644,19 +654,14 @@ __global__ __launch_bounds__(256) void adapters_up_few_kernel(const float* __res
 #pragma unroll
         for (int c = 0; c < FEW_COLUMNS; ++c) br[c] = b + ((size_t)e * slices.begin[slices.n] + min(begin + 256 * c, end - 1)) * rank;
         const float scale = scales != nullptr ? scales[e] : 1.f;
-        for (int k = 0; k < rank; k += 8) {
-            uint4 v[FEW_COLUMNS];
+        for (int k = 0; k < rank; k += N) {
+            Some<N> v[FEW_COLUMNS];
 #pragma unroll
-            for (int c = 0; c < FEW_COLUMNS; ++c) v[c] = *reinterpret_cast<const uint4*>(br[c] + k);
+            for (int c = 0; c < FEW_COLUMNS; ++c) v[c] = *reinterpret_cast<const Some<N>*>(br[c] + k);
 #pragma unroll
-            for (int c = 0; c < FEW_COLUMNS; ++c) {
-                const uint32_t w[4] = {v[c].x, v[c].y, v[c].z, v[c].w};
+            for (int c = 0; c < FEW_COLUMNS; ++c)
 #pragma unroll
-                for (int u = 0; u < 4; ++u) {
-                    sum[c] = fmaf(t[k + 2 * u], __uint_as_float(w[u] << 16), sum[c]);
-                    sum[c] = fmaf(t[k + 2 * u + 1], __uint_as_float(w[u] & 0xffff0000u), sum[c]);
-                }
-            }
+                for (int u = 0; u < N; ++u) sum[c] = fmaf(t[k + u], v[c][u], sum[c]);
         }
 #pragma unroll
         for (int c = 0; c < FEW_COLUMNS; ++c) was[c] = fmaf(scale, sum[c], was[c]);
@@ -670,6 +675,7 @@ bool aligned(const void* p, int bytes) { return (size_t)p % bytes == 0; }
 
 // Both ways in one launch, where making a row's sums anew for every strip of its columns costs less than a second launch: a wave makes every fourth sum, then a thread has its columns as above.  One
 // row of 2,048 onto 2,048, rank 16: 4.6 us, the waits of three loads that follow one another.
+template <int N>
 __global__ __launch_bounds__(256) void adapters_both_few_kernel(const bf16_t* __restrict__ x, long ldx, const bf16_t* __restrict__ a, const bf16_t* __restrict__ b, const float* __restrict__ scales,
                                                                 const int* __restrict__ ids, Rows io, int width, int rank, Slices slices, int n_adapters) {
     __shared__ float t[MAX_RANK];
@@ -688,11 +694,11 @@ __global__ __launch_bounds__(256) void adapters_both_few_kernel(const bf16_t* __
     }
     if (some) {
         const bf16_t* br[FEW_COLUMNS];
-        uint4 v[FEW_COLUMNS];
+        Some<N> v[FEW_COLUMNS];
 #pragma unroll
         for (int c = 0; c < FEW_COLUMNS; ++c) {
             br[c] = b + ((size_t)e * slices.begin[slices.n] + min(begin + 256 * c, end - 1)) * rank;
-            v[c] = *reinterpret_cast<const uint4*>(br[c]);
+            v[c] = *reinterpret_cast<const Some<N>*>(br[c]);
         }
         const float scale = scales != nullptr ? scales[e] : 1.f;
         const bf16_t* xr = x + (size_t)row * ldx;
@@ -723,16 +729,13 @@ __global__ __launch_bounds__(256) void adapters_both_few_kernel(const bf16_t* __
             }
         }
         __syncthreads();
-        for (int k = 0; k < rank; k += 8) {
+        for (int k = 0; k < rank; k += N) {
 #pragma unroll
             for (int c = 0; c < FEW_COLUMNS; ++c) {
-                const uint32_t w[4] = {v[c].x, v[c].y, v[c].z, v[c].w};
-                if (k + 8 < rank) v[c] = *reinterpret_cast<const uint4*>(br[c] + k + 8);
+                const Some<N> now = v[c];
+                if (k + N < rank) v[c] = *reinterpret_cast<const Some<N>*>(br[c] + k + N);
 #pragma unroll
-                for (int u = 0; u < 4; ++u) {
-                    sum[c] = fmaf(t[k + 2 * u], __uint_as_float(w[u] << 16), sum[c]);
-                    sum[c] = fmaf(t[k + 2 * u + 1], __uint_as_float(w[u] & 0xffff0000u), sum[c]);
-                }
+                for (int u = 0; u < N; ++u) sum[c] = fmaf(t[k + u], now[u], sum[c]);
             }
         }
 #pragma unroll
@@ -820,22 +823,21 @@ template <bool LOW> constexpr int up_lds(int rank) {
     return TILE * ((rank + DEPTH - 1) / DEPTH * DEPTH + Piece<LOW>::RUN) * (LOW ? 2 * PIECES : 4);
 }
 
-template <bool LOW, typename W, bool ALIGNED, int KS, bool LOW_BASE, bool LOW_OUT>
+template <bool LOW, typename W, bool ALIGNED, int AT_ONCE, int KS, bool LOW_BASE, bool LOW_OUT>
 int up_launch(const Call& c, const Slices& slices, int strip) {
     static bool raised[MAX_DEVICES] = {};
     constexpr int most = up_lds<LOW>(MAX_RANK);
-    if (raise_lds((const void*)adapters_up_kernel<LOW, W, ALIGNED, KS, LOW_BASE, LOW_OUT>, most, raised) != 0) return -1;
+    if (raise_lds((const void*)adapters_up_kernel<LOW, W, ALIGNED, AT_ONCE, KS, LOW_BASE, LOW_OUT>, most, raised) != 0) return -1;
     const int grid = (int)min(most_tiles(c.n_rows) * slices.strip[slices.n], 4l * gi_compute_units());
-    adapters_up_kernel<LOW, W, ALIGNED, KS, LOW_BASE, LOW_OUT><<<grid, UP_NT, up_lds<LOW>(c.rank), c.stream>>>(c.sums, (const W*)c.b, c.scales, c.list, c.n_listed, c.io, c.n_rows, c.rank,
+    adapters_up_kernel<LOW, W, ALIGNED, AT_ONCE, KS, LOW_BASE, LOW_OUT><<<grid, UP_NT, up_lds<LOW>(c.rank), c.stream>>>(c.sums, (const W*)c.b, c.scales, c.list, c.n_listed, c.io, c.n_rows, c.rank,
                                                                                                                c.n_segments, slices, strip, c.n_adapters);
     return 0;
 }
 
-template <bool LOW, typename W, bool ALIGNED, int KS>
+template <bool LOW, typename W, int AT_ONCE, int KS>
 int up_sized(const Call& c, const Slices& slices, int strip) {
-    if constexpr (!ALIGNED) return up_launch<LOW, W, ALIGNED, KS, false, false>(c, slices, strip);
-    else if (c.io.low_base) return c.io.low_out ? up_launch<LOW, W, ALIGNED, KS, true, true>(c, slices, strip) : up_launch<LOW, W, ALIGNED, KS, true, false>(c, slices, strip);
-    else return c.io.low_out ? up_launch<LOW, W, ALIGNED, KS, false, true>(c, slices, strip) : up_launch<LOW, W, ALIGNED, KS, false, false>(c, slices, strip);
+    if (c.io.low_base) return c.io.low_out ? up_launch<LOW, W, true, AT_ONCE, KS, true, true>(c, slices, strip) : up_launch<LOW, W, true, AT_ONCE, KS, true, false>(c, slices, strip);
+    return c.io.low_out ? up_launch<LOW, W, true, AT_ONCE, KS, false, true>(c, slices, strip) : up_launch<LOW, W, true, AT_ONCE, KS, false, false>(c, slices, strip);
 }
 
 template <bool LOW, typename W>
@@ -852,9 +854,13 @@ int up(const Call& c) {
     // What a wave keeps of B it has for all rows of a tile: of four runs that pays where it takes them all (8,192 rows of 14,336 columns, rank 128: 309 us both ways instead of 526; 4,096 of 4,096, rank 96, 58 instead
     // of 68), not where the waves share the rows out (600 of 4,096, rank 128: 43 us instead of 32; 1,024 of 2,048 in 32 bits, rank 64, 28 instead of 26).
     const bool keeps_four = steps <= 4 && strip > 64;
-    if (c.io.vectors && c.rank % Piece<LOW>::RUN == 0 && aligned(c.b, Piece<LOW>::RUN * sizeof(W)))
-        return steps == 1 ? up_sized<LOW, W, true, 1>(c, slices, strip) : steps == 2 ? up_sized<LOW, W, true, 2>(c, slices, strip) : keeps_four ? up_sized<LOW, W, true, 4>(c, slices, strip) : up_sized<LOW, W, true, 0>(c, slices, strip);
-    return up_sized<LOW, W, false, 0>(c, slices, strip);
+    constexpr int RUN = Piece<LOW>::RUN;
+    if (!c.io.vectors) return up_launch<LOW, W, false, 1, 0, false, false>(c, slices, strip);
+    if (c.rank % RUN == 0 && aligned(c.b, RUN * sizeof(W)))
+        return steps == 1 ? up_sized<LOW, W, RUN, 1>(c, slices, strip) : steps == 2 ? up_sized<LOW, W, RUN, 2>(c, slices, strip) : keeps_four ? up_sized<LOW, W, RUN, 4>(c, slices, strip) : up_sized<LOW, W, RUN, 0>(c, slices, strip);
+    if constexpr (LOW)
+        if (c.rank % 4 == 0 && aligned(c.b, 8)) return steps == 1 ? up_sized<LOW, W, 4, 1>(c, slices, strip) : up_sized<LOW, W, 4, 0>(c, slices, strip);
+    return steps == 1 ? up_sized<LOW, W, 1, 1>(c, slices, strip) : up_sized<LOW, W, 1, 0>(c, slices, strip);
 }
 
 // bfloat16 rows that may be loaded 8 numbers at a time, few enough that loading an adapter once for every row that takes it costs less than tiles that share it.  Only the device knows which rows share:
@@ -863,9 +869,10 @@ int up(const Call& c) {
 // rank 64: 336 MB, 36 against 22) and at fewer where there are more rows (768 of 2,048 onto 2,048: 100 MB, 13.7 against 13.6; 1,024: 134 MB, 18.3 against 14.2).
 bool few_rows(const Call& c) {
     const long loaded = 2l * c.n_rows * c.rank * ((long)c.slices.n * c.width + c.columns);
-    return c.n_rows <= 512 && loaded <= 160 << 20 && c.rank % 8 == 0 && c.width % 8 == 0 && c.ldx % 8 == 0 && aligned(c.x, 16) && aligned(c.a, 16) && aligned(c.b, 16);
+    return c.n_rows <= 512 && loaded <= 160 << 20 && c.width % 8 == 0 && c.ldx % 8 == 0 && aligned(c.x, 16) && aligned(c.a, 16);
 }
 
+template <int N>
 void add_few(const Call& c) {
     const int ranks = c.rank * c.slices.n;
     Slices slices = c.slices;
@@ -875,11 +882,11 @@ void add_few(const Call& c) {
     // One launch takes the host 3 us less than two, and the device as long as two where a workgroup reads 64 KB of A again (1 row of 2,048 onto 2,048 or 8,192, rank 16: 4.7 us either way); at 128 KB 5.7 us
     // against 4.8, at 256 KB 9.0 against 5.4, and 40 rows onto 8,192 columns 6.4 to 7.2 against 5.6.
     if (again <= 64 << 10 && again * strips.x * strips.y <= 16 << 20) {
-        adapters_both_few_kernel<<<strips, 256, 0, c.stream>>>((const bf16_t*)c.x, c.ldx, (const bf16_t*)c.a, (const bf16_t*)c.b, c.scales, c.ids, c.io, c.width, c.rank, slices, c.n_adapters);
+        adapters_both_few_kernel<N><<<strips, 256, 0, c.stream>>>((const bf16_t*)c.x, c.ldx, (const bf16_t*)c.a, (const bf16_t*)c.b, c.scales, c.ids, c.io, c.width, c.rank, slices, c.n_adapters);
         return;
     }
     adapters_down_few_kernel<<<dim3(ranks, c.n_rows), 256, 0, c.stream>>>((const bf16_t*)c.x, c.ldx, (const bf16_t*)c.a, c.ids, c.sums, c.width, ranks, c.n_adapters);
-    adapters_up_few_kernel<<<strips, 256, 0, c.stream>>>(c.sums, (const bf16_t*)c.b, c.scales, c.ids, c.io, c.rank, slices, c.n_adapters);
+    adapters_up_few_kernel<N><<<strips, 256, 0, c.stream>>>(c.sums, (const bf16_t*)c.b, c.scales, c.ids, c.io, c.rank, slices, c.n_adapters);
 }
 
 // In 32 bits only the width says how long a segment is: few rows want many (64 of 14,336 onto 4,096, rank 16: 18.8, 20.0 and 22.8 us with 16, 12 and 8 at most, 21.8 always at 256 numbers), many rows few
@@ -926,7 +933,11 @@ GI_API int gi_adapters_add(const void* x, int x_type, long ldx, const void* a, c
     GI_REQUIRE(c.slices.begin[n_slices] == columns, "adapters_add: the packed projections have %d columns, out has %d", c.slices.begin[n_slices], columns);
     c.io.vectors = fours;
     if (low && few_rows(c)) {
-        add_few(c);
+        const auto brings = [&](int n) { return rank % n == 0 && aligned(b, 2 * n); };
+        if (brings(8)) add_few<8>(c);
+        else if (brings(4)) add_few<4>(c);
+        else if (brings(2)) add_few<2>(c);
+        else add_few<1>(c);
         GI_CHECK_LAUNCH("adapters_add (few rows)");
         return 0;
     }

@@ -75,7 +75,7 @@ def run(c, result=F32, in_place=False):
 SIZES = [(1, 1, 1, 1, 1), (1, 8, 16, 8, 2), (1, 2048, 2048, 16, 3), (3, 65, 33, 5, 2), (7, 256, 129, 16, 8), (16, 512, 512, 32, 4), (17, 264, 200, 24, 5), (33, 520, 264, 1, 33), (64, 1024, 1000, 64, 70),
          (65, 1000, 72, 12, 3), (100, 2049, 130, 7, 9), (129, 640, 384, 128, 3), (250, 328, 520, 130, 4), (515, 4096, 256, 16, 6), (70, 72, 4104, 40, 2), (300, 31, 31, 31, 31),
          (130, 96, 80, 256, 2), (20, 96, 80, 256, 2), (200, 100, 50, 225, 9), (1200, 1536, 1100, 48, 3),
-         (600, 328, 520, 128, 4), (530, 96, 80, 256, 2), (520, 264, 200, 24, 5), (1600, 520, 2100, 104, 3), (1700, 264, 2048, 52, 4), (1025, 1000, 72, 40, 1100)]
+         (600, 328, 520, 128, 4), (530, 96, 80, 256, 2), (520, 264, 200, 24, 5), (40, 264, 201, 4, 9), (7, 1032, 96, 12, 7), (3, 72, 600, 6, 2), (2, 4096, 512, 10, 2), (90, 136, 64, 1, 3), (900, 264, 2048, 12, 4), (700, 520, 1024, 44, 3), (800, 128, 512, 10, 2), (1600, 520, 2100, 104, 3), (1700, 264, 2048, 52, 4), (1025, 1000, 72, 40, 1100)]
 
 
 @pytest.mark.parametrize("n,width,columns,rank,adapters", SIZES)
