@@ -426,6 +426,16 @@ __device__ __forceinline__ floatx4 times(const Held<true>& t, const Run<true>& n
 __device__ __forceinline__ void load_row(Held<false>& t, const float* row, int) { t.v = *reinterpret_cast<const float4*>(row); }
 __device__ __forceinline__ floatx4 times(const Held<false>& t, const Run<false>& n, floatx4 sum) { return times(t.v, n.v, sum); }
 
+// A strip's workgroup first makes its rows' sums, so strips are as long as leaves every compute unit (of 256) two or three workgroups, by the number of tiles that the way down has counted
+// (600 rows with adapters of their own, 4,096 columns, rank 32: 135 us both ways; with strips for as many rows in whole tiles 466).  Aimed at 350 and 700
+// workgroups, 1,024 rows of 2,048 32-bit columns and rank 64 take 36.4 and 29.1 us both ways, 2,048 rows of 2,048 columns and rank 32 19.1 either way.  All four waves have columns of their own, 256 a step of the
+// strip (strips of other multiples of 64: 531 rows 31.0 us instead of 26.5), or, where there are no 256 for each, rows of the same 64 (301 rows of 1,024 in 32 bits: 13.0 us instead of 14.5).  Strips end at 512
+// columns (8,192 rows of 14,336 columns: 236 us at 256, 219 at 512, 239 at 1,024).
+__host__ __device__ inline int strip_bits(int n_tiles, int columns) {          // 64, 256 or 512 columns
+    const long work = (long)n_tiles * columns;
+    return work <= 700l * 64 ? 6 : work <= 700l * 256 ? 8 : 9;
+}
+
 // A tile and a strip of columns.  The workgroup first adds up its rows' sums over the segments and keeps them in LDS: where B is bfloat16 and so multiplied, in PIECES, which lose nothing of their 24 bits.
 // Then a wave takes 64 columns at a time and of them 16 rows after 16 rows, with the columns' runs of B in registers throughout (loaded, they lie as the matrix cores want them, every lane in another
 // row of B: 64 accesses to the first-level cache a load); where the strip is no wider than 64 columns the waves share out the rows.  In the product D = M N the rows are M's and the columns
@@ -436,7 +446,7 @@ __device__ __forceinline__ floatx4 times(const Held<false>& t, const Run<false>&
 // rank 10, 10.6.  Asking for a whole tile's base at once instead of 16 rows ahead makes it no faster: 4,096 rows of 4,096 both ways 50 us instead of 47, with 256 registers instead of 141.
 template <bool LOW, typename W, bool ALIGNED, int AT_ONCE, int KS, bool LOW_BASE, bool LOW_OUT>
 __global__ __launch_bounds__(UP_NT) void adapters_up_kernel(const float* __restrict__ sums, const W* __restrict__ b, const float* __restrict__ scales, const Tile* __restrict__ list,
-                                                            const int* __restrict__ n_listed, Rows io, int n_rows, int rank, int n_segments, Slices slices, int strip_columns, int n_adapters) {
+                                                            const int* __restrict__ n_listed, Rows io, int n_rows, int rank, int n_segments, Slices slices, int n_adapters) {
     typedef Piece<LOW> P;
     typedef typename P::T T;
     extern __shared__ __align__(16) unsigned char room[];
@@ -444,13 +454,15 @@ __global__ __launch_bounds__(UP_NT) void adapters_up_kernel(const float* __restr
     const int padded = (rank + DEPTH - 1) / DEPTH * DEPTH, pitch = padded + P::RUN, apart = TILE * pitch;       // (rows of LDS a run further apart than a multiple of all banks)
     T* held = (T*)room;                                    // [pieces][TILE][pitch], the largest piece first
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, at = lane & 15, group = lane >> 4;
-    const int columns = slices.begin[slices.n], ranks = rank * slices.n, n_strips = slices.strip[slices.n];
-    const long n_items = (long)*n_listed * n_strips;
+    const int columns = slices.begin[slices.n], ranks = rank * slices.n, n_tiles = *n_listed, bits = strip_bits(n_tiles, columns), strip_columns = 1 << bits;
+    auto strips_of = [&](int s) { return (slices.begin[s + 1] - slices.begin[s] + strip_columns - 1) >> bits; };
+    int n_strips = 0;
+    for (int s = 0; s < slices.n; ++s) n_strips += strips_of(s);
+    const long n_items = (long)n_tiles * n_strips;
     for (long item = blockIdx.x; item < n_items; item += gridDim.x) {
-        const int strip = (int)(item % n_strips);
-        int s = 0;
-        while (s + 1 < slices.n && strip >= slices.strip[s + 1]) ++s;
-        const int begin = slices.begin[s] + (strip - slices.strip[s]) * strip_columns, end = min(slices.begin[s + 1], begin + strip_columns);
+        int strip = (int)(item % n_strips), s = 0;
+        for (; s + 1 < slices.n && strip >= strips_of(s); ++s) strip -= strips_of(s);
+        const int begin = slices.begin[s] + strip * strip_columns, end = min(slices.begin[s + 1], begin + strip_columns);
         const Tile tile = list[item / n_strips];
         const int first_row = tile.first, rows = tile.rows, e = tile.id;
         if (e < 0 || e >= n_adapters) {                    // rows without an adapter
@@ -824,43 +836,35 @@ template <bool LOW> constexpr int up_lds(int rank) {
 }
 
 template <bool LOW, typename W, bool ALIGNED, int AT_ONCE, int KS, bool LOW_BASE, bool LOW_OUT>
-int up_launch(const Call& c, const Slices& slices, int strip) {
+int up_launch(const Call& c) {
     static bool raised[MAX_DEVICES] = {};
     constexpr int most = up_lds<LOW>(MAX_RANK);
     if (raise_lds((const void*)adapters_up_kernel<LOW, W, ALIGNED, AT_ONCE, KS, LOW_BASE, LOW_OUT>, most, raised) != 0) return -1;
-    const int grid = (int)min(most_tiles(c.n_rows) * slices.strip[slices.n], 4l * gi_compute_units());
+    const int grid = (int)min((long)c.n_rows * ((c.columns + 63) / 64 + c.slices.n), 4l * gi_compute_units());
     adapters_up_kernel<LOW, W, ALIGNED, AT_ONCE, KS, LOW_BASE, LOW_OUT><<<grid, UP_NT, up_lds<LOW>(c.rank), c.stream>>>(c.sums, (const W*)c.b, c.scales, c.list, c.n_listed, c.io, c.n_rows, c.rank,
-                                                                                                               c.n_segments, slices, strip, c.n_adapters);
+                                                                                                               c.n_segments, c.slices, c.n_adapters);
     return 0;
 }
 
 template <bool LOW, typename W, int AT_ONCE, int KS>
-int up_sized(const Call& c, const Slices& slices, int strip) {
-    if (c.io.low_base) return c.io.low_out ? up_launch<LOW, W, true, AT_ONCE, KS, true, true>(c, slices, strip) : up_launch<LOW, W, true, AT_ONCE, KS, true, false>(c, slices, strip);
-    return c.io.low_out ? up_launch<LOW, W, true, AT_ONCE, KS, false, true>(c, slices, strip) : up_launch<LOW, W, true, AT_ONCE, KS, false, false>(c, slices, strip);
+int up_sized(const Call& c) {
+    if (c.io.low_base) return c.io.low_out ? up_launch<LOW, W, true, AT_ONCE, KS, true, true>(c) : up_launch<LOW, W, true, AT_ONCE, KS, true, false>(c);
+    return c.io.low_out ? up_launch<LOW, W, true, AT_ONCE, KS, false, true>(c) : up_launch<LOW, W, true, AT_ONCE, KS, false, false>(c);
 }
 
 template <bool LOW, typename W>
 int up(const Call& c) {
-    // A strip's workgroup first makes its rows' sums, so strips are as long as leaves every compute unit (of 256) two or three workgroups: aimed at 350 and 700 of them, 1,024 rows of 2,048 32-bit columns and
-    // rank 64 take 36.4 and 29.1 us both ways, 2,048 rows of 2,048 columns and rank 32 19.1 either way.  All four waves have columns of their own, 256 a step of the strip (strips of other multiples of 64:
-    // 531 rows 31.0 us instead of 26.5), or, where there are no 256 for each, rows of the same 64 (301 rows of 1,024 in 32 bits: 13.0 us instead of 14.5).  Strips end at 512 columns (8,192 rows of 14,336
-    // columns: 236 us at 256, 219 at 512, 239 at 1,024).
-    const long even = usual_tiles(c.n_rows) * c.columns / 700;
     const int steps = (c.rank + Piece<LOW>::BLOCK / 2 - 1) / (Piece<LOW>::BLOCK / 2);
-    const int strip = even <= 64 ? 64 : (int)min((even + 255) / 256 * 256, 512l);
-    Slices slices = c.slices;
-    for (int s = 0; s < slices.n; ++s) slices.strip[s + 1] = slices.strip[s] + (slices.begin[s + 1] - slices.begin[s] + strip - 1) / strip;
     // What a wave keeps of B it has for all rows of a tile: of four runs that pays where it takes them all (8,192 rows of 14,336 columns, rank 128: 309 us both ways instead of 526; 4,096 of 4,096, rank 96, 58 instead
     // of 68), not where the waves share the rows out (600 of 4,096, rank 128: 43 us instead of 32; 1,024 of 2,048 in 32 bits, rank 64, 28 instead of 26).
-    const bool keeps_four = steps <= 4 && strip > 64;
+    const bool keeps_four = steps <= 4 && strip_bits((int)usual_tiles(c.n_rows), c.columns) > 6;       // (then the strips there are, of at least as many tiles, are no shorter)
     constexpr int RUN = Piece<LOW>::RUN;
-    if (!c.io.vectors) return up_launch<LOW, W, false, 1, 0, false, false>(c, slices, strip);
+    if (!c.io.vectors) return up_launch<LOW, W, false, 1, 0, false, false>(c);
     if (c.rank % RUN == 0 && aligned(c.b, RUN * sizeof(W)))
-        return steps == 1 ? up_sized<LOW, W, RUN, 1>(c, slices, strip) : steps == 2 ? up_sized<LOW, W, RUN, 2>(c, slices, strip) : keeps_four ? up_sized<LOW, W, RUN, 4>(c, slices, strip) : up_sized<LOW, W, RUN, 0>(c, slices, strip);
+        return steps == 1 ? up_sized<LOW, W, RUN, 1>(c) : steps == 2 ? up_sized<LOW, W, RUN, 2>(c) : keeps_four ? up_sized<LOW, W, RUN, 4>(c) : up_sized<LOW, W, RUN, 0>(c);
     if constexpr (LOW)
-        if (c.rank % 4 == 0 && aligned(c.b, 8)) return steps == 1 ? up_sized<LOW, W, 4, 1>(c, slices, strip) : up_sized<LOW, W, 4, 0>(c, slices, strip);
-    return steps == 1 ? up_sized<LOW, W, 1, 1>(c, slices, strip) : up_sized<LOW, W, 1, 0>(c, slices, strip);
+        if (c.rank % 4 == 0 && aligned(c.b, 8)) return steps == 1 ? up_sized<LOW, W, 4, 1>(c) : up_sized<LOW, W, 4, 0>(c);
+    return steps == 1 ? up_sized<LOW, W, 1, 1>(c) : up_sized<LOW, W, 1, 0>(c);
 }
 
 // bfloat16 rows that may be loaded 8 numbers at a time, few enough that loading an adapter once for every row that takes it costs less than tiles that share it.  Only the device knows which rows share:
