@@ -868,9 +868,9 @@ int up(const Call& c) {
 }
 
 // bfloat16 rows that may be loaded 8 numbers at a time, few enough that loading an adapter once for every row that takes it costs less than tiles that share it.  Only the device knows which rows share:
-// with an adapter a row tiles lose by far (64 rows of 4,096 onto 4,096, rank 32: 10.7 us against 54; 256: 31 against 188; 512 of 2,048 onto 2,048, rank 16: 17.5 against 135), with one for all the two meet
-// at some 150 MB loaded (256 of 4,096 onto 4,096: 134 MB, 13.4 us against 15.3; 512 of 2,048 onto 2,048: 67 MB, 10.5 against 12.6; 512 onto 8,192: 168 MB, 18.7 against 15.3; 256 of 8,192 onto 2,048,
-// rank 64: 336 MB, 36 against 22) and at fewer where there are more rows (768 of 2,048 onto 2,048: 100 MB, 13.7 against 13.6; 1,024: 134 MB, 18.3 against 14.2).
+// with an adapter a row tiles lose (64 rows of 4,096 onto 4,096, rank 32: 10.5 us against 15.5; 256: 31 against 45; 512 of 2,048 onto 2,048, rank 16: 17 against 46), with one for all the two meet at some
+// 150 MB loaded (256 of 4,096 onto 4,096: 134 MB, 12.5 us against 13.5; 128 of 8,192 onto 2,048, rank 64: 168 MB, 19.1 against 19.6; 512 of 2,048 onto 8,192, rank 16: as many, 17.8 against 14.7; 256 of 8,192 onto
+// 2,048: 336 MB, 36 against 20, and 102 against 76 with an adapter each) and at fewer where there are more rows (768 of 2,048 onto 2,048: 100 MB, 12.6 against 13.0; 1,024: 134 MB, 16.9 against 13.7).
 bool few_rows(const Call& c) {
     const long loaded = 2l * c.n_rows * c.rank * ((long)c.slices.n * c.width + c.columns);
     return c.n_rows <= 512 && loaded <= 160 << 20 && c.width % 8 == 0 && c.ldx % 8 == 0 && aligned(c.x, 16) && aligned(c.a, 16);
@@ -895,10 +895,11 @@ void add_few(const Call& c) {
 
 // In 32 bits only the width says how long a segment is: few rows want many (64 of 14,336 onto 4,096, rank 16: 18.8, 20.0 and 22.8 us with 16, 12 and 8 at most, 21.8 always at 256 numbers), many rows few
 // (2,048 of 4,096: 30.3, 26.3, 26.4 and 30.4 us; 4,096 of 14,336, rank 64: 180, 169, 155 and 246).  Otherwise there are as many as give every compute unit (of 256) a workgroup: the sums of every segment are written and read again, and with two workgroups a unit
-// the way down gains less than the way up loses (4,096 rows of 14,336, rank 64, both ways: 84 us aimed at 500 workgroups, 79 at 250, 114 at 125; 531 rows of 4,096, rank 3 * 24: 24.7 at 500, 20.3 at 250).
+// the way down gains less than the way up loses (4,096 rows of 14,336, rank 64, both ways: 84 us aimed at 500 workgroups, 79 at 250, 114 at 125; 531 rows of 4,096, rank 3 * 24: 24.7 at 500, 20.3 at 250).  Nor
+// more than 8: 256 rows of 8,192, rank 64, take 29.2, 22.0, 20.8 and 20.5 us with any number, 16, 12 and 8 at most, 64 of 4,096, rank 32, with an adapter each 19.1, 19.0, 15.5 and 15.5.
 int segment_of(int n_rows, int width, int ranks, bool low) {
     if (!low) return (width + EXACT_SEGMENTS * SEGMENT - 1) / (EXACT_SEGMENTS * SEGMENT) * SEGMENT;
-    const long segments = max(250 / (usual_tiles(n_rows) * ((ranks + 63) / 64)), 1l);
+    const long segments = min(max(250 / (usual_tiles(n_rows) * ((ranks + 63) / 64)), 1l), 8l);
     return (int)(((width + segments - 1) / segments + SEGMENT - 1) / SEGMENT * SEGMENT);
 }
 
