@@ -26,6 +26,12 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float floatx4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) void* lds_ptr_t;
 
+// Numbers side by side that begin wherever one of their kind may: memory takes 4 to 16 bytes at once from any place.
+struct __attribute__((packed, aligned(2))) Low8 { uint32_t x, y, z, w; };
+struct __attribute__((packed, aligned(2))) Low4 { uint32_t x, y; };
+struct __attribute__((packed, aligned(2))) Low2 { uint32_t x; };
+struct __attribute__((packed, aligned(4))) High4 { float x, y, z, w; };
+
 struct Slices {                             // of the columns: slice s begins at begin[s] and reads block s of the ranks; its strips begin at strip[s]
     int n;
     int begin[MAX_SLICES + 1];
@@ -111,6 +117,29 @@ template <int AT_ONCE, typename T>
 __device__ __forceinline__ void load_piece(Piece<false>& p, const T* __restrict__ row, int k, int end, int group) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) p.v[h] = load_run_f32<AT_ONCE>(row, k + 16 * h + 4 * group, end);
+}
+
+// A whole piece, from any place.
+__device__ __forceinline__ void load_whole(Piece<true>& p, const bf16_t* __restrict__ row, int k, int group) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const Low8 v = *reinterpret_cast<const Low8*>(row + k + 32 * h + 8 * group);
+        p.v[h] = uint4{v.x, v.y, v.z, v.w};
+    }
+}
+__device__ __forceinline__ void load_whole(Piece<false>& p, const float* __restrict__ row, int k, int group) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const High4 v = *reinterpret_cast<const High4*>(row + k + 16 * h + 4 * group);
+        p.v[h] = float4{v.x, v.y, v.z, v.w};
+    }
+}
+__device__ __forceinline__ void load_whole(Piece<false>& p, const bf16_t* __restrict__ row, int k, int group) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const Low4 v = *reinterpret_cast<const Low4*>(row + k + 16 * h + 4 * group);
+        p.v[h] = float4{__uint_as_float(v.x << 16), __uint_as_float(v.x & 0xffff0000u), __uint_as_float(v.y << 16), __uint_as_float(v.y & 0xffff0000u)};
+    }
 }
 
 // The tiles of a batch, counted by every workgroup: a tile begins at every 64th row and where a row's adapter is not its neighbour's.
@@ -329,7 +358,7 @@ __global__ __launch_bounds__(64 * WAVES) void adapters_down_kernel(const typenam
 
 // Operands of two types, or rows that do not begin at 16 bytes: through registers, in the same order.  2,048 rows of 4,096 onto 4,096, rank 16, both ways: two types 30 us, as both of 32 bits; rows at odd places
 // 63 (32 bits, 30 at even ones) and 78 (bfloat16, 25): every number is a load of its own.
-template <bool LOW, typename X, typename W, bool ALIGNED>
+template <bool LOW, typename X, typename W>
 __global__ __launch_bounds__(64 * ANY_WAVES) void adapters_down_any_kernel(const X* __restrict__ x, const W* __restrict__ a, const int* __restrict__ ids, float* __restrict__ sums, Down d) {
     typedef Piece<LOW> P;
     constexpr int MT = 2;
@@ -361,15 +390,27 @@ __global__ __launch_bounds__(64 * ANY_WAVES) void adapters_down_any_kernel(const
         for (int j = 0; j < 4; ++j)
 #pragma unroll
             for (int i = 0; i < MT; ++i) sum[j][i] = floatx4{0.f, 0.f, 0.f, 0.f};
-        for (int k = begin + wave * P::BLOCK; k < end; k += P::BLOCK * ANY_WAVES) {
+        int k = begin + wave * P::BLOCK;
+        for (; k + P::BLOCK <= end; k += P::BLOCK * ANY_WAVES) {
+            P ap[MT], xp[4];
+#pragma unroll
+            for (int i = 0; i < MT; ++i) load_whole(ap[i], ar[i], k, group);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) load_whole(xp[j], xr[j], k, group);             // (rows behind the last are that one)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int i = 0; i < MT; ++i) sum[j][i] = times(ap[i], xp[j], sum[j][i]);
+        }
+        if (k < end) {
             P ap[MT];
 #pragma unroll
-            for (int i = 0; i < MT; ++i) load_piece<ALIGNED ? P::RUN : 1>(ap[i], ar[i], k, end, group);
+            for (int i = 0; i < MT; ++i) load_piece<1>(ap[i], ar[i], k, end, group);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 if (16 * j >= rows) break;
                 P xp;
-                load_piece<ALIGNED ? P::RUN : 1>(xp, xr[j], k, end, group);
+                load_piece<1>(xp, xr[j], k, end, group);
 #pragma unroll
                 for (int i = 0; i < MT; ++i) sum[j][i] = times(ap[i], xp, sum[j][i]);
             }
@@ -381,8 +422,11 @@ __global__ __launch_bounds__(64 * ANY_WAVES) void adapters_down_any_kernel(const
 // ------------------------------------------------------------------ up, in tiles
 // 4 numbers of base, as they lie in memory and as numbers, and of out.
 __device__ __forceinline__ uint4 raw4(const unsigned char* base, uint32_t i, bool low) {
-    if (!low) return *reinterpret_cast<const uint4*>(base + 4 * i);
-    const uint2 v = *reinterpret_cast<const uint2*>(base + 2 * i);
+    if (!low) {
+        const High4 v = *reinterpret_cast<const High4*>(base + 4 * i);
+        return uint4{__float_as_uint(v.x), __float_as_uint(v.y), __float_as_uint(v.z), __float_as_uint(v.w)};
+    }
+    const Low4 v = *reinterpret_cast<const Low4*>(base + 2 * i);
     return uint4{v.x, v.y, 0u, 0u};
 }
 __device__ __forceinline__ floatx4 numbers4(uint4 v, bool low) {
@@ -390,8 +434,8 @@ __device__ __forceinline__ floatx4 numbers4(uint4 v, bool low) {
     return floatx4{__uint_as_float(v.x << 16), __uint_as_float(v.x & 0xffff0000u), __uint_as_float(v.y << 16), __uint_as_float(v.y & 0xffff0000u)};
 }
 __device__ __forceinline__ void store4(unsigned char* out, uint32_t i, floatx4 v, bool low) {
-    if (low) *reinterpret_cast<uint2*>(out + 2 * i) = uint2{f32x2_to_bf16x2(v[0], v[1]), f32x2_to_bf16x2(v[2], v[3])};
-    else *reinterpret_cast<floatx4*>(out + 4 * i) = v;
+    if (low) *reinterpret_cast<Low4*>(out + 2 * i) = Low4{f32x2_to_bf16x2(v[0], v[1]), f32x2_to_bf16x2(v[2], v[3])};
+    else *reinterpret_cast<High4*>(out + 4 * i) = High4{v[0], v[1], v[2], v[3]};
 }
 __device__ __forceinline__ float number1(const void* base, size_t i, bool low) { return low ? load_f32((const bf16_t*)base, i) : load_f32((const float*)base, i); }
 __device__ __forceinline__ void store1(void* out, size_t i, float v, bool low) { low ? store_f32((bf16_t*)out, i, v) : store_f32((float*)out, i, v); }
@@ -400,7 +444,7 @@ struct Rows {                               // base and out
     const void* base;
     void* out;
     long ldb, ldo;
-    bool low_base, low_out, vectors;        // bfloat16; columns come in fours that may be loaded and stored at once
+    bool low_base, low_out;                 // bfloat16
 };
 
 constexpr int PIECES = 3;                   // bfloat16 numbers that hold a 32-bit one: each the first 8 bits of what the ones before leave of its 24, cut off, so that none passes the number
@@ -440,11 +484,11 @@ __host__ __device__ inline int strip_bits(int n_tiles, int columns) {          /
 // Then a wave takes 64 columns at a time and of them 16 rows after 16 rows, with the columns' runs of B in registers throughout (loaded, they lie as the matrix cores want them, every lane in another
 // row of B: 64 accesses to the first-level cache a load); where the strip is no wider than 64 columns the waves share out the rows.  In the product D = M N the rows are M's and the columns
 // N's: number n of the four products of a step has columns 4 l + n, l = 0 .. 15, so that a lane ends with four neighbours and sixteen lanes with whole lines of base and out.  As on the way down no
-// row's values meet another's.  ALIGNED: fours of columns of base and out may be loaded at once, and columns come in fours.  AT_ONCE: numbers of B that one load brings.  KS: runs of ranks that a wave keeps; 0 for any number,
+// row's values meet another's.  FOURS: a projection has four columns or more, so base and out come four at a time.  AT_ONCE: numbers of B that one load brings.  KS: runs of ranks that a wave keeps; 0 for any number,
 // loaded again for every 16 rows (8,192 rows of 14,336 columns, rank 16: 239 us kept, 272 loaded again).  LOW_BASE, LOW_OUT: of aligned ones whether they are bfloat16 (a branch on it where they are loaded would have every load waited for); `io` says it of others.
 // 4,096 rows of 4,096 32-bit columns, rank 64: 41 us for the 134 MB of base and out (a copy of as much takes 25); 531 of 6,144, rank 24, onto bfloat16 10.3; 2,048 of 2,048, rank 32, 9.4; 301 of 2,048 in 32 bits,
 // rank 10, 10.6.  Asking for a whole tile's base at once instead of 16 rows ahead makes it no faster: 4,096 rows of 4,096 both ways 50 us instead of 47, with 256 registers instead of 141.
-template <bool LOW, typename W, bool ALIGNED, int AT_ONCE, int KS, bool LOW_BASE, bool LOW_OUT>
+template <bool LOW, typename W, bool FOURS, int AT_ONCE, int KS, bool LOW_BASE, bool LOW_OUT>
 __global__ __launch_bounds__(UP_NT) void adapters_up_kernel(const float* __restrict__ sums, const W* __restrict__ b, const float* __restrict__ scales, const Tile* __restrict__ list,
                                                             const int* __restrict__ n_listed, Rows io, int n_rows, int rank, int n_segments, Slices slices, int n_adapters) {
     typedef Piece<LOW> P;
@@ -487,7 +531,7 @@ __global__ __launch_bounds__(UP_NT) void adapters_up_kernel(const float* __restr
         // Rows behind the last are taken as that one throughout, and columns behind the end as the last four: their lanes load and store what the lanes that own them do, at the same time.  Without a branch
         // around any store the wait for a load counts what was asked for behind it, and no load waits for a store's end.
         auto ask_base = [&](int c0, int j) {
-            if constexpr (ALIGNED)
+            if constexpr (FOURS)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) next[i] = raw4(base_at, (uint32_t)(min(16 * j + 4 * group + i, rows - 1) * (int)io.ldb + min(c0 + 4 * at, end - 4)), LOW_BASE);
         };
@@ -557,7 +601,7 @@ __global__ __launch_bounds__(UP_NT) void adapters_up_kernel(const float* __restr
         __syncthreads();
         if (idle) continue;
         while (true) {
-            const int col = ALIGNED ? min(c0 + 4 * at, end - 4) : c0 + 4 * at;
+            const int col = FOURS ? min(c0 + 4 * at, end - 4) : c0 + 4 * at;
 #pragma unroll 1
             for (int j = j0; j <= last_j; j += j_step) {
                 uint4 was[4];
@@ -579,7 +623,7 @@ __global__ __launch_bounds__(UP_NT) void adapters_up_kernel(const float* __restr
                 } else {
                     for (int k = 0; k < padded; k += DEPTH) {
 #pragma unroll
-                        for (int n = 0; n < 4; ++n) load_b<AT_ONCE>(br[0][n], be + (size_t)(ALIGNED ? col + n : min(col + n, end - 1)) * rank, k + P::RUN * group, rank);
+                        for (int n = 0; n < 4; ++n) load_b<AT_ONCE>(br[0][n], be + (size_t)(FOURS ? col + n : min(col + n, end - 1)) * rank, k + P::RUN * group, rank);
                         load_row(t, row + k, apart);
 #pragma unroll
                         for (int n = 0; n < 4; ++n) sum[n] = times(t, br[0][n], sum[n]);
@@ -588,9 +632,16 @@ __global__ __launch_bounds__(UP_NT) void adapters_up_kernel(const float* __restr
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const int r = 16 * j + 4 * group + i;
-                    if constexpr (ALIGNED) {
+                    if constexpr (FOURS) {
                         const uint32_t to = (uint32_t)(min(r, rows - 1) * (int)io.ldo + col);
-                        store4(out_at, to, numbers4(was[i], LOW_BASE) + floatx4{sum[0][i], sum[1][i], sum[2][i], sum[3][i]}, LOW_OUT);
+                        const floatx4 v = numbers4(was[i], LOW_BASE) + floatx4{sum[0][i], sum[1][i], sum[2][i], sum[3][i]};
+                        if (end - c0 >= 4) {
+                            store4(out_at, to, v, LOW_OUT);
+                        } else {                           // fewer are left: of the last four those before c0 are another wave's, which may have stored them already
+#pragma unroll
+                            for (int n = 0; n < 4; ++n)
+                                if (col + n >= c0) store1(out_at, to + n, v[n], LOW_OUT);
+                        }
                     } else if (r < rows) {
                         const uint32_t to = (uint32_t)(r * (int)io.ldo + col);
 #pragma unroll
@@ -608,6 +659,12 @@ __global__ __launch_bounds__(UP_NT) void adapters_up_kernel(const float* __restr
 }
 
 // ------------------------------------------------------------------ a few rows
+template <int N> struct Some;               // N bfloat16 numbers, loaded at once
+template <> struct Some<8> { Low8 v; __device__ float operator[](int i) const { const uint32_t w[4] = {v.x, v.y, v.z, v.w}; return __uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16); } };
+template <> struct Some<4> { Low4 v; __device__ float operator[](int i) const { const uint32_t w[2] = {v.x, v.y}; return __uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16); } };
+template <> struct Some<2> { Low2 v; __device__ float operator[](int i) const { return __uint_as_float(i & 1 ? v.x & 0xffff0000u : v.x << 16); } };
+template <> struct Some<1> { bf16_t v; __device__ float operator[](int) const { return bf16_to_f32(v); } };
+
 // Decoded rows, as a rule each with an adapter of its own: nothing is shared, the adapters' bytes bound it, and what counts is that all of them are asked for at once and few waits
 // follow one another.  Every row is taken alone, without tiles.  Down: a workgroup has a row and one rank, its threads share out the width.  (With four ranks, which share the row's numbers, 8 rows of
 // 4,096 onto 4,096, rank 32, take 6.2 us instead of 5.6, 128 rows 18.8 instead of 18.0; rows that share an adapter of 2 MB gain a tenth.)  64 rows of 4,096, rank 16: 4.1 us.
@@ -619,16 +676,13 @@ __global__ __launch_bounds__(256) void adapters_down_few_kernel(const bf16_t* __
     if (e < 0 || e >= n_adapters) return;
     const bf16_t* xr = x + (size_t)row * ldx;
     const bf16_t* ar = a + ((size_t)e * ranks + blockIdx.x) * width;
-    float sum = 0.f;
+    const int eights = width & ~7;
+    float sum = tid < width - eights ? bf16_to_f32(xr[eights + tid]) * bf16_to_f32(ar[eights + tid]) : 0.f;
 #pragma unroll 2
-    for (int k = 8 * tid; k < width; k += 2048) {
-        const uint4 xv = *reinterpret_cast<const uint4*>(xr + k), av = *reinterpret_cast<const uint4*>(ar + k);
-        const uint32_t xw[4] = {xv.x, xv.y, xv.z, xv.w}, aw[4] = {av.x, av.y, av.z, av.w};
+    for (int k = 8 * tid; k < eights; k += 2048) {
+        const Some<8> xv = *reinterpret_cast<const Some<8>*>(xr + k), av = *reinterpret_cast<const Some<8>*>(ar + k);
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            sum = fmaf(__uint_as_float(xw[u] << 16), __uint_as_float(aw[u] << 16), sum);
-            sum = fmaf(__uint_as_float(xw[u] & 0xffff0000u), __uint_as_float(aw[u] & 0xffff0000u), sum);
-        }
+        for (int u = 0; u < 8; ++u) sum = fmaf(xv[u], av[u], sum);
     }
     sum = over_wave(sum, Add());
     if ((tid & 63) == 0) red[tid >> 6] = sum;
@@ -638,12 +692,6 @@ __global__ __launch_bounds__(256) void adapters_down_few_kernel(const bf16_t* __
 
 // Up: a thread has FEW_COLUMNS columns, 256 apart, of a row; the row's sums come as scalars.  64 rows of 14,336, rank 16: 8.1 us for 37 MB (4.5 TB/s).
 constexpr int FEW_COLUMNS = 2;
-template <int N> struct Some;               // N bfloat16 numbers, loaded at once
-template <> struct Some<8> { uint4 v; __device__ float operator[](int i) const { const uint32_t w[4] = {v.x, v.y, v.z, v.w}; return __uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16); } };
-template <> struct Some<4> { uint2 v; __device__ float operator[](int i) const { const uint32_t w[2] = {v.x, v.y}; return __uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16); } };
-template <> struct Some<2> { uint32_t v; __device__ float operator[](int i) const { return __uint_as_float(i & 1 ? v & 0xffff0000u : v << 16); } };
-template <> struct Some<1> { bf16_t v; __device__ float operator[](int) const { return bf16_to_f32(v); } };
-
 template <int N>                            // ranks of a column that one load brings
 __global__ __launch_bounds__(256) void adapters_up_few_kernel(const float* __restrict__ sums, const bf16_t* __restrict__ b, const float* __restrict__ scales, const int* __restrict__ ids,
                                                               Rows io, int rank, Slices slices, int n_adapters) {
@@ -715,24 +763,24 @@ __global__ __launch_bounds__(256) void adapters_both_few_kernel(const bf16_t* __
         const float scale = scales != nullptr ? scales[e] : 1.f;
         const bf16_t* xr = x + (size_t)row * ldx;
         const bf16_t* ae = a + ((size_t)e * slices.n + s) * rank * width;
+        const int eights = width & ~7;
         for (int k0 = 0; k0 < rank; k0 += 16) {            // four sums of a wave at a time
-            float four[4] = {0.f, 0.f, 0.f, 0.f};
+            const bf16_t* ar[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) ar[i] = ae + (size_t)min(k0 + wave + 4 * i, rank - 1) * width;
+            float four[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) four[i] = lane < width - eights ? bf16_to_f32(xr[eights + lane]) * bf16_to_f32(ar[i][eights + lane]) : 0.f;
 #pragma unroll 2
-            for (int k = 8 * lane; k < width; k += 512) {
-                const uint4 xv = *reinterpret_cast<const uint4*>(xr + k);
-                uint4 av[4];
+            for (int k = 8 * lane; k < eights; k += 512) {
+                const Some<8> xv = *reinterpret_cast<const Some<8>*>(xr + k);
+                Some<8> av[4];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) av[i] = *reinterpret_cast<const uint4*>(ae + (size_t)min(k0 + wave + 4 * i, rank - 1) * width + k);
-                const uint32_t xw[4] = {xv.x, xv.y, xv.z, xv.w};
+                for (int i = 0; i < 4; ++i) av[i] = *reinterpret_cast<const Some<8>*>(ar[i] + k);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const uint32_t aw[4] = {av[i].x, av[i].y, av[i].z, av[i].w};
+                for (int i = 0; i < 4; ++i)
 #pragma unroll
-                    for (int u = 0; u < 4; ++u) {
-                        four[i] = fmaf(__uint_as_float(xw[u] << 16), __uint_as_float(aw[u] << 16), four[i]);
-                        four[i] = fmaf(__uint_as_float(xw[u] & 0xffff0000u), __uint_as_float(aw[u] & 0xffff0000u), four[i]);
-                    }
-                }
+                    for (int u = 0; u < 8; ++u) four[i] = fmaf(xv[u], av[i][u], four[i]);
             }
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -762,6 +810,7 @@ struct Call {
     const void* x; long ldx; const void* a; const void* b; const int* ids; const float* scales; Rows io; float* sums; Tile* list; int* n_listed;
     int n_rows, width, columns, rank, n_adapters, segment, n_segments;
     Slices slices;
+    bool fours;                             // every projection has four columns or more
     hipStream_t stream;
 };
 
@@ -819,13 +868,7 @@ int down(const Call& c) {
     }
     d.n_parts = d.n_segments * ((ranks + 31) / 32);
     const int grid = (int)min(most_tiles(c.n_rows) * d.n_parts, (long)gi_compute_units() * 8);
-    if constexpr (!std::is_same<X, W>::value) {
-        if (even) {
-            adapters_down_any_kernel<LOW, X, W, true><<<grid, 64 * ANY_WAVES, 0, c.stream>>>((const X*)c.x, (const W*)c.a, c.ids, c.sums, d);
-            return 0;
-        }
-    }
-    adapters_down_any_kernel<LOW, X, W, false><<<grid, 64 * ANY_WAVES, 0, c.stream>>>((const X*)c.x, (const W*)c.a, c.ids, c.sums, d);
+    adapters_down_any_kernel<LOW, X, W><<<grid, 64 * ANY_WAVES, 0, c.stream>>>((const X*)c.x, (const W*)c.a, c.ids, c.sums, d);
     return 0;
 }
 
@@ -835,13 +878,13 @@ template <bool LOW> constexpr int up_lds(int rank) {
     return TILE * ((rank + DEPTH - 1) / DEPTH * DEPTH + Piece<LOW>::RUN) * (LOW ? 2 * PIECES : 4);
 }
 
-template <bool LOW, typename W, bool ALIGNED, int AT_ONCE, int KS, bool LOW_BASE, bool LOW_OUT>
+template <bool LOW, typename W, bool FOURS, int AT_ONCE, int KS, bool LOW_BASE, bool LOW_OUT>
 int up_launch(const Call& c) {
     static bool raised[MAX_DEVICES] = {};
     constexpr int most = up_lds<LOW>(MAX_RANK);
-    if (raise_lds((const void*)adapters_up_kernel<LOW, W, ALIGNED, AT_ONCE, KS, LOW_BASE, LOW_OUT>, most, raised) != 0) return -1;
+    if (raise_lds((const void*)adapters_up_kernel<LOW, W, FOURS, AT_ONCE, KS, LOW_BASE, LOW_OUT>, most, raised) != 0) return -1;
     const int grid = (int)min((long)c.n_rows * ((c.columns + 63) / 64 + c.slices.n), 4l * gi_compute_units());
-    adapters_up_kernel<LOW, W, ALIGNED, AT_ONCE, KS, LOW_BASE, LOW_OUT><<<grid, UP_NT, up_lds<LOW>(c.rank), c.stream>>>(c.sums, (const W*)c.b, c.scales, c.list, c.n_listed, c.io, c.n_rows, c.rank,
+    adapters_up_kernel<LOW, W, FOURS, AT_ONCE, KS, LOW_BASE, LOW_OUT><<<grid, UP_NT, up_lds<LOW>(c.rank), c.stream>>>(c.sums, (const W*)c.b, c.scales, c.list, c.n_listed, c.io, c.n_rows, c.rank,
                                                                                                                c.n_segments, c.slices, c.n_adapters);
     return 0;
 }
@@ -859,7 +902,7 @@ int up(const Call& c) {
     // of 68), not where the waves share the rows out (600 of 4,096, rank 128: 43 us instead of 32; 1,024 of 2,048 in 32 bits, rank 64, 28 instead of 26).
     const bool keeps_four = steps <= 4 && strip_bits((int)usual_tiles(c.n_rows), c.columns) > 6;       // (then the strips there are, of at least as many tiles, are no shorter)
     constexpr int RUN = Piece<LOW>::RUN;
-    if (!c.io.vectors) return up_launch<LOW, W, false, 1, 0, false, false>(c);
+    if (!c.fours) return up_launch<LOW, W, false, 1, 0, false, false>(c);
     if (c.rank % RUN == 0 && aligned(c.b, RUN * sizeof(W)))
         return steps == 1 ? up_sized<LOW, W, RUN, 1>(c) : steps == 2 ? up_sized<LOW, W, RUN, 2>(c) : keeps_four ? up_sized<LOW, W, RUN, 4>(c) : up_sized<LOW, W, RUN, 0>(c);
     if constexpr (LOW)
@@ -867,13 +910,13 @@ int up(const Call& c) {
     return steps == 1 ? up_sized<LOW, W, 1, 1>(c) : up_sized<LOW, W, 1, 0>(c);
 }
 
-// bfloat16 rows that may be loaded 8 numbers at a time, few enough that loading an adapter once for every row that takes it costs less than tiles that share it.  Only the device knows which rows share:
+// bfloat16 rows few enough that loading an adapter once for every row that takes it costs less than tiles that share it.  Only the device knows which rows share:
 // with an adapter a row tiles lose (64 rows of 4,096 onto 4,096, rank 32: 10.5 us against 15.5; 256: 31 against 45; 512 of 2,048 onto 2,048, rank 16: 17 against 46), with one for all the two meet at some
 // 150 MB loaded (256 of 4,096 onto 4,096: 134 MB, 12.5 us against 13.5; 128 of 8,192 onto 2,048, rank 64: 168 MB, 19.1 against 19.6; 512 of 2,048 onto 8,192, rank 16: as many, 17.8 against 14.7; 256 of 8,192 onto
 // 2,048: 336 MB, 36 against 20, and 102 against 76 with an adapter each) and at fewer where there are more rows (768 of 2,048 onto 2,048: 100 MB, 12.6 against 13.0; 1,024: 134 MB, 16.9 against 13.7).
 bool few_rows(const Call& c) {
     const long loaded = 2l * c.n_rows * c.rank * ((long)c.slices.n * c.width + c.columns);
-    return c.n_rows <= 512 && loaded <= 160 << 20 && c.width % 8 == 0 && c.ldx % 8 == 0 && aligned(c.x, 16) && aligned(c.a, 16);
+    return c.n_rows <= 512 && loaded <= 160 << 20;
 }
 
 template <int N>
@@ -927,21 +970,18 @@ GI_API int gi_adapters_add(const void* x, int x_type, long ldx, const void* a, c
     GI_REQUIRE(scratch != nullptr && aligned(scratch, 16), "adapters_add: scratch is missing");
     const bool low = x_type == GI_BF16 && w_type == GI_BF16;
     Tile* list = (Tile*)(scratch + sums_for(x_type, w_type, n_rows, width, rank * n_slices));
-    Call c{x, ldx, a, b, ids, scales, Rows{base, out, ldb, ldo, base_type == GI_BF16, out_type == GI_BF16, false}, scratch, list, (int*)(list + n_rows), n_rows, width, columns, rank, n_adapters,
-           segment_of(n_rows, width, rank * n_slices, low), (int)segments_for(x_type, w_type, n_rows, width, rank * n_slices), Slices{n_slices, {0}, {0}}, stream};
-    bool fours = ldb % 4 == 0 && ldo % 4 == 0 && aligned(base, base_type == GI_BF16 ? 8 : 16) && aligned(out, out_type == GI_BF16 ? 8 : 16);
+    Call c{x, ldx, a, b, ids, scales, Rows{base, out, ldb, ldo, base_type == GI_BF16, out_type == GI_BF16}, scratch, list, (int*)(list + n_rows), n_rows, width, columns, rank, n_adapters,
+           segment_of(n_rows, width, rank * n_slices, low), (int)segments_for(x_type, w_type, n_rows, width, rank * n_slices), Slices{n_slices, {0}, {0}}, true, stream};
     for (int s = 0; s < n_slices; ++s) {
         GI_REQUIRE(slice_columns[s] > 0, "adapters_add: a packed projection of %d columns", slice_columns[s]);
-        fours = fours && slice_columns[s] % 4 == 0;
+        c.fours = c.fours && slice_columns[s] >= 4;
         c.slices.begin[s + 1] = c.slices.begin[s] + slice_columns[s];
     }
     GI_REQUIRE(c.slices.begin[n_slices] == columns, "adapters_add: the packed projections have %d columns, out has %d", c.slices.begin[n_slices], columns);
-    c.io.vectors = fours;
     if (low && few_rows(c)) {
-        const auto brings = [&](int n) { return rank % n == 0 && aligned(b, 2 * n); };
-        if (brings(8)) add_few<8>(c);
-        else if (brings(4)) add_few<4>(c);
-        else if (brings(2)) add_few<2>(c);
+        if (rank % 8 == 0) add_few<8>(c);
+        else if (rank % 4 == 0) add_few<4>(c);
+        else if (rank % 2 == 0) add_few<2>(c);
         else add_few<1>(c);
         GI_CHECK_LAUNCH("adapters_add (few rows)");
         return 0;

@@ -251,6 +251,18 @@ def test_offsets_beyond_32_bits():
         assert_right(out, c)
 
 
+@pytest.mark.parametrize("result", [F32, BF16])
+@pytest.mark.parametrize("n", [1, 70, 600, 1500])
+@pytest.mark.parametrize("columns,slices", [(65, None), (66, None), (67, None), (515, None), (2049, None), (193, (65, 128)), (262, (66, 67, 129)), (1031, (513, 4, 514))])
+def test_columns_that_are_no_fours(columns, slices, n, result):
+    """One to three columns behind whole blocks, onto base elsewhere and onto base itself; the rows begin at every place."""
+    for dtype in (BF16, F32):
+        c = make(n, 136, columns, 16, 3, dtype=dtype, ids="runs", base=result, slices=slices)
+        apart = run(c, result)
+        assert_right(apart, c)
+        assert torch.equal(run(c, result, in_place=True), apart)
+
+
 def test_the_most_rows_and_one_more():
     n = 2 ** 20
     for runs in ("mixed", "runs"):
