@@ -356,8 +356,8 @@ __global__ __launch_bounds__(64 * WAVES) void adapters_down_kernel(const typenam
     }
 }
 
-// Operands of two types, or rows that do not begin at 16 bytes: through registers, in the same order.  2,048 rows of 4,096 onto 4,096, rank 16, both ways: two types 30 us, as both of 32 bits; rows at odd places
-// 63 (32 bits, 30 at even ones) and 78 (bfloat16, 25): every number is a load of its own.
+// Operands of two types, or rows that do not begin at 16 bytes: through registers, in the same order, whole blocks by wide loads from any place.  2,048 rows of 4,096 onto 4,096, rank 16, both ways: two types 29 us, as
+// both of 32 bits 27; rows at odd places 31 (32 bits) and 32 (bfloat16, at even ones 25).
 template <bool LOW, typename X, typename W>
 __global__ __launch_bounds__(64 * ANY_WAVES) void adapters_down_any_kernel(const X* __restrict__ x, const W* __restrict__ a, const int* __restrict__ ids, float* __restrict__ sums, Down d) {
     typedef Piece<LOW> P;
@@ -600,15 +600,10 @@ __global__ __launch_bounds__(UP_NT) void adapters_up_kernel(const float* __restr
         }
         __syncthreads();
         if (idle) continue;
+        const int further_columns = by_rows ? 64 : 64 * UP_WAVES;
         while (true) {
             const int col = FOURS ? min(c0 + 4 * at, end - 4) : c0 + 4 * at;
-#pragma unroll 1
-            for (int j = j0; j <= last_j; j += j_step) {
-                uint4 was[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) was[i] = next[i];
-                ask_base(c0, min(j + j_step, last_j));
-                floatx4 sum[4];
+            auto products = [&](int j, floatx4 (&sum)[4]) {
 #pragma unroll
                 for (int n = 0; n < 4; ++n) sum[n] = floatx4{0.f, 0.f, 0.f, 0.f};
                 const T* row = held + (16 * j + at) * pitch + P::RUN * group;
@@ -629,31 +624,42 @@ __global__ __launch_bounds__(UP_NT) void adapters_up_kernel(const float* __restr
                         for (int n = 0; n < 4; ++n) sum[n] = times(t, br[0][n], sum[n]);
                     }
                 }
+            };
+            if (!FOURS || end - c0 < 4) {                  // one by one; of the last four columns those before c0 are another wave's, which may have stored them already
+#pragma unroll 1
+                for (int j = j0; j <= last_j; j += j_step) {
+                    floatx4 sum[4];
+                    products(j, sum);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int r = 16 * j + 4 * group + i;
-                    if constexpr (FOURS) {
-                        const uint32_t to = (uint32_t)(min(r, rows - 1) * (int)io.ldo + col);
-                        const floatx4 v = numbers4(was[i], LOW_BASE) + floatx4{sum[0][i], sum[1][i], sum[2][i], sum[3][i]};
-                        if (end - c0 >= 4) {
-                            store4(out_at, to, v, LOW_OUT);
-                        } else {                           // fewer are left: of the last four those before c0 are another wave's, which may have stored them already
-#pragma unroll
-                            for (int n = 0; n < 4; ++n)
-                                if (col + n >= c0) store1(out_at, to + n, v[n], LOW_OUT);
-                        }
-                    } else if (r < rows) {
+                    for (int i = 0; i < 4; ++i) {
+                        const int r = 16 * j + 4 * group + i;
+                        if (r >= rows) continue;
                         const uint32_t to = (uint32_t)(r * (int)io.ldo + col);
 #pragma unroll
                         for (int n = 0; n < 4; ++n)
-                            if (col + n < end) store1(out_at, to + n, number1(base_at, (size_t)(uint32_t)(r * (int)io.ldb + col + n), io.low_base) + sum[n][i], io.low_out);
+                            if (col + n >= c0 && col + n < end) store1(out_at, to + n, number1(base_at, (size_t)(uint32_t)(r * (int)io.ldb + col + n), io.low_base) + sum[n][i], io.low_out);
+                    }
+                }
+            } else {
+#pragma unroll 1
+                for (int j = j0; j <= last_j; j += j_step) {
+                    uint4 was[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) was[i] = next[i];
+                    const bool last = j + j_step > last_j;                             // the next columns' first rows are asked for behind these columns' last
+                    ask_base(last ? c0 + further_columns : c0, last ? j0 : j + j_step);
+                    floatx4 sum[4];
+                    products(j, sum);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const uint32_t to = (uint32_t)(min(16 * j + 4 * group + i, rows - 1) * (int)io.ldo + col);
+                        store4(out_at, to, numbers4(was[i], LOW_BASE) + floatx4{sum[0][i], sum[1][i], sum[2][i], sum[3][i]}, LOW_OUT);
                     }
                 }
             }
-            c0 += by_rows ? 64 : 64 * UP_WAVES;
+            c0 += further_columns;
             if (c0 >= end) break;
             ask_b(c0);
-            ask_base(c0, j0);
         }
     }
 }
