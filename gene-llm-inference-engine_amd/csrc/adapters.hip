@@ -259,8 +259,8 @@ __device__ __forceinline__ void store_sums(floatx4 (&sum)[4][MT], unsigned char*
 // Rows of one type, 16-byte loads.  Global memory goes straight into LDS (a lane's 16 bytes land behind the lane's before it), every wave through a ring of its own, so that no barrier stands in the loop: in registers the
 // operands' layout, neighbouring lanes in different rows, would take a load through the first-level cache in 64 pieces of 16 bytes instead of 16 whole sectors.  A stage is 64 rows of x and 16 MT of A,
 // 128 bytes each, its 16-byte chunk c of a row at place c ^ (row / 2 % 8), so that 16 rows' chunks lie in different banks (the counters show no conflict).
-// 4,096 rows of 14,336, rank 64: 38 us for 117 MB, 9 of them for counting tiles, the first loads and joining the waves' sums (without the products the time is the same); 2,048 of 2,048, rank 32, 7.0;
-// 531 of 4,096, rank 3 * 24, 10.0; 301 of 2,048 in 32 bits, rank 10, 6.8.
+// 4,096 rows of 14,336, rank 64: 37.5 us for 117 MB, 9 of them for counting tiles, the first loads and joining the waves' sums (without the products the time is the same); 2,048 of 2,048, rank 32, 6.7;
+// 531 of 4,096, rank 3 * 24, 10.2; 301 of 2,048 in 32 bits, rank 10, 6.9.
 constexpr int STAGES = 2;                   // (a third makes no difference of 1%: other workgroups of the unit load meanwhile)
 template <int MT> constexpr int stage_bytes() { return (TILE + 16 * MT) * 128; }
 
@@ -487,7 +487,7 @@ __host__ __device__ inline int strip_bits(int n_tiles, int columns) {          /
 // row's values meet another's.  FOURS: a projection has four columns or more, so base and out come four at a time.  AT_ONCE: numbers of B that one load brings.  KS: runs of ranks that a wave keeps; 0 for any number,
 // loaded again for every 16 rows (8,192 rows of 14,336 columns, rank 16: 239 us kept, 272 loaded again).  LOW_BASE, LOW_OUT: of aligned ones whether they are bfloat16 (a branch on it where they are loaded would have every load waited for); `io` says it of others.
 // 4,096 rows of 4,096 32-bit columns, rank 64: 41 us for the 134 MB of base and out (a copy of as much takes 25); 531 of 6,144, rank 24, onto bfloat16 10.3; 2,048 of 2,048, rank 32, 9.4; 301 of 2,048 in 32 bits,
-// rank 10, 10.6.  Asking for a whole tile's base at once instead of 16 rows ahead makes it no faster: 4,096 rows of 4,096 both ways 50 us instead of 47, with 256 registers instead of 141.
+// rank 10, 8.4.  Asking for a whole tile's base at once instead of 16 rows ahead makes it no faster: 4,096 rows of 4,096 both ways 50 us instead of 47, with 256 registers instead of 141.
 template <bool LOW, typename W, bool FOURS, int AT_ONCE, int KS, bool LOW_BASE, bool LOW_OUT>
 __global__ __launch_bounds__(UP_NT) void adapters_up_kernel(const float* __restrict__ sums, const W* __restrict__ b, const float* __restrict__ scales, const Tile* __restrict__ list,
                                                             const int* __restrict__ n_listed, Rows io, int n_rows, int rank, int n_segments, Slices slices, int n_adapters) {
@@ -696,7 +696,7 @@ __global__ __launch_bounds__(256) void adapters_down_few_kernel(const bf16_t* __
     if (tid == 0) sums[(size_t)row * ranks + blockIdx.x] = (red[0] + red[1]) + (red[2] + red[3]);
 }
 
-// Up: a thread has FEW_COLUMNS columns, 256 apart, of a row; the row's sums come as scalars.  64 rows of 14,336, rank 16: 8.1 us for 37 MB (4.5 TB/s).
+// Up: a thread has FEW_COLUMNS columns, 256 apart, of a row; the row's sums come as scalars.  64 rows of 14,336, rank 16: 7.4 us for 37 MB (5 TB/s); of a rank that is no multiple of 8 fewer numbers come at once.
 constexpr int FEW_COLUMNS = 2;
 template <int N>                            // ranks of a column that one load brings
 __global__ __launch_bounds__(256) void adapters_up_few_kernel(const float* __restrict__ sums, const bf16_t* __restrict__ b, const float* __restrict__ scales, const int* __restrict__ ids,
@@ -740,7 +740,7 @@ __global__ __launch_bounds__(256) void adapters_up_few_kernel(const float* __res
 bool aligned(const void* p, int bytes) { return (size_t)p % bytes == 0; }
 
 // Both ways in one launch, where making a row's sums anew for every strip of its columns costs less than a second launch: a wave makes every fourth sum, then a thread has its columns as above.  One
-// row of 2,048 onto 2,048, rank 16: 4.6 us, the waits of three loads that follow one another.
+// row of 2,048 onto 2,048, rank 16: 4.4 us, the waits of three loads that follow one another.
 template <int N>
 __global__ __launch_bounds__(256) void adapters_both_few_kernel(const bf16_t* __restrict__ x, long ldx, const bf16_t* __restrict__ a, const bf16_t* __restrict__ b, const float* __restrict__ scales,
                                                                 const int* __restrict__ ids, Rows io, int width, int rank, Slices slices, int n_adapters) {

@@ -12,8 +12,8 @@
 //
 // Three launches.  All rows once, in runs of 4,096 logits: the runs' maxima and sums.  Then, per request and run, the verdict (every workgroup of a request comes to it by itself, from the runs' numbers) and,
 // where a draft fell, the run's share of what is drawn from.  Then a request's draw.  What bounds them: of many rows the logits' bytes and, as much, the weights' instructions (64 requests, 401 rows of 128,256
-// tokens, 206 MB: 51 + 20 + 9 us); of a few the waits that follow one another (one request with 4 drafts, 9 such rows: 4.5 + 8.7 + 7.0 us).  A last workgroup that draws by itself instead of a third launch has
-// to see what the others wrote: with the fences for that one request takes 29.7 us instead of 20.5, 64 take 121 instead of 81.
+// tokens, 206 MB: 49 + 20 + 8 us); of a few the waits that follow one another (one request with 4 drafts, 9 such rows: 4.5 + 7.0 + 6.1 us).  A last workgroup that draws by itself instead of a third launch has
+// to see what the others wrote: with the fences for that one request took 29.7 us instead of 20.5, 64 took 121 instead of 81.
 #include "common.h"
 #include "lanes.h"
 
@@ -59,8 +59,7 @@ __device__ __forceinline__ float number(float v) { return v == v ? v : -INFINITY
 
 // Weights exp((l - top) / T) of a row whose largest logit is `top`: 1 for the largest, 0 for what is no token (-infinity, NaN) and below 2^-1020.  With m = (l - top) log2(e) / T, n the nearest integer (what is left in
 // the low bits of a sum with 1.5 * 2^52) and f = m - n, 2^m is 2^n (1 + f q(f)), q the polynomial through (2^f - 1) / f at eight Chebyshev points of [-1/2, 1/2]: off by 2e-12 relative, less than a draw over a
-// million tokens can notice.  No scaling by an instruction of its own: those, as conversions, run at a quarter of the rate, and instructions are what bounds a sum over many rows (four fifths of the cycles issue
-// one; a polynomial of nine points and a product of its own for m: 55 us for 401 rows of 128,256 tokens that now take 51).
+// million tokens can notice.  No scaling by an instruction of its own: those, as conversions, run at a quarter of the rate, and instructions are what bounds a sum over many rows (four fifths of the cycles one; a polynomial of nine points and a product of its own for m: 55 us for 401 rows of 128,256 tokens that took 51 so). of nine points and a product of its own for m: 55 us for 401 rows of 128,256 tokens that now take 51).
 __device__ __forceinline__ double horner(double f, double q, double c) {        // f q + c, the coefficient in scalar registers: as the accumulator it would be moved there for every step
     double out;
     asm("v_fma_f64 %0, %1, %2, %3" : "=v"(out) : "v"(f), "v"(q), "s"(c));
@@ -134,7 +133,7 @@ struct RunOf {
 };
 
 // Largest logit (with its lowest index) and sum of exp((l - that) / T) of every run: workgroup (run, request, group of rows).  Of the rows that the request has, the target's 0 .. n and the drafter's 0 .. n - 1 behind
-// them, every gridDim.z-th is a workgroup's.  4.5 us for 9 rows of 128,256 tokens, 8.0 for 192 greedy ones of 32,003 (3.1 TB/s), 51 for 401 of 128,256 (4.0 TB/s; the loads alone take 40).
+// them, every gridDim.z-th is a workgroup's.  4.5 us for 9 rows of 128,256 tokens, 7.7 for 192 greedy ones of 32,003 (3.2 TB/s), 49 for 401 of 128,256 (4.2 TB/s; the loads alone take 40).
 constexpr int PARTS_NT = 256;
 __global__ __launch_bounds__(PARTS_NT) void parts_kernel(Inputs in, float* __restrict__ part_m, int* __restrict__ part_i, double* __restrict__ part_s) {
     constexpr int NT = PARTS_NT, PER = CHUNK / NT, WAVES = NT / 64;
@@ -218,7 +217,7 @@ struct Drawn {
 };
 
 // Which drafts stay, and the sums over runs of what is drawn from, where the parts do not hold them already: every run of a request whose drafter's row is taken off, and the run that a draft is
-// left out of.  Workgroup (run, request); run 0's writes what the request has so far.  8.7 us for one request with 4 drafts, 20 for 64 with up to 7, which read two rows of 128,256 again
+// left out of.  Workgroup (run, request); run 0's writes what the request has so far.  7.0 us for one request with 4 drafts, 20 for 64 with up to 7, which read two rows of 128,256 again
 // each (58 MB), once the verdict says which: its waits (6 us) have nothing beside them.
 template <int NT>
 __global__ __launch_bounds__(NT) void judge_kernel(Inputs in, const float* __restrict__ part_m, const int* __restrict__ part_i, const double* __restrict__ part_s, Verdict* __restrict__ verdicts,
@@ -360,7 +359,7 @@ __global__ __launch_bounds__(NT) void judge_kernel(Inputs in, const float* __res
 }
 
 // The draw: one workgroup a request.  The run is found among the runs' sums (by a prefix sum over a wave's lanes, which share the runs out, and a walk over one lane's), then the token in the run: a
-// thread owns four consecutive tokens, a prefix sum over the threads finds the thread, which walks its tokens.  7 us for one request, 9 for 64, all of it waits; with 256 threads, sixteen tokens each, 12 for one.
+// thread owns four consecutive tokens, a prefix sum over the threads finds the thread, which walks its tokens.  6 us for one request, 8 for 64, all of it waits; with 256 threads, sixteen tokens each, 5 us more.
 constexpr int PICK_NT = 1024, PICK_WAVES = PICK_NT / 64, PICK_PER = CHUNK / PICK_NT;
 __global__ __launch_bounds__(PICK_NT) void pick_kernel(Inputs in, const Verdict* __restrict__ verdicts, const float* __restrict__ part_m, const double* __restrict__ part_s,
                                                        const double* __restrict__ rest, int* __restrict__ tokens) {
