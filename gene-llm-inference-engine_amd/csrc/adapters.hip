@@ -696,9 +696,26 @@ __global__ __launch_bounds__(256) void adapters_down_few_kernel(const bf16_t* __
     if (tid == 0) sums[(size_t)row * ranks + blockIdx.x] = (red[0] + red[1]) + (red[2] + red[3]);
 }
 
-// Up: a thread has FEW_COLUMNS columns, 256 apart, of a row; the row's sums come as scalars.  64 rows of 14,336, rank 16: 7.4 us for 37 MB (5 TB/s); of a rank that is no multiple of 8 fewer numbers come at once.
+// Up: a thread has FEW_COLUMNS columns, 256 apart, of a row; the row's sums come as scalars.  64 rows of 14,336, rank 16: 7.4 us for 37 MB (5 TB/s).
 constexpr int FEW_COLUMNS = 2;
-template <int N>                            // ranks of a column that one load brings
+// The ranks' sums times N of them of each of a thread's columns, from rank k on.
+template <int N>
+__device__ __forceinline__ void add_ranks(float (&sum)[FEW_COLUMNS], const float* t, const bf16_t* const (&br)[FEW_COLUMNS], int k) {
+    Some<N> v[FEW_COLUMNS];
+#pragma unroll
+    for (int c = 0; c < FEW_COLUMNS; ++c) v[c] = *reinterpret_cast<const Some<N>*>(br[c] + k);
+#pragma unroll
+    for (int c = 0; c < FEW_COLUMNS; ++c)
+#pragma unroll
+        for (int u = 0; u < N; ++u) sum[c] = fmaf(t[k + u], v[c][u], sum[c]);
+}
+__device__ __forceinline__ void add_last_ranks(float (&sum)[FEW_COLUMNS], const float* t, const bf16_t* const (&br)[FEW_COLUMNS], int rank) {       // those behind the last eight
+    int k = rank & ~7;
+    if (rank & 4) { add_ranks<4>(sum, t, br, k); k += 4; }
+    if (rank & 2) { add_ranks<2>(sum, t, br, k); k += 2; }
+    if (rank & 1) add_ranks<1>(sum, t, br, k);
+}
+
 __global__ __launch_bounds__(256) void adapters_up_few_kernel(const float* __restrict__ sums, const bf16_t* __restrict__ b, const float* __restrict__ scales, const int* __restrict__ ids,
                                                               Rows io, int rank, Slices slices, int n_adapters) {
     const int row = blockIdx.y;
@@ -720,15 +737,8 @@ __global__ __launch_bounds__(256) void adapters_up_few_kernel(const float* __res
 #pragma unroll
         for (int c = 0; c < FEW_COLUMNS; ++c) br[c] = b + ((size_t)e * slices.begin[slices.n] + min(begin + 256 * c, end - 1)) * rank;
         const float scale = scales != nullptr ? scales[e] : 1.f;
-        for (int k = 0; k < rank; k += N) {
-            Some<N> v[FEW_COLUMNS];
-#pragma unroll
-            for (int c = 0; c < FEW_COLUMNS; ++c) v[c] = *reinterpret_cast<const Some<N>*>(br[c] + k);
-#pragma unroll
-            for (int c = 0; c < FEW_COLUMNS; ++c)
-#pragma unroll
-                for (int u = 0; u < N; ++u) sum[c] = fmaf(t[k + u], v[c][u], sum[c]);
-        }
+        for (int k = 0; k + 8 <= rank; k += 8) add_ranks<8>(sum, t, br, k);
+        add_last_ranks(sum, t, br, rank);
 #pragma unroll
         for (int c = 0; c < FEW_COLUMNS; ++c) was[c] = fmaf(scale, sum[c], was[c]);
     }
@@ -741,7 +751,6 @@ bool aligned(const void* p, int bytes) { return (size_t)p % bytes == 0; }
 
 // Both ways in one launch, where making a row's sums anew for every strip of its columns costs less than a second launch: a wave makes every fourth sum, then a thread has its columns as above.  One
 // row of 2,048 onto 2,048, rank 16: 4.4 us, the waits of three loads that follow one another.
-template <int N>
 __global__ __launch_bounds__(256) void adapters_both_few_kernel(const bf16_t* __restrict__ x, long ldx, const bf16_t* __restrict__ a, const bf16_t* __restrict__ b, const float* __restrict__ scales,
                                                                 const int* __restrict__ ids, Rows io, int width, int rank, Slices slices, int n_adapters) {
     __shared__ float t[MAX_RANK];
@@ -760,11 +769,11 @@ __global__ __launch_bounds__(256) void adapters_both_few_kernel(const bf16_t* __
     }
     if (some) {
         const bf16_t* br[FEW_COLUMNS];
-        Some<N> v[FEW_COLUMNS];
+        Some<8> v[FEW_COLUMNS] = {};
 #pragma unroll
         for (int c = 0; c < FEW_COLUMNS; ++c) {
             br[c] = b + ((size_t)e * slices.begin[slices.n] + min(begin + 256 * c, end - 1)) * rank;
-            v[c] = *reinterpret_cast<const Some<N>*>(br[c]);
+            if (rank >= 8) v[c] = *reinterpret_cast<const Some<8>*>(br[c]);
         }
         const float scale = scales != nullptr ? scales[e] : 1.f;
         const bf16_t* xr = x + (size_t)row * ldx;
@@ -795,15 +804,16 @@ __global__ __launch_bounds__(256) void adapters_both_few_kernel(const bf16_t* __
             }
         }
         __syncthreads();
-        for (int k = 0; k < rank; k += N) {
+        for (int k = 0; k + 8 <= rank; k += 8) {
 #pragma unroll
             for (int c = 0; c < FEW_COLUMNS; ++c) {
-                const Some<N> now = v[c];
-                if (k + N < rank) v[c] = *reinterpret_cast<const Some<N>*>(br[c] + k + N);
+                const Some<8> now = v[c];
+                if (k + 16 <= rank) v[c] = *reinterpret_cast<const Some<8>*>(br[c] + k + 8);
 #pragma unroll
-                for (int u = 0; u < N; ++u) sum[c] = fmaf(t[k + u], now[u], sum[c]);
+                for (int u = 0; u < 8; ++u) sum[c] = fmaf(t[k + u], now[u], sum[c]);
             }
         }
+        add_last_ranks(sum, t, br, rank);
 #pragma unroll
         for (int c = 0; c < FEW_COLUMNS; ++c) was[c] = fmaf(scale, sum[c], was[c]);
     }
@@ -925,7 +935,6 @@ bool few_rows(const Call& c) {
     return c.n_rows <= 512 && loaded <= 160 << 20;
 }
 
-template <int N>
 void add_few(const Call& c) {
     const int ranks = c.rank * c.slices.n;
     Slices slices = c.slices;
@@ -935,11 +944,11 @@ void add_few(const Call& c) {
     // One launch takes the host 3 us less than two, and the device as long as two where a workgroup reads 64 KB of A again (1 row of 2,048 onto 2,048 or 8,192, rank 16: 4.7 us either way); at 128 KB 5.7 us
     // against 4.8, at 256 KB 9.0 against 5.4, and 40 rows onto 8,192 columns 6.4 to 7.2 against 5.6.
     if (again <= 64 << 10 && again * strips.x * strips.y <= 16 << 20) {
-        adapters_both_few_kernel<N><<<strips, 256, 0, c.stream>>>((const bf16_t*)c.x, c.ldx, (const bf16_t*)c.a, (const bf16_t*)c.b, c.scales, c.ids, c.io, c.width, c.rank, slices, c.n_adapters);
+        adapters_both_few_kernel<<<strips, 256, 0, c.stream>>>((const bf16_t*)c.x, c.ldx, (const bf16_t*)c.a, (const bf16_t*)c.b, c.scales, c.ids, c.io, c.width, c.rank, slices, c.n_adapters);
         return;
     }
     adapters_down_few_kernel<<<dim3(ranks, c.n_rows), 256, 0, c.stream>>>((const bf16_t*)c.x, c.ldx, (const bf16_t*)c.a, c.ids, c.sums, c.width, ranks, c.n_adapters);
-    adapters_up_few_kernel<N><<<strips, 256, 0, c.stream>>>(c.sums, (const bf16_t*)c.b, c.scales, c.ids, c.io, c.rank, slices, c.n_adapters);
+    adapters_up_few_kernel<<<strips, 256, 0, c.stream>>>(c.sums, (const bf16_t*)c.b, c.scales, c.ids, c.io, c.rank, slices, c.n_adapters);
 }
 
 // In 32 bits only the width says how long a segment is: few rows want many (64 of 14,336 onto 4,096, rank 16: 18.8, 20.0 and 22.8 us with 16, 12 and 8 at most, 21.8 always at 256 numbers), many rows few
@@ -985,10 +994,7 @@ GI_API int gi_adapters_add(const void* x, int x_type, long ldx, const void* a, c
     }
     GI_REQUIRE(c.slices.begin[n_slices] == columns, "adapters_add: the packed projections have %d columns, out has %d", c.slices.begin[n_slices], columns);
     if (low && few_rows(c)) {
-        if (rank % 8 == 0) add_few<8>(c);
-        else if (rank % 4 == 0) add_few<4>(c);
-        else if (rank % 2 == 0) add_few<2>(c);
-        else add_few<1>(c);
+        add_few(c);
         GI_CHECK_LAUNCH("adapters_add (few rows)");
         return 0;
     }
