@@ -495,7 +495,7 @@ __global__ __launch_bounds__(UP_NT) void adapters_up_kernel(const float* __restr
     typedef typename P::T T;
     extern __shared__ __align__(16) unsigned char room[];
     constexpr int DEPTH = P::BLOCK / 2;                    // ranks of a matrix instruction (of four, in 32 bits)
-    const int padded = (rank + DEPTH - 1) / DEPTH * DEPTH, pitch = padded + P::RUN, apart = TILE * pitch;       // (rows of LDS a run further apart than a multiple of all banks)
+    const int padded = KS > 0 ? KS * DEPTH : (rank + DEPTH - 1) / DEPTH * DEPTH, pitch = padded + P::RUN, apart = TILE * pitch;       // (rows of LDS a run further apart than a multiple of all banks)
     T* held = (T*)room;                                    // [pieces][TILE][pitch], the largest piece first
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, at = lane & 15, group = lane >> 4;
     const int columns = slices.begin[slices.n], ranks = rank * slices.n, n_tiles = *n_listed, bits = strip_bits(n_tiles, columns), strip_columns = 1 << bits;
@@ -889,18 +889,19 @@ int down(const Call& c) {
 }
 
 // Bytes of LDS that the way up keeps a tile's sums in.
-template <bool LOW> constexpr int up_lds(int rank) {
+template <bool LOW, int KS> constexpr int up_lds(int rank) {
     constexpr int DEPTH = Piece<LOW>::BLOCK / 2;
+    if (KS > 0) rank = KS * DEPTH;
     return TILE * ((rank + DEPTH - 1) / DEPTH * DEPTH + Piece<LOW>::RUN) * (LOW ? 2 * PIECES : 4);
 }
 
 template <bool LOW, typename W, bool FOURS, int AT_ONCE, int KS, bool LOW_BASE, bool LOW_OUT>
 int up_launch(const Call& c) {
     static bool raised[MAX_DEVICES] = {};
-    constexpr int most = up_lds<LOW>(MAX_RANK);
+    constexpr int most = up_lds<LOW, KS>(MAX_RANK);
     if (raise_lds((const void*)adapters_up_kernel<LOW, W, FOURS, AT_ONCE, KS, LOW_BASE, LOW_OUT>, most, raised) != 0) return -1;
     const int grid = (int)min((long)c.n_rows * ((c.columns + 63) / 64 + c.slices.n), 4l * gi_compute_units());
-    adapters_up_kernel<LOW, W, FOURS, AT_ONCE, KS, LOW_BASE, LOW_OUT><<<grid, UP_NT, up_lds<LOW>(c.rank), c.stream>>>(c.sums, (const W*)c.b, c.scales, c.list, c.n_listed, c.io, c.n_rows, c.rank,
+    adapters_up_kernel<LOW, W, FOURS, AT_ONCE, KS, LOW_BASE, LOW_OUT><<<grid, UP_NT, up_lds<LOW, KS>(c.rank), c.stream>>>(c.sums, (const W*)c.b, c.scales, c.list, c.n_listed, c.io, c.n_rows, c.rank,
                                                                                                                c.n_segments, c.slices, c.n_adapters);
     return 0;
 }

@@ -75,7 +75,7 @@ def run(c, result=F32, in_place=False):
 SIZES = [(1, 1, 1, 1, 1), (1, 8, 16, 8, 2), (1, 2048, 2048, 16, 3), (3, 65, 33, 5, 2), (7, 256, 129, 16, 8), (16, 512, 512, 32, 4), (17, 264, 200, 24, 5), (33, 520, 264, 1, 33), (64, 1024, 1000, 64, 70),
          (65, 1000, 72, 12, 3), (100, 2049, 130, 7, 9), (129, 640, 384, 128, 3), (250, 328, 520, 130, 4), (515, 4096, 256, 16, 6), (70, 72, 4104, 40, 2), (300, 31, 31, 31, 31),
          (130, 96, 80, 256, 2), (20, 96, 80, 256, 2), (200, 100, 50, 225, 9), (1200, 1536, 1100, 48, 3),
-         (600, 328, 520, 128, 4), (530, 96, 80, 256, 2), (520, 264, 200, 24, 5), (40, 264, 201, 4, 9), (7, 1032, 96, 12, 7), (3, 72, 600, 6, 2), (2, 4096, 512, 10, 2), (90, 136, 64, 1, 3), (900, 264, 2048, 12, 4), (700, 520, 1024, 44, 3), (800, 128, 512, 10, 2), (1600, 520, 2100, 104, 3), (1700, 264, 2048, 52, 4), (1025, 1000, 72, 40, 1100)]
+         (600, 328, 520, 128, 4), (530, 96, 80, 256, 2), (520, 264, 200, 24, 5), (40, 264, 201, 4, 9), (7, 1032, 96, 12, 7), (3, 72, 600, 6, 2), (2, 4096, 512, 10, 2), (90, 136, 64, 1, 3), (900, 264, 2048, 12, 4), (700, 520, 1024, 44, 3), (800, 128, 512, 10, 2), (1600, 520, 2100, 104, 3), (1600, 264, 2100, 72, 3), (1700, 264, 2048, 52, 4), (1700, 264, 2048, 36, 4), (1025, 1000, 72, 40, 1100)]
 
 
 @pytest.mark.parametrize("n,width,columns,rank,adapters", SIZES)
@@ -139,6 +139,23 @@ def test_a_row_of_no_numbers_stays_its_own(dtype):
         assert got[0].isnan().all() and not got[ids == 1].isfinite().any() and got[ids == 2][:, 5].isnan().all()
         others = got[ids == 2]
         assert torch.equal(torch.cat([others[:, :5], others[:, 6:]], 1), torch.cat([clean[ids == 2][:, :5], clean[ids == 2][:, 6:]], 1))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("rank", [5, 8, 20, 24, 36, 40, 72, 96, 136, 200])
+def test_a_row_of_no_numbers_stays_its_own_at_every_rank(rank, dtype):
+    """The ranks' places behind the last, which the products run over, hold nothing of the rows beside."""
+    for n in (90, 1600):
+        c = make(n, 128, 2048, rank, 2, dtype=dtype, ids=0)
+        clean = run(c)
+        for bad in (float("nan"), float("inf")):
+            other = dict(c, x=c["x"].clone())
+            other["x"][3::5] = bad
+            got = run(other)
+            whole = torch.ones(n, dtype=torch.bool, device=DEV)
+            whole[3::5] = False
+            assert torch.equal(got[whole], clean[whole])
+            assert not got[~whole].isfinite().any()
 
 
 @pytest.mark.parametrize("n", [1, 20, 600])
