@@ -214,6 +214,17 @@ struct Tile {                               // of the list that the way down lea
     int first, rows, id, unused;
 };
 
+// A workgroup's pieces of work, every gridDim.x-th of `tiles` times `parts`, without a division for each.
+struct Share {
+    int tile, part, parts, by_tiles, by_parts;
+    __device__ explicit Share(int of) : tile(blockIdx.x / of), part(blockIdx.x % of), parts(of), by_tiles(gridDim.x / of), by_parts(gridDim.x % of) {}
+    __device__ void next() {
+        tile += by_tiles;
+        part += by_parts;
+        if (part >= parts) { part -= parts; ++tile; }
+    }
+};
+
 // ------------------------------------------------------------------ down, in tiles
 // sums[segment][row][rank] of a tile, a segment of the width and a group of 16 MT ranks.  A workgroup's waves share out the segment, every second block of 128 bytes a row, so that none
 // loads what the other does.  In the product D = M N the ranks are M's rows and the tile's rows N's columns: a lane of the result has values of one row only, and rows behind the tile's
@@ -275,12 +286,11 @@ __global__ __launch_bounds__(64 * WAVES) void adapters_down_kernel(const typenam
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, at = lane & 15, group = lane >> 4;
     Tiles<WAVES> tiles{ids, d.n_rows, 0, 0};
     const int n_tiles = tiles.count(before);
-    const long n_items = (long)n_tiles * d.n_parts;
     unsigned char* mine = ring + wave * STAGES * BYTES;
     const unsigned mine_at = (unsigned)(size_t)(lds_ptr_t)mine;
-    for (long item = blockIdx.x; item < n_items; item += gridDim.x) {
+    for (Share work(d.n_parts); work.tile < n_tiles; work.next()) {
         int first_row, rows, e;
-        const int part = (int)(item % d.n_parts), which = (int)(item / d.n_parts);
+        const int part = work.part, which = work.tile;
         tiles.find(before, which, first_row, rows, e);
         if (part == 0 && threadIdx.x == 0) {
             d.list[which] = Tile{first_row, rows, e, 0};
@@ -367,10 +377,9 @@ __global__ __launch_bounds__(64 * ANY_WAVES) void adapters_down_any_kernel(const
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, at = lane & 15, group = lane >> 4;
     Tiles<ANY_WAVES> tiles{ids, d.n_rows, 0, 0};
     const int n_tiles = tiles.count(before);
-    const long n_items = (long)n_tiles * d.n_parts;
-    for (long item = blockIdx.x; item < n_items; item += gridDim.x) {
+    for (Share work(d.n_parts); work.tile < n_tiles; work.next()) {
         int first_row, rows, e;
-        const int part = (int)(item % d.n_parts), which = (int)(item / d.n_parts);
+        const int part = work.part, which = work.tile;
         tiles.find(before, which, first_row, rows, e);
         if (part == 0 && threadIdx.x == 0) {
             d.list[which] = Tile{first_row, rows, e, 0};
@@ -502,12 +511,11 @@ __global__ __launch_bounds__(UP_NT) void adapters_up_kernel(const float* __restr
     auto strips_of = [&](int s) { return (slices.begin[s + 1] - slices.begin[s] + strip_columns - 1) >> bits; };
     int n_strips = 0;
     for (int s = 0; s < slices.n; ++s) n_strips += strips_of(s);
-    const long n_items = (long)n_tiles * n_strips;
-    for (long item = blockIdx.x; item < n_items; item += gridDim.x) {
-        int strip = (int)(item % n_strips), s = 0;
+    for (Share work(n_strips); work.tile < n_tiles; work.next()) {
+        int strip = work.part, s = 0;
         for (; s + 1 < slices.n && strip >= strips_of(s); ++s) strip -= strips_of(s);
         const int begin = slices.begin[s] + strip * strip_columns, end = min(slices.begin[s + 1], begin + strip_columns);
-        const Tile tile = list[item / n_strips];
+        const Tile tile = list[work.tile];
         const int first_row = tile.first, rows = tile.rows, e = tile.id;
         if (e < 0 || e >= n_adapters) {                    // rows without an adapter
             if (io.base != io.out)
