@@ -950,8 +950,8 @@ void add_few(const Call& c) {
     for (int s = 0; s < slices.n; ++s) slices.strip[s + 1] = slices.strip[s] + (slices.begin[s + 1] - slices.begin[s] + 256 * FEW_COLUMNS - 1) / (256 * FEW_COLUMNS);
     const dim3 strips(slices.strip[slices.n], c.n_rows);
     const long again = (long)c.rank * c.width * 2;         // bytes of A that every strip's workgroup reads
-    // One launch takes the host 3 us less than two, and the device as long as two where a workgroup reads 64 KB of A again (1 row of 2,048 onto 2,048 or 8,192, rank 16: 4.7 us either way); at 128 KB 5.7 us
-    // against 4.8, at 256 KB 9.0 against 5.4, and 40 rows onto 8,192 columns 6.4 to 7.2 against 5.6.
+    // One launch takes the host 3 us less than two, and the device no longer where a workgroup reads 64 KB of A again (1 row of 2,048 onto 2,048 or 8,192, rank 16: 4.1 and 4.2 us against 4.6 and 4.7); at 128 KB 5.1 us
+    // against 4.7, at 256 KB 7.7 against 5.5, and 40 rows onto 8,192 columns 6.7 against 5.6.
     if (again <= 64 << 10 && again * strips.x * strips.y <= 16 << 20) {
         adapters_both_few_kernel<<<strips, 256, 0, c.stream>>>((const bf16_t*)c.x, c.ldx, (const bf16_t*)c.a, (const bf16_t*)c.b, c.scales, c.ids, c.io, c.width, c.rank, slices, c.n_adapters);
         return;
