@@ -2183,7 +2183,7 @@ def verify_drafts(logits, drafts, temperature, uniform, tokens, counts, draft_lo
     tokens, int32 [requests, K + 1], receives the drafts that stay, the token behind them and then -1; counts, int32 [requests], how many tokens those are.
     A draft x stays if those before it do and u q(x) < p(x) (arg max: if it is the row's lowest arg max); the token behind is drawn in index order
     from max(p - q, 0) where a draft fell (from p, where less than 1e-12 of that is left: a draft outside the vocabulary may fall with q equal to p) and from p where none did.  Logits of -infinity or NaN are no tokens (a row of nothing else lets no draft stay and gives token
-    0), a draft outside the vocabulary falls.  A request whose rows do not lie among those given gets count 0."""
+    0), a draft outside the vocabulary falls.  A request whose rows do not lie among those given gets count 0.  At most VERIFY_MAX_DRAFTS drafts a request, 65,535 requests and 4,194,304 tokens."""
     what = "verify_drafts"
     f32, i32 = torch.float32, torch.int32
     if not (logits.dtype == f32 and logits.dim() == 2 and logits.shape[1] > 0 and (logits.stride(1) == 1 or logits.shape[1] == 1)):
@@ -2282,6 +2282,7 @@ def adapters_add(x, a, b, ids, out, scales=None, base=None, slices=None, checked
     also be given as both, but otherwise out shares no memory with an operand); out likewise.  slices: the columns of the projections that out packs, in their order
     (at most ADAPTER_MAX_SLICES); a then holds a block of `rank` rows for each, [adapters, len(slices) * rank, width].  Adapters of smaller rank are filled up with zeros.
     Sums are in 32 bits; a row's result does not depend on what the other rows hold, and with float32 x not on how many there are either.
+    At most 2^20 rows, a width of 2^24, 2^22 columns and rank ADAPTER_MAX_RANK; rows of base and out at most 2^23 numbers apart.
     checked: what `adapters_check` gave for these operands, if it has been asked."""
     if base is None:
         base = out

@@ -267,3 +267,18 @@ def test_offsets_beyond_32_bits():
     given = dict(c, first_row=first)
     got = run(given, logits=logits, draft_logits=big)
     assert np.array_equal(got[0], want[0]) and np.array_equal(got[1], want[1])
+
+
+def test_the_most_requests_and_tokens_and_one_more():
+    n = 65535
+    c = case(3, 1, 5)
+    many = {name: None if values is None else np.concatenate([values] * (n // 3)) for name, values in c.items()}
+    many["first_row"] = (c["first_row"][None] + 6 * np.arange(n // 3, dtype=np.int32)[:, None]).reshape(-1)
+    got, few = run(many), plain_drafts.verify(**c)
+    assert np.array_equal(got[0].reshape(-1, 3, 2), np.broadcast_to(few[0], (n // 3, 3, 2))) and np.array_equal(got[1].reshape(-1, 3), np.broadcast_to(few[1], (n // 3, 3)))
+    check(case(1, 1, 1024 * 4096))
+    for requests, vocab, message in ((n + 1, 2, "bad sizes"), (1, 1024 * 4096 + 1, "vocabulary")):
+        i32 = dict(dtype=torch.int32, device=DEV)
+        with pytest.raises(ops().KernelError, match=message):
+            ops().verify_drafts(torch.zeros((requests, vocab), device=DEV), torch.zeros((requests, 0), **i32), torch.ones(requests, device=DEV), torch.zeros((requests, 1), device=DEV),
+                                torch.zeros((requests, 1), **i32), torch.zeros(requests, **i32))
