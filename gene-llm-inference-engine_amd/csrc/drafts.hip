@@ -399,12 +399,14 @@ __global__ __launch_bounds__(PICK_NT) void pick_kernel(Inputs in, const Verdict*
                 double walked = below, before_last = walked;
                 int run = -1, last = -1;
                 for (int c = from; c < to && run < 0; ++c) {
-                    if (sums[c] > 0.0) { last = c; before_last = walked; }
+                    if (!(sums[c] > 0.0)) continue;        // (the goal may lie a rounding below `below`, where no lane before holds it: a run of no weight is none to draw from)
+                    last = c;
+                    before_last = walked;
                     if (goal < walked + sums[c]) run = c;
                     walked += sums[c];
                 }
                 the_run = run >= 0 ? run : last;
-                before_run = before_last;                  // (a run that holds the goal weighs something: the last seen)
+                before_run = before_last;                  // (the last seen, be it the one that holds the goal or not)
                 target = goal;
             }
             if (owner < 0 && lane == 0) the_run = -1;

@@ -115,6 +115,18 @@ def test_equal_logits_ties_and_the_ends_of_the_unit_interval():
     assert (check(c)[0][:, 0] == 0).all()
 
 
+def test_a_goal_between_two_roundings_of_one_sum_draws_no_masked_token():
+    """With a, b, c the weights e^l of the first three tokens that have any, (b + c) + a rounds to the uniform number given and c + (a + b) to the next 64-bit number: the goal lies at
+    the end of the third's share by one order of additions and just below it by another, with a run of masked tokens behind.  The third or the fourth may be drawn, nothing else."""
+    vocab = 300007                                            # 74 runs of 4,096, two a lane of the draw
+    weighs = [5, 2 * 4096, 4 * 4096 + 77, 9 * 4096 + 9, vocab - 1]
+    logits = np.full((1, vocab), -np.inf, dtype=np.float32)
+    logits[0, weighs] = [-40.48126220703125, -40.11710739135742, -40.94380187988281, -40.5, 0.0]
+    tokens, counts = run(dict(logits=logits, drafts=np.zeros((1, 0), np.int32), temperature=np.ones(1, np.float32), uniform=np.array([[8.057590335116807e-18]], np.float32),
+                              draft_logits=None, n_drafts=None, first_row=None))
+    assert counts[0] == 1 and tokens[0, 0] in weighs[2:4]
+
+
 def test_masked_rows_infinities_and_nan():
     c = case(9, 3, 4200, seed=7)
     first = c["first_row"]
