@@ -27,7 +27,7 @@ class GenerateResult:
     prefill_ms: float = 0.0          # the prompt, including the sampling of the first new token
     decode_ms: float = 0.0
     decode_steps: int = 0
-    drafted_tokens: int = 0          # tokens that a drafter proposed, and how many of them stayed
+    drafted_tokens: int = 0          # tokens that a drafter proposed, and how many of the generated ones are such
     kept_tokens: int = 0
 
 
@@ -190,7 +190,6 @@ def generate_with_drafts(runner: Runner, drafter: Runner, sampler: Sampler, prom
                 else:
                     new = verify_rows(logits, proposals[:, :k].contiguous(), [sampler], beside)[0]
                 result.drafted_tokens += k
-                result.kept_tokens += len(new) - 1
                 if not result.generated_tokens:
                     t_first = time.perf_counter()
                     result.prefill_ms = (t_first - t_start) * 1e3
@@ -199,9 +198,10 @@ def generate_with_drafts(runner: Runner, drafter: Runner, sampler: Sampler, prom
                 pos += len(new)
                 runner.truncate(request, pos)
                 drafter.truncate(request, min(drafter.cache.length(request), pos))
-                for token in new:
+                for i, token in enumerate(new):
                     tokens.append(int(token))
                     result.generated_tokens.append(int(token))
+                    result.kept_tokens += i + 1 < len(new)                # (the last is the target's own; drafts behind an end token are not taken)
                     if token in end_tokens:
                         result.stopped_by_end_token = True
                         break

@@ -72,6 +72,16 @@ def test_an_end_token_stops_and_is_kept():
         assert got.generated_tokens == want[:first + 1] and got.stopped_by_end_token and seen == want[:first]
 
 
+def test_drafts_behind_an_end_token_are_not_counted_as_kept():
+    """An agreeing drafter, steps of five tokens of which the fifth is the target's own."""
+    want = generate(Runner(), Sampler(SamplerConfig(0.0), VOCAB), PROMPT, 60, sample=host_sample_row).generated_tokens
+    for at, kept in ((0, 1), (1, 2), (3, 4), (4, 4), (5, 5), (11, 10)):
+        if want[at] in want[:at]:
+            continue
+        got = run(Runner(), Runner(), SamplerConfig(0.0), PROMPT, 4, 60, end=[want[at]])
+        assert got.generated_tokens == want[:at + 1] and got.kept_tokens == kept and got.drafted_tokens == 4 * (at // 5 + 1)
+
+
 def test_a_drafter_that_agrees_is_believed_at_any_temperature():
     """Equal distributions: every draft stays, so a step brings n_drafts + 1 tokens."""
     target = Runner()
