@@ -152,8 +152,7 @@ def generate_with_drafts(runner: Runner, drafter: Runner, sampler: Sampler, prom
             proposals = torch.zeros((1, max(most, 1)), dtype=torch.int32, device=getattr(drafter.model, "device", "cpu"))
             rows = None
             while pos < steps:
-                k = max(0, min(most, steps - pos - 1, drafter.max_positions - pos))
-                drafts: List[int] = []
+                k, made = max(0, min(most, steps - pos - 1, drafter.max_positions - pos)), 0
                 if k:
                     try:
                         # what the drafter has not seen (the last token, and the one before where all of its proposals stayed), then one proposal after the other
@@ -161,20 +160,21 @@ def generate_with_drafts(runner: Runner, drafter: Runner, sampler: Sampler, prom
                         logits = drafter.step([StepEntry(request, [tokens[pos]], (0,))])
                         if rows is None and not filtered and not sampler.config.greedy:
                             rows = torch.empty((1, most, vocab), dtype=torch.float32, device=logits.device)
-                        for j in range(k):
+                        while True:
                             if rows is not None:
-                                rows[0, j].copy_(logits[0])
+                                rows[0, made].copy_(logits[0])
                             token = sample_rows_on_device(logits, [own]) if draft is None else torch.tensor([draft(logits[0], own)], dtype=torch.int32)
-                            proposals[0, j:j + 1].copy_(token)
-                            if j + 1 == k:
+                            proposals[0, made:made + 1].copy_(token)
+                            made += 1
+                            if made == k:
                                 break
                             if getattr(drafter, "can_step_from_device", False):           # (the host need not know the proposal to have the next one made)
                                 logits = drafter.step_from_device([request], token)
                             else:
                                 logits = drafter.step([StepEntry(request, [int(token[0])], (0,))])
-                        drafts = proposals[0, :k].tolist()
-                    except OutOfPages:                        # (what has been proposed so far is lost)
-                        k, drafts = 0, []
+                    except OutOfPages:                        # what has been proposed so far is judged
+                        pass
+                k, drafts = made, proposals[0, :made].tolist()
                 try:
                     logits = runner.step([StepEntry(request, [tokens[pos]] + drafts, tuple(range(k + 1)))])
                 except OutOfPages:

@@ -119,6 +119,20 @@ def test_small_pools_and_contexts():
     assert target.cache.free_pages() == [3] and drafter.cache.free_pages() == [64]
 
 
+@pytest.mark.parametrize("config", [SamplerConfig(0.0), SamplerConfig(1.3, seed=9), SamplerConfig(0.9, top_k=6, seed=4)])
+def test_what_was_proposed_before_the_drafters_pool_ran_out_is_judged(config):
+    """12 positions: behind the prompt's 4 and the last token four proposals, then from position 9 three more; from position 12 on there is room for none."""
+    target = Runner()
+    got = run(target, Runner(n_pages=3), config, PROMPT, 4, 30)
+    alone = run(Runner(), Runner(), config, PROMPT, 4, 30)
+    proposed = [entries[0][1] - 1 for entries in target.log if entries[0][2]]
+    assert len(got.generated_tokens) == 26 and got.drafted_tokens == sum(proposed) > 0 and proposed[0] == 4
+    if config.greedy or config.top_k == 0:                    # an agreeing drafter: all stay
+        assert proposed[:3] == [4, 3, 0] and got.kept_tokens == got.drafted_tokens == 7
+    if config.greedy or config.top_k:
+        assert got.generated_tokens == alone.generated_tokens
+
+
 def test_refusals():
     target, sampler = Runner(), Sampler(SamplerConfig(0.0), VOCAB)
     with pytest.raises(ValueError, match="no tokens"):
