@@ -110,7 +110,7 @@ def generate_with_drafts(runner: Runner, drafter: Runner, sampler: Sampler, prom
     brings the logits at all their places, and of the proposals as many stay as leave the sequence distributed as the target's own
     (`sampling.verify_rows`; a greedy sampler's tokens are `generate`'s, and so are those of one with top-k or top-p, whose proposals stay where they are what its own draw gives:
     all but for the rounding of bfloat16 products, which add up in another order for several rows than for one).
-    What was fed beyond is cut off again, so neither model may keep a state or give pages back behind a window.
+    What was fed beyond is cut off again, so neither model may keep a state or give pages back behind a window.  Both lie on one device.
     The drafter draws at the sampler's settings from numbers of its own.  draft(logits, sampler) -> token and judge(logits, drafts, sampler, draft_logits) -> new tokens replace the device's
     (tests without a GPU use them)."""
     import torch
@@ -122,6 +122,9 @@ def generate_with_drafts(runner: Runner, drafter: Runner, sampler: Sampler, prom
     vocab = runner.model.spec.vocab_size
     if drafter is runner or drafter.model.spec.vocab_size != vocab:
         raise ValueError("generate: the drafter must be another runner whose model has the same vocabulary")
+    places = [torch.device(getattr(r.model, "device", "cpu")) for r in (runner, drafter)]
+    if places[0] != places[1]:
+        raise ValueError(f"generate: the target lies on {places[0]} and the drafter on {places[1]}; drafts are judged where both models' logits lie")
     for r, what in ((runner, "target"), (drafter, "drafter")):
         if not r.cache.rewinds:
             raise ValueError(f"generate: the {what} keeps a state or gives pages back; drafts that fall could not be taken back")

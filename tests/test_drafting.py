@@ -158,6 +158,15 @@ def test_refusals():
         generate_with_drafts(target, Runner(max_positions=4), sampler, PROMPT)
 
 
+def test_models_on_two_devices_are_refused_before_anything_runs():
+    target, drafter = Runner(), Runner()
+    for r, device in ((target, "cuda:0"), (drafter, "cuda:1")):
+        r.model = SimpleNamespace(spec=SimpleNamespace(vocab_size=VOCAB), device=torch.device(device))
+    with pytest.raises(ValueError, match="lies on cuda:0 and the drafter on cuda:1"):
+        generate_with_drafts(target, drafter, Sampler(SamplerConfig(0.0), VOCAB), PROMPT)
+    assert not target.log and not drafter.log and not target.fed
+
+
 def test_verify_rows_refuses():
     plain, drafts, logits = Sampler(SamplerConfig(1.0), VOCAB), torch.zeros((2, 3), dtype=torch.int32), torch.zeros(8, VOCAB)
     with pytest.raises(ValueError, match="samplers"):
