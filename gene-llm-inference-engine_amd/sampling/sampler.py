@@ -124,7 +124,8 @@ _KIND_ORDER = {"greedy": 0, "plain": 1, "filtered": 2}
 class _Staging:
     """The rows' parameters go to the device through pinned memory with a copy that does not wait.  (A copy from ordinary
     memory makes the host wait until the device has reached it, that is until the step before it has run: the host could then
-    queue nothing ahead.)  A ring of buffers; one is taken again only after its last copy has finished."""
+    queue nothing ahead.)  A ring of buffers; one is taken again only after its last copy has finished, and is made larger
+    where it does not hold what is asked for."""
     DEPTH, FLOATS = 8, 5 * 1024
 
     def __init__(self, device):
@@ -134,13 +135,13 @@ class _Staging:
         self.turn = 0
 
     def upload(self, values: np.ndarray) -> torch.Tensor:
-        if values.size > self.FLOATS:
-            return torch.from_numpy(values).to(self.device)
         self.turn = (self.turn + 1) % self.DEPTH
         if self.done[self.turn] is None:
             self.done[self.turn] = torch.cuda.Event()
         else:
             self.done[self.turn].synchronize()
+        if values.size > self.host[self.turn].numel():
+            self.host[self.turn] = torch.empty(1 << (values.size - 1).bit_length(), dtype=torch.float32, pin_memory=True)
         staged = self.host[self.turn][:values.size].view(values.shape)
         staged.copy_(torch.from_numpy(values))
         out = torch.empty(values.shape, dtype=torch.float32, device=self.device)

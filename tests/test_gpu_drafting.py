@@ -93,6 +93,26 @@ def test_verify_rows_of_many_requests(folders):
     assert verify_rows(logits, drafts.to("cuda:0"), make(), n_drafts=counts) == [row[:c].tolist() for row, c in zip(tokens, n)]
 
 
+def test_the_numbers_of_many_requests_do_not_wait_for_the_device():
+    """600 requests bring 6,600 numbers.  The device has some hundreds of milliseconds of products before it; the call returns while they run, whichever buffers it takes."""
+    from geneinfer_amd.sampling import Sampler, SamplerConfig, verify_rows_on_device
+    n, k, vocab = 600, 7, 64
+    logits, drafts = torch.randn(n * (k + 1), vocab, device="cuda:0"), torch.zeros((n, k), dtype=torch.int32, device="cuda:0")
+    samplers = [[Sampler(SamplerConfig(1.0, seed=i), vocab) for i in range(n)] for _ in range(3)]
+    want = verify_rows_on_device(logits, drafts, samplers[0])                     # (the library and its memory are there from now on)
+    a = torch.randn(8192, 8192, device="cuda:0", dtype=torch.bfloat16)
+    b = a @ a
+    torch.cuda.synchronize()
+    for _ in range(400):
+        torch.mm(a, a, out=b)
+    busy = torch.cuda.Event()
+    busy.record()
+    got = [verify_rows_on_device(logits, drafts, s) for s in samplers[1:]]
+    assert not busy.query()
+    for tokens, counts in got:
+        assert torch.equal(tokens, want[0]) and torch.equal(counts, want[1])
+
+
 def test_a_model_with_memories_is_refused(folders):
     import geneinfer_amd as gi
     target = llm(folders["target"])
