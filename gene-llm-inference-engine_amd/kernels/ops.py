@@ -2292,7 +2292,7 @@ def adapters_add(x, a, b, ids, out, scales=None, base=None, slices=None, checked
         return out
     x_code, w_code, n_slices = _CODE[x.dtype], _CODE[a.dtype], len(slices)
     scratch = torch.empty(_adapter_scratch(x_code, w_code, n, width, rank, n_slices), dtype=torch.float32, device=x.device)
-    base_row, out_row = base.stride(0), out.stride(0)
+    base_row, out_row = (base.stride(0), out.stride(0)) if n > 1 else (columns, columns)         # (a single row is apart from none)
     _call("gi_adapters_add", x.data_ptr(), x_code, max(x.stride(0), width), a.data_ptr(), b.data_ptr(), w_code, ids.data_ptr(), _ptr(scales), base.data_ptr(), _CODE[base.dtype],
           max(base_row, columns), out.data_ptr(), _CODE[out.dtype], max(out_row, columns), scratch.data_ptr(), n, width, columns, rank, n_slices, _adapter_slices(slices),
           n_adapters, _stream())

@@ -209,6 +209,19 @@ def test_strides_and_places(dtype):
         assert_right(run(dict(c, base=base)), c)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_a_single_row_of_a_buffer_whose_rows_are_far_apart(dtype):
+    """Rows may be at most 2^23 numbers apart; one row is apart from none."""
+    c = make(1, 128, 96, 16, 3, dtype=dtype, ids=1)
+    apart = 2 ** 23 + 64
+    out, base = torch.zeros((2, apart), device=DEV)[1:, 7:103], torch.zeros((2, apart), device=DEV)[1:, 1:97]
+    base.copy_(c["base"])
+    assert_right(ops().adapters_add(c["x"], c["a"], c["b"], c["ids"], out, scales=c["scales"], base=base), c)
+    two = make(2, 128, 96, 16, 3, dtype=dtype, ids=1)
+    with pytest.raises(ops().KernelError, match="numbers apart"):
+        ops().adapters_add(two["x"], two["a"], two["b"], two["ids"], torch.zeros((2, apart), device=DEV)[:, :96], scales=two["scales"], base=two["base"])
+
+
 def test_captured_and_replayed_with_other_requests():
     for n in (6, 140, 600):
         cs = [make(n, 512, 640, 16, 4, seed=s, ids="runs") for s in range(3)]
