@@ -2182,8 +2182,8 @@ def verify_drafts(logits, drafts, temperature, uniform, tokens, counts, draft_lo
 
     tokens, int32 [requests, K + 1], receives the drafts that stay, the token behind them and then -1; counts, int32 [requests], how many tokens those are.
     A draft x stays if those before it do and u q(x) < p(x) (arg max: if it is the row's lowest arg max); the token behind is drawn in index order
-    from max(p - q, 0) where a draft fell (from p, where less than 1e-12 of that is left: a draft outside the vocabulary may fall with q equal to p) and from p where none did.  Logits of -infinity or NaN are no tokens (a row of nothing else lets no draft stay and gives token
-    0), a draft outside the vocabulary falls.  A request whose rows do not lie among those given gets count 0.  At most VERIFY_MAX_DRAFTS drafts a request, 65,535 requests and 4,194,304 tokens."""
+    from max(p - q, 0) where a draft fell (from p, where less than 1e-12 of that is left: a draft outside the vocabulary may fall with q equal to p) and from p where none did.  Logits of -infinity or NaN are no tokens: a row of nothing else lets no draft stay and gives token
+    0; the arg max of such a row is token 0 (as `argmax` has it), and a draft of 0 stays there.  A draft outside the vocabulary falls.  A request whose rows do not lie among those given gets count 0.  At most VERIFY_MAX_DRAFTS drafts a request, 65,535 requests and 4,194,304 tokens."""
     what = "verify_drafts"
     f32, i32 = torch.float32, torch.int32
     if not (logits.dtype == f32 and logits.dim() == 2 and logits.shape[1] > 0 and (logits.stride(1) == 1 or logits.shape[1] == 1)):

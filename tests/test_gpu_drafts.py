@@ -151,6 +151,19 @@ def test_masked_rows_infinities_and_nan():
     check(c)
 
 
+def test_rows_without_a_token():
+    """At a temperature no draft stays and the token is 0; the arg max of such a row is 0, as without drafts, so a draft of 0 stays and the next row is asked."""
+    from geneinfer_amd.kernels import ops as o
+    c = case(2, 2, 500, drafter=False, seed=15)
+    c["logits"][[0, 1]], c["logits"][3] = -np.inf, np.nan
+    c["logits"][[2, 4], 77], c["drafts"][:] = 40.0, [[0, 0], [5, 0]]
+    assert check(c)[0].tolist() == [[0, -1, -1], [0, -1, -1]]
+    c["temperature"][:] = 0.0
+    assert check(c)[0].tolist() == [[0, 0, 77], [0, -1, -1]]
+    alone = torch.empty(6, dtype=torch.int32, device=DEV)
+    assert o.argmax(on_device(np.where(np.isnan(c["logits"]), -np.inf, c["logits"]).astype(np.float32)), alone)[:5].tolist() == [0, 0, 77, 0, 77]
+
+
 @pytest.mark.parametrize("drafter", [True, False])
 def test_drafts_outside_the_vocabulary_fall(drafter):
     c = case(4, 3, 777, drafter=drafter, seed=8, noise=0.0)
