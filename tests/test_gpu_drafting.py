@@ -123,3 +123,19 @@ def test_a_model_with_memories_is_refused(folders):
     recurrent = gi.LLM(gi.random_model(config, 0), max_tokens=64, max_running=2)
     with pytest.raises(ValueError):
         target.generate(prompt(4), steps=9, drafter=recurrent)
+
+
+def test_real_models_with_memories_are_refused_on_either_side(folders):
+    """Of one vocabulary, so that the memories are what is refused."""
+    import json
+    from pathlib import Path
+    import geneinfer_amd as gi
+    from geneinfer_amd.config import parse_config
+    target = llm(folders["target"])
+    config = json.loads((Path(__file__).resolve().parent.parent / "configs" / "fekorax-small.json").read_text())
+    config["vocab"] = target.model.spec.vocab_size
+    recurrent = gi.LLM(gi.random_model(parse_config(config), 0), max_tokens=64, max_running=2)
+    with pytest.raises(ValueError, match="the drafter keeps a state or gives pages back; .* taken back"):
+        target.generate(prompt(4), steps=9, drafter=recurrent)
+    with pytest.raises(ValueError, match="the target keeps a state or gives pages back; .* taken back"):
+        recurrent.generate(prompt(4), steps=9, drafter=target)
