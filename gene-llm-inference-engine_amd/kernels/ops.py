@@ -2270,6 +2270,8 @@ def adapters_check(x, a, b, ids, out, scales, base, slices):
                 raise KernelError(f"{what}: {name} must have unit inner stride and rows that do not overlap")
     if base is not out and n and base.data_ptr() == out.data_ptr() and not (base.dtype == out.dtype and (n == 1 or base.stride(0) == out.stride(0))):
         raise KernelError(f"{what}: base and out begin at the same place, but their rows or dtypes differ")
+    if n and x.data_ptr() == out.data_ptr():
+        raise KernelError(f"{what}: x and out begin at the same place; a row's result may be stored while its numbers are still read")
     if n:
         _here(what, x, a, b, ids, out, scales, base)
     return slices

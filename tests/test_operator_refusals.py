@@ -56,6 +56,15 @@ def test_base_and_out_at_one_place_must_be_the_same():
             ops.adapters_add(**{**args, "base": base, "out": out})
 
 
+def test_x_and_out_at_one_place():
+    args = adapter_args(columns=16)
+    with pytest.raises(ops.KernelError, match="x and out begin at the same place"):
+        ops.adapters_add(**{**args, "out": args["x"]})
+    room = torch.zeros(5, 32)                                 # beside one another in one buffer they share nothing
+    with pytest.raises(ops.KernelError, match="device memory"):
+        ops.adapters_add(**{**args, "x": room[:, :16], "out": room[:, 16:]})
+
+
 def test_adapters_of_no_rows_change_nothing():
     args = adapter_args(n=0)
     assert ops.adapters_add(**args) is args["out"]
