@@ -495,7 +495,8 @@ __host__ __device__ inline int strip_bits(int n_tiles, int columns) {          /
 // N's: number n of the four products of a step has columns 4 l + n, l = 0 .. 15, so that a lane ends with four neighbours and sixteen lanes with whole lines of base and out.  As on the way down no
 // row's values meet another's.  FOURS: a projection has four columns or more, so base and out come four at a time.  AT_ONCE: numbers of B that one load brings.  KS: runs of ranks that a wave keeps; 0 for any number,
 // loaded again for every 16 rows (8,192 rows of 14,336 columns, rank 16: 239 us kept, 272 loaded again).  LOW_BASE, LOW_OUT: of aligned ones whether they are bfloat16 (a branch on it where they are loaded would have every load waited for); `io` says it of others.
-// 4,096 rows of 4,096 32-bit columns, rank 64: 41 us for the 134 MB of base and out (a copy of as much takes 25); 531 of 6,144, rank 24, onto bfloat16 10.3; 2,048 of 2,048, rank 32, 9.4; 301 of 2,048 in 32 bits,
+// 4,096 rows of 4,096 32-bit columns, rank 64: 41 us for the 134 MB of base and out (a copy of as much takes 25; every one of a tile's eight strips adds up its rows' sums over the segments anew, 25 MB in all,
+// before its first product, with one step's base under way beside it: no more is known of the difference); 531 of 6,144, rank 24, onto bfloat16 10.3; 2,048 of 2,048, rank 32, 9.4; 301 of 2,048 in 32 bits,
 // rank 10, 8.4.  Asking for a whole tile's base at once instead of 16 rows ahead makes it no faster: 4,096 rows of 4,096 both ways 50 us instead of 47, with 256 registers instead of 141.
 template <bool LOW, typename W, bool FOURS, int AT_ONCE, int KS, bool LOW_BASE, bool LOW_OUT>
 __global__ __launch_bounds__(UP_NT) void adapters_up_kernel(const float* __restrict__ sums, const W* __restrict__ b, const float* __restrict__ scales, const Tile* __restrict__ list,
@@ -926,6 +927,9 @@ int up(const Call& c) {
     // What a wave keeps of B it has for all rows of a tile: of four runs that pays where it takes them all (8,192 rows of 14,336 columns, rank 128: 309 us both ways instead of 526; 4,096 of 4,096, rank 96, 58 instead
     // of 68), not where the waves share the rows out (600 of 4,096, rank 128: 43 us instead of 32; 1,024 of 2,048 in 32 bits, rank 64, 28 instead of 26).
     const bool keeps_four = steps <= 4 && strip_bits((int)usual_tiles(c.n_rows), c.columns) > 6;       // (then the strips there are, of at least as many tiles, are no shorter)
+    // B's rows begin at whole loads only where the rank is a multiple of one, so of other ranks B comes in halves of a run or number by number, and again for every 16 rows once a run of ranks does not hold
+    // them.  2,048 rows of 4,096 onto 4,096, both ways: bfloat16, rank 31, 32: 31 and 26 us; 33, 36, 40: 57, 34 and 30; 50, 56: 67 and 30; 32 bits, rank 10, 16: 29 and 26 us; 33, 36: 66 and 40; 50, 56: 102 and 44.
+    // (An adapter filled up with zeros to the next multiple of 8 gives the same numbers at that rank's time.)
     constexpr int RUN = Piece<LOW>::RUN;
     if (!c.fours) return up_launch<LOW, W, false, 1, 0, false, false>(c);
     if (c.rank % RUN == 0 && aligned(c.b, RUN * sizeof(W)))

@@ -8,12 +8,16 @@
 // distribution in index order: the first token whose running sum is greater than u_K times the whole.
 //
 // A running sum over a hundred thousand tokens is compared with a number that falls anywhere between: in 32 bits one draw in some thousands
-// comes out a token off.  So weights exp((l - max) / T) and all sums are held in 64 bits, which this chip computes at the rate of 32.
+// comes out a token off.  So weights exp((l - max) / T) are made and added up in 64-bit arithmetic, which this chip does at the rate of 32; of
+// a weight's bits 39 are good (2e-12 relative), a running sum keeps what its additions leave.
 //
-// Three launches.  All rows once, in runs of 4,096 logits: the runs' maxima and sums.  Then, per request and run, the verdict (every workgroup of a request comes to it by itself, from the runs' numbers) and,
-// where a draft fell, the run's share of what is drawn from.  Then a request's draw.  What bounds them: of many rows the logits' bytes and, as much, the weights' instructions (64 requests, 401 rows of 128,256
-// tokens, 206 MB: 49 + 20 + 8 us); of a few the waits that follow one another (one request with 4 drafts, 9 such rows: 4.5 + 7.0 + 6.1 us).  A last workgroup that draws by itself instead of a third launch has
-// to see what the others wrote: with the fences for that one request took 29.7 us instead of 20.5, 64 took 121 instead of 81.
+// Three launches.  All rows once, in runs of 4,096 logits: the runs' maxima and sums.  Then, per request and run, the verdict (every
+// workgroup of a request comes to it by itself, from the runs' numbers) and, where a draft fell, the run's share of what is drawn from.
+// Then a request's draw.  What bounds them: of many rows the logits' bytes and, as much, the weights' instructions (64 requests, 401 rows of
+// 128,256 tokens, 206 MB: 49 + 20 + 8 us); of a few the waits that follow one another (one request with 4 drafts, 9 such rows: 4.5 + 7.0 +
+// 6.1 us).  A last workgroup that draws by itself instead of a third launch has to see what the others wrote: with fences, which write caches
+// back, one request took 29.7 us instead of 20.5, 64 took 121 instead of 81.  (Stores past the caches and a relaxed counter, as the matrix
+// products' workgroups meet, were not tried here.)
 #include "common.h"
 #include "lanes.h"
 
@@ -57,9 +61,12 @@ __device__ __forceinline__ int drafts_of(const Inputs& in, int r, long& first) {
 
 __device__ __forceinline__ float number(float v) { return v == v ? v : -INFINITY; }        // (what is no number is no token)
 
-// Weights exp((l - top) / T) of a row whose largest logit is `top`: 1 for the largest, 0 for what is no token (-infinity, NaN) and below 2^-1020.  With m = (l - top) log2(e) / T, n the nearest integer (what is left in
-// the low bits of a sum with 1.5 * 2^52) and f = m - n, 2^m is 2^n (1 + f q(f)), q the polynomial through (2^f - 1) / f at eight Chebyshev points of [-1/2, 1/2]: off by 2e-12 relative, less than a draw over a
-// million tokens can notice.  No scaling by an instruction of its own: those, as conversions, run at a quarter of the rate, and instructions are what bounds a sum over many rows (four fifths of the cycles one; a polynomial of nine points and a product of its own for m: 55 us for 401 rows of 128,256 tokens that took 51 so). of nine points and a product of its own for m: 55 us for 401 rows of 128,256 tokens that now take 51).
+// Weights exp((l - top) / T) of a row whose largest logit is `top`: 1 for the largest, 0 for what is no token (-infinity, NaN) and below
+// 2^-1020.  With m = (l - top) log2(e) / T, n the nearest integer (what is left in the low bits of a sum with 1.5 * 2^52) and f = m - n, 2^m
+// is 2^n (1 + f q(f)), q the polynomial through (2^f - 1) / f at eight Chebyshev points of [-1/2, 1/2]: off by 2e-12 relative, less than a
+// draw over a million tokens can notice.  No scaling by an instruction of its own: those, as conversions, run at a quarter of the rate, and
+// instructions are what bounds a sum over many rows (a vector instruction in four fifths of the cycles).  A polynomial of nine points (4e-14)
+// with a product of its own for m takes 55 us for 401 rows of 128,256 tokens that take 51 so.
 __device__ __forceinline__ double horner(double f, double q, double c) {        // f q + c, the coefficient in scalar registers: as the accumulator it would be moved there for every step
     double out;
     asm("v_fma_f64 %0, %1, %2, %3" : "=v"(out) : "v"(f), "v"(q), "s"(c));
@@ -216,9 +223,11 @@ struct Drawn {
     }
 };
 
-// Which drafts stay, and the sums over runs of what is drawn from, where the parts do not hold them already: every run of a request whose drafter's row is taken off, and the run that a draft is
-// left out of.  Workgroup (run, request); run 0's writes what the request has so far.  7.0 us for one request with 4 drafts, 20 for 64 with up to 7, which read two rows of 128,256 again
-// each (58 MB), once the verdict says which: its waits (6 us) have nothing beside them.
+// Which drafts stay, and the sums over runs of what is drawn from, where the parts do not hold them already: every run of a request whose
+// drafter's row is taken off, and the run that a draft is left out of.  Workgroup (run, request); run 0's writes what the request has so far.
+// 7.0 us for one request with 4 drafts, 20 for 64 with up to 7, which read two rows of 128,256 again each (58 MB), once the verdict says
+// which: its waits (6 us) have nothing beside them, and of the 2,048 workgroups of 256 threads 1,280 fit at once (81 registers, five a compute
+// unit), so the rest come to their verdict, and wait, after these.
 template <int NT>
 __global__ __launch_bounds__(NT) void judge_kernel(Inputs in, const float* __restrict__ part_m, const int* __restrict__ part_i, const double* __restrict__ part_s, Verdict* __restrict__ verdicts,
                                                    double* __restrict__ rest, int* __restrict__ tokens, int* __restrict__ counts) {
